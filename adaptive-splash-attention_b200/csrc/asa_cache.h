@@ -1,0 +1,65 @@
+// asa_cache.h -- launch-side declarations of the 4-bit paged key/value cache's
+// kernels (asa_cache_*.cu), and the layout both sides share.  Not part of the
+// public ABI; include/asa.h describes the formats.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "../../include/asa.h"
+
+namespace asa {
+
+void note_launch(int n = 1);
+int* device_error_word();              // asa_capi.cu
+int cuda_status_of(cudaError_t e);
+void* profile_open(const char* label, cudaStream_t st);
+void profile_close(void* scope);
+
+namespace cache {
+
+constexpr int kBlock = 16;       // tokens of a block: the unit a record is laid out in
+constexpr int kGroup = 32;       // channels that share a scale and an offset
+constexpr float kF16Max = 65504.0f;
+// The formats multiply by the nearest fp32 numbers to 1/15 and 1/127.
+constexpr float kFifteenth = 1.0f / 15.0f;
+constexpr float k127th = 1.0f / 127.0f;
+
+// One call's sizes, checked on the host.
+struct Shape {
+    int B, T, HQ, H, G, d, P;        // G = HQ / H query heads a key head; P tokens a page
+    int pages, width;                // the pool's pages; entries of a block table row
+    int dtype;
+    float scale, alpha;
+    long long spins;
+    int64_t rec;                     // bytes of one page's record of one key head
+};
+
+__host__ __device__ constexpr int row_bytes(int d) { return d / 2; }
+__host__ __device__ constexpr int par_bytes(int d) { return d / 8; }             // 2 * d/32 fp16
+__host__ __device__ constexpr int block_bytes(int d) { return kBlock * (row_bytes(d) + par_bytes(d)); }
+__host__ __device__ constexpr int64_t record_bytes(int d, int P) { return 2ll * (P / kBlock) * block_bytes(d); }
+__host__ __device__ constexpr int bounds_bytes(int d) { return 2 * d + ASA_CACHE_BOUNDS_PAD; }
+
+struct Strides { int64_t b, t, h; };
+
+cudaError_t write(const Shape& s, const void* K, const void* V, Strides ks, Strides vs, uint8_t* pool,
+                  int8_t* bounds, const int32_t* table, const int32_t* start, const int32_t* count,
+                  int* err, cudaStream_t st);
+cudaError_t read(const Shape& s, const uint8_t* pool, const int32_t* table, const int32_t* start,
+                 const int32_t* count, void* K, void* V, int* err, cudaStream_t st);
+cudaError_t read_bounds(const Shape& s, const int8_t* bounds, const int32_t* pages, int n, float* upper,
+                        float* lower, int* err, cudaStream_t st);
+
+size_t select_workspace(const Shape& s);
+cudaError_t select(const Shape& s, const void* Q, Strides qs, const int8_t* bounds, const int32_t* table,
+                   const int32_t* lengths, int keep, int32_t* pages, void* ws, int* err, cudaStream_t st);
+
+size_t attend_workspace(const Shape& s, int keep);
+cudaError_t attend(const Shape& s, const void* Q, Strides qs, const uint8_t* pool, const int32_t* table,
+                   const int32_t* lengths, const int32_t* list, int keep, void* O, void* ws, int* err,
+                   cudaStream_t st);
+
+}  // namespace cache
+}  // namespace asa

@@ -10,6 +10,7 @@
 #include "asa_sm100.cuh"
 #include <atomic>
 #include <mutex>
+#include <new>
 #include <climits>
 #include <cmath>
 #include <cstring>
@@ -220,6 +221,16 @@ int cuda_status(cudaError_t e) {
 }
 
 }  // namespace
+
+// The same services for the cache's entry points (asa_cache_capi.cu).
+namespace asa {
+int* device_error_word() { return error_word(); }
+int cuda_status_of(cudaError_t e) { return cuda_status(e); }
+void* profile_open(const char* label, cudaStream_t st) {
+    return g_prof.on ? new (std::nothrow) ProfScope(label, st) : nullptr;
+}
+void profile_close(void* scope) { delete static_cast<ProfScope*>(scope); }
+}  // namespace asa
 
 extern "C" {
 

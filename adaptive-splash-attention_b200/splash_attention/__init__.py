@@ -13,6 +13,9 @@ Drop-in surface of mvideet/Adaptive-Splash-Attention:
   build settings (BLOCK_M=32, BLOCK_N=64, K_KEEP=8, :8-19) and its host-side
   NaN/Inf scrub.
 
+What the training operators make is served from a 4-bit paged cache: see
+``cache.py`` (``new_cache``, ``cache_write``, ``cache_attention``, ``select_pages``, ...).
+
 Every computation runs in hand-written CUDA kernels for sm_100a behind the C
 ABI of include/asa.h (libasa.so).  There is no CPU fallback.
 """
@@ -34,9 +37,13 @@ if not os.path.exists(_TORCH_OPS):
 torch.ops.load_library(_TORCH_OPS)
 _ops = torch.ops.splash_attention
 
+from .cache import KVCache, new_cache, cache_write, cache_read, cache_bounds, select_pages, \
+    cache_attention  # noqa: E402  (its operators are in the library loaded above)
+
 __all__ = ["AdaptiveSplashAttention", "splash_attention", "forward", "backward", "tau_mask",
            "Settings", "device_error", "forward_backward_host", "stable_attention", "stable_forward",
-           "stable_backward"]
+           "stable_backward", "KVCache", "new_cache", "cache_write", "cache_read", "cache_bounds",
+           "select_pages", "cache_attention"]
 
 # Reference compile-time defaults (adasplashattention.cu:8-19).
 REF_BLOCK_M, REF_BLOCK_N, REF_K_KEEP = 32, 64, 8

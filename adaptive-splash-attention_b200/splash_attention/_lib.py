@@ -24,7 +24,9 @@ SYMBOLS = ("asa_params_default", "asa_workspace_bytes", "asa_resolve_backend", "
            "asa_version", "asa_profile_begin", "asa_profile_end", "asa_profile_get",
            "asa_launch_count", "asa_last_cuda_error", "asa_tau_mask_noalloc",
            "asa_device_error_async", "asa_wait_probe", "asa_stable_workspace_bytes",
-           "asa_stable_forward", "asa_stable_backward")
+           "asa_stable_forward", "asa_stable_backward", "asa_cache_record_bytes",
+           "asa_cache_workspace_bytes", "asa_cache_write", "asa_cache_read", "asa_cache_bounds",
+           "asa_cache_select", "asa_cache_attention")
 NOALLOC_SCRATCH_BYTES = 1 << 20
 
 
@@ -39,6 +41,15 @@ class Params(ctypes.Structure):
                 ("timeout_spins", ctypes.c_longlong), ("ref_tile_load", ctypes.c_int),
                 ("tau_mode", ctypes.c_int), ("grad_mode", ctypes.c_int),
                 ("fused_forward", ctypes.c_int)]
+
+
+class CacheParams(ctypes.Structure):
+    """Mirror of struct asa_cache_params (include/asa.h)."""
+    _fields_ = [("B", ctypes.c_int), ("T", ctypes.c_int), ("heads", ctypes.c_int),
+                ("kv_heads", ctypes.c_int), ("d", ctypes.c_int), ("page_size", ctypes.c_int),
+                ("num_pages", ctypes.c_int), ("table_width", ctypes.c_int),
+                ("dtype", ctypes.c_int), ("sm_scale", ctypes.c_float), ("alpha", ctypes.c_float),
+                ("timeout_spins", ctypes.c_longlong)]
 
 
 class AsaError(RuntimeError):
@@ -90,6 +101,15 @@ def lib():
         L.asa_stable_workspace_bytes.argtypes = [pp, ctypes.POINTER(sz), ctypes.POINTER(sz)]
         L.asa_stable_forward.argtypes = [pp] + [vp] * 11 + [vp, sz, vp]
         L.asa_stable_backward.argtypes = [pp] + [vp] * 12 + [vp, sz, vp]
+        cp, i64x3 = ctypes.POINTER(CacheParams), ctypes.POINTER(ctypes.c_int64)
+        L.asa_cache_record_bytes.argtypes = [ctypes.c_int, ctypes.c_int]
+        L.asa_cache_record_bytes.restype = ctypes.c_longlong
+        L.asa_cache_workspace_bytes.argtypes = [cp, ctypes.c_int, ctypes.POINTER(sz), ctypes.POINTER(sz)]
+        L.asa_cache_write.argtypes = [cp, vp, vp, i64x3, i64x3, vp, vp, vp, vp, vp, vp]
+        L.asa_cache_read.argtypes = [cp, vp, vp, vp, vp, vp, vp, vp]
+        L.asa_cache_bounds.argtypes = [cp, vp, vp, ctypes.c_int, vp, vp, vp]
+        L.asa_cache_select.argtypes = [cp, vp, i64x3, vp, vp, vp, ctypes.c_int, vp, vp, sz, vp]
+        L.asa_cache_attention.argtypes = [cp, vp, i64x3, vp, vp, vp, vp, ctypes.c_int, vp, vp, sz, vp]
         L.asa_last_cuda_error.argtypes = []
         L.asa_last_cuda_error.restype = ctypes.c_char_p
         for name in SYMBOLS:

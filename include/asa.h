@@ -200,6 +200,103 @@ int asa_stable_backward(const asa_params* p, const void* Q, const void* K, const
                         const float* tau, const float* tau_coef, const void* dO, void* dQ,
                         void* dK, void* dV, void* ws, size_t ws_bytes, asa_stream_t stream);
 
+/* ---- serving from a 4-bit paged key/value cache ------------------------------
+ * A pool of pages of page_size tokens (16, 32, 64 or 128) holds the keys and
+ * values of every sequence in 4 bits; a block table names each sequence's
+ * pages.  No counterpart in the reference, which has no cache.
+ *
+ *   pool     uint8 [num_pages, kv_heads, asa_cache_record_bytes()]: a record
+ *            holds a page's keys, then its values, each as page_size/16 blocks
+ *            of 16 tokens.  A block holds 16 rows of d/2 bytes of codes, then 16
+ *            rows of 2*d/32 fp16: the scales of the row's d/32 groups of 32
+ *            channels, then their offsets.  A value is offset + code * scale
+ *            (code 0..15), offset = fp16(min), scale = fp16((max - offset) * r)
+ *            with r the fp32 number nearest 1/15, code = rint((x - offset)/scale)
+ *            clipped to 0..15, all in fp32, after x is clipped to +-65504.  A group holding a NaN reads back as NaN.
+ *            A row of codes lists, run by run over the groups, the bytes of a
+ *            run of 8 (keys) or 4 (values) channels: channel c = 32 g + w of a
+ *            key row lies in byte (w/8)*4*(d/32) + 4 g + (w%8)/2, of a value
+ *            row in byte (w/4)*2*(d/32) + 2 g + (w%4)/2; even channels in the
+ *            low four bits.
+ *   bounds   int8 [num_pages, kv_heads, 2 d + 16]: each channel's largest key
+ *            of the page (upper codes, rounded up), its smallest (lower codes,
+ *            rounded down), and the int32 exponent e of their unit 2^e, the
+ *            least with max |key| <= 127 * 2^e (-126 for a page of zeros).  They
+ *            start over when a page's first slot is written, and do not depend
+ *            on how many calls wrote the page.  NaN counts as 0.
+ *   block_table  int32 [B, table_width], the page of each page_size tokens
+ *   start, count, lengths  int32 [B]
+ *
+ * A sequence's positions at or past table_width * page_size, negative ones, and
+ * pages outside the pool are neither read nor written; their keys are not seen.
+ * Reading or writing such a position, or meeting such a page, records
+ * ASA_ERR_INVALID in the device error word (a length past the table's end does
+ * not: the keys there are just not seen).  d: 32, 64, 96 or 128.
+ * pool and bounds must be 16-byte aligned.  Strides are in elements; the
+ * innermost dimension is contiguous. */
+#define ASA_CACHE_BOUNDS_PAD 16
+typedef struct asa_cache_params {
+    int B, T;              /* sequences, and tokens of each in this call         */
+    int heads, kv_heads;   /* query heads (a multiple of kv_heads) and key heads */
+    int d;                 /* head dim                                           */
+    int page_size;         /* tokens a page                                      */
+    int num_pages;         /* pages in the pool                                  */
+    int table_width;       /* entries of a block table row                       */
+    int dtype;             /* asa_dtype of K, V (write, read)                    */
+    float sm_scale;        /* score scale                                        */
+    float alpha;           /* 1: softmax; 1.05..3: alpha-entmax, its scores      */
+                           /* clamped to +-10 as in training                     */
+    long long timeout_spins; /* bound on every device-side wait; 0 = default     */
+} asa_cache_params;
+
+/* Bytes of one page's record of one key head. */
+long long asa_cache_record_bytes(int d, int page_size);
+
+/* Workspace of asa_cache_attention (keep > 0: over that many selected pages)
+ * and of asa_cache_select, in bytes. */
+int asa_cache_workspace_bytes(const asa_cache_params* p, int keep, size_t* attend_bytes,
+                              size_t* select_bytes);
+
+/* Quantises K and V [B, T, kv_heads, d] (bf16 or fp32) into the pool at
+ * positions start[b] .. start[b] + count[b] - 1 (count NULL: T each) and brings
+ * the touched pages' bounds up to date.  No two sequences may write one page. */
+int asa_cache_write(const asa_cache_params* p, const void* K, const void* V,
+                    const int64_t k_strides[3], const int64_t v_strides[3], void* pool,
+                    void* bounds, const int32_t* block_table, const int32_t* start,
+                    const int32_t* count, asa_stream_t stream);
+
+/* Reads positions start[b] + t, t < min(count[b], T), back into contiguous K and V
+ * [B, T, kv_heads, d] (bf16 or fp32); the other rows are zero. */
+int asa_cache_read(const asa_cache_params* p, const void* pool, const int32_t* block_table,
+                   const int32_t* start, const int32_t* count, void* K, void* V,
+                   asa_stream_t stream);
+
+/* The bounds of n pages of the pool as values, upper and lower fp32
+ * [n, kv_heads, d]; zero for ids outside the pool. */
+int asa_cache_bounds(const asa_cache_params* p, const void* bounds, const int32_t* pages, int n,
+                     float* upper, float* lower, asa_stream_t stream);
+
+/* For each query and key head the `keep` pages that score highest, ascending,
+ * -1 behind the last.  Query t of sequence b stands at position
+ * lengths[b] - T + t; its own page is always among them, later ones never.  The
+ * score is max over the group's heads of unit_q * 2^e * sum_c max(n_c upper_c,
+ * n_c lower_c), n = rint(q / unit_q), unit_q = max|q| * r with r the fp32
+ * number nearest 1/127: sums of whole numbers, the same in any order.  Ties go to the lower page; a NaN scores
+ * lowest.  Q [B, T, heads, d] bf16, pages int32 [B, T, kv_heads, keep]. */
+int asa_cache_select(const asa_cache_params* p, const void* Q, const int64_t q_strides[3],
+                     const void* bounds, const int32_t* block_table, const int32_t* lengths,
+                     int keep, int32_t* pages, void* ws, size_t ws_bytes, asa_stream_t stream);
+
+/* Attention of Q [B, T, heads, d] bf16 over the cache: query t of sequence b, at
+ * position lengths[b] - T + t, sees the keys up to its own position -- with
+ * pages (int32 [B, T, kv_heads, keep], no page twice, -1 ignored) only those of
+ * its key head's listed pages.  O contiguous [B, T, heads, d] bf16; rows that
+ * see no key are zero, rows of a query holding a NaN or an infinity NaN. */
+int asa_cache_attention(const asa_cache_params* p, const void* Q, const int64_t q_strides[3],
+                        const void* pool, const int32_t* block_table, const int32_t* lengths,
+                        const int32_t* pages, int keep, void* O, void* ws, size_t ws_bytes,
+                        asa_stream_t stream);
+
 /* The reference's host-side scrub done on the device: NaN -> 0, and if any
  * element is ±Inf the whole tensor is clamped to [-100, 100]
  * (:599-606, :684-697).  ws needs 16 bytes. */
