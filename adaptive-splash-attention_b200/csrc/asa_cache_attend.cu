@@ -1,143 +1,1240 @@
 // asa_cache_attend.cu -- attention over the 4-bit paged cache.
+//
+// For each query row: softmax weights in one pass over keys and values, or the
+// exact alpha-entmax in three (scores; the threshold of each row; the weighted
+// values of the blocks that the threshold leaves weight in).
+//
+// Work.  An item is a tile of 8 or 16 query rows of one key head (rows of one
+// sequence, or of one query token where each has its own pages); its keys are
+// walked in tiles of 32 tokens.  The items' tiles, laid end to end with a few
+// tiles' worth of time between items for what starting one costs, are cut into
+// equal runs, one a CTA, so that a batch of very unequal sequences keeps every SM
+// busy; an item that a cut divides is joined by combine_kernel from its runs'
+// partial sums (largest score, sum of weights, weighted values), in a fixed order.
+// A CTA's warps take an item's tiles in turn, each with its own ring of bulk
+// copies that runs ahead into the CTA's next item.
+//
+// Arithmetic.  A code 0..15 in an fp16 half is the subnormal n * 2^-24, and in
+// the next nibble n * 2^-20: masking a word gives tensor-core operands without
+// converting anything.  Scores are S^T = K Q^T on mma.m16n8k16 (tokens x rows):
+// per group of 32 channels the product of codes and q (q scaled by a power of two
+// a row, so that fp16 holds bf16 exactly), times the token's fp32 scale; offsets
+// enter as one more product, with the group sums of q in two fp16 halves.
+// Weights stay in registers: a movmatrix turns P^T into the operand of
+// O^T = V^T P^T.  P is rounded to fp16 once (11 bits; the plain rounding of an
+// output to bf16 has 8); its products with the values' scales are taken as the
+// rounded product and the rest, two products of the codes, so that codes and
+// offsets are weighted by the same P and a value near zero, a difference of the
+// two, is not disturbed by more than its own size.  P is kept near 2^14, so
+// neither a small weight nor a small scale falls among fp16's subnormals; a running
+// exponent lowers it where scales above 2 would overflow.  Sums, maxima and
+// accumulators are fp32.
 #include "asa_cache.h"
+#include "asa_sm100.cuh"
 
 namespace asa {
 namespace cache {
 namespace {
 
-__device__ __forceinline__ float block_sum(float v, float* part) {
-#pragma unroll
-    for (int k = 16; k; k >>= 1) v += __shfl_xor_sync(~0u, v, k);
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    return part[0] + part[1] + part[2] + part[3];
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kTop = 14.0f;         // log2 of the weight that a row's largest score gets
+constexpr float kLow = -1.0e30f;      // below any score
+constexpr int kTile = 2;              // blocks of a tile
+constexpr int kStages = 2;            // tiles a warp has in flight
+constexpr int kItemCost = 8;          // what starting an item costs, in tiles of one CTA
+constexpr int kSegments = 32;         // segments a CTA lines up at a time
+constexpr int kListCap = 2048;        // scores a row keeps in shared memory while its threshold is solved
+
+enum Mode { kSoftmax = 0, kScores = 1, kValues = 2 };
+
+// How a call's rows are tiled and its work cut.
+struct Plan {
+    int U, R, tiles;                  // units of rows (sequences; with lists, query tokens), rows each, tiles each
+    int keep;                         // pages listed a query and key head (0: all of the table)
+    int cap;                          // tiles an item can have at most
+    int split;                        // items are cut into equal runs (else one CTA an item)
+    int vec;                          // q rows may be read 16 bytes at a time
+    int least;                        // tiles a run has at least
+};
+
+// The workspace: [run length | prefix per unit | partials | scores, tile maxima, thresholds]
+struct Space {
+    int64_t* run;                     // [1 + U]
+    float* part;                      // [2 * CTAs][rows][D]
+    float* part_ml;                   // [2 * CTAs][2][rows]
+    float4* score;                    // [items][cap][2][NT][32]
+    float* top;                       // [items][cap][8 NT]
+    float* tau;                       // [items][8 NT]
+};
+
+struct Args {
+    Shape s;
+    Plan p;
+    Space w;
+    Strides qs;
+    const __nv_bfloat16* Q;
+    const uint8_t* pool;
+    const int32_t* table;
+    const int32_t* lengths;
+    const int32_t* list;
+    __nv_bfloat16* O;
+    int* err;
+};
+
+// ---- small pieces --------------------------------------------------------------
+__device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                    uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float block_max(float v, float* part) {
-#pragma unroll
-    for (int k = 16; k; k >>= 1) v = fmaxf(v, __shfl_xor_sync(~0u, v, k));
-    __syncthreads();
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
-    __syncthreads();
-    return fmaxf(fmaxf(part[0], part[1]), fmaxf(part[2], part[3]));
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack(float lo, float hi) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float2 unpack(uint32_t x) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&x));
+}
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+    const __half2 h = __hmul2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+// a * b - c: with c the rounded a * b, what the rounding cut off.
+__device__ __forceinline__ uint32_t hrest2(uint32_t a, uint32_t b, uint32_t c) {
+    const __half2 h = __hfma2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b),
+                              __hneg2(*reinterpret_cast<const __half2*>(&c)));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ uint32_t hmax2(uint32_t a, uint32_t b) {
+    const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }   // e in -126..127
+
+__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(sm100::smem_u32(dst)), "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar)) : "memory");
+}
+// Bounded wait for a block's copy.  An error word set by something else than a
+// wait that gave up (a page outside the pool) does not cut it short.
+__device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity, long long spins, int* err) {
+    if (sm100::mbar_try(bar, parity)) return true;
+    for (long long i = 0; i < spins; ++i) {
+        if (sm100::mbar_try(bar, parity)) return true;
+        if ((i & 1023) == 1023 && err && *reinterpret_cast<volatile int*>(err) == ASA_ERR_DEVICE_TIMEOUT) return false;
+    }
+    if (err) atomicExch(err, ASA_ERR_DEVICE_TIMEOUT);
+    return false;
 }
 
-// The j-th token that a query's walk over the cache meets: its record's block
-// and row, or null where it sees none.
-__device__ __forceinline__ const uint8_t* token_at(const Shape& s, const uint8_t* pool, const int32_t* table_b,
-                                                   const int32_t* list, int h, long long pos, int j, int* err) {
-    int page = j / s.P;
-    if (list) page = __ldg(list + page);
-    if (page < 0 || page >= s.width || (long long)page * s.P + j % s.P > pos) return nullptr;
-    const int id = __ldg(table_b + page);
-    if (id < 0 || id >= s.pages) {
-        if (err) atomicCAS(err, 0, ASA_ERR_INVALID);
-        return nullptr;
+// The token (0..7) that stands at index m of an 8-token half block in the
+// fragments: neighbours 2, 3 and 6, 7 trade places, which spreads the values' rows
+// over the shared-memory banks.
+__device__ __forceinline__ int token_of(int m) { return m ^ ((m >> 1) & 1); }
+
+// NW words from shared memory, as wide as their number allows.
+template <int NW>
+__device__ __forceinline__ void lds(const uint8_t* p, uint32_t (&w)[NW]) {
+    if constexpr (NW == 4) {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+    } else if constexpr (NW == 2) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else {
+#pragma unroll
+        for (int i = 0; i < NW; ++i) w[i] = reinterpret_cast<const uint32_t*>(p)[i];
     }
-    return pool + ((int64_t)id * s.H + h) * s.rec + (int64_t)(j % s.P / kBlock) * block_bytes(s.d);
+}
+// NH halves (2 NH bytes) as ceil(NH / 2) words.
+template <int NH>
+__device__ __forceinline__ void lds_halves(const uint8_t* p, uint32_t (&w)[(NH + 1) / 2]) {
+    if constexpr (NH == 4) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        w[0] = v.x, w[1] = v.y;
+    } else if constexpr (NH == 3) {
+        const uint16_t* q = reinterpret_cast<const uint16_t*>(p);
+        w[0] = q[0] | (uint32_t)q[1] << 16;
+        w[1] = q[2];
+    } else if constexpr (NH == 2) {
+        w[0] = *reinterpret_cast<const uint32_t*>(p);
+    } else {
+        w[0] = *reinterpret_cast<const uint16_t*>(p);
+    }
 }
 
-// One CTA a row (query token and head): scores to the workspace, their weights,
-// and the weighted sum of the values, a channel a thread.
-__global__ void __launch_bounds__(128) rows_kernel(Shape s, const __nv_bfloat16* __restrict__ Q, Strides qs,
-                                                   const uint8_t* __restrict__ pool,
-                                                   const int32_t* __restrict__ table,
-                                                   const int32_t* __restrict__ lengths,
-                                                   const int32_t* __restrict__ list, int keep,
-                                                   __nv_bfloat16* __restrict__ O, float* __restrict__ ws, int n_max,
-                                                   int* err) {
-    __shared__ float s_q[128], s_part[4];
-    const int tid = threadIdx.x, hq = blockIdx.x % s.HQ, bt = blockIdx.x / s.HQ, t = bt % s.T, b = bt / s.T;
-    const int h = hq / s.G, NG = s.d / 32;
-    const int32_t* table_b = table + (int64_t)b * s.width;
-    const int32_t* mine = list ? list + ((int64_t)bt * s.H + h) * keep : nullptr;
-    const long long pos = (long long)__ldg(lengths + b) - s.T + t;
-    const int n = list ? n_max : (int)max(0ll, min(pos + 1, (long long)n_max));
-    float* sc = ws + (int64_t)blockIdx.x * n_max;
-    if (tid < s.d) {
-        const float x = __bfloat162float(Q[b * qs.b + t * qs.t + (int64_t)hq * qs.h + tid]);
-        s_q[tid] = isfinite(x) ? x : NAN;
+__device__ __forceinline__ int unit_tiles(const Args& a, int u) {
+    if (a.list) return a.p.cap;
+    const long long n = min((long long)max(__ldg(a.lengths + u), 0), (long long)a.s.width * a.s.P);
+    return (int)((n + kTile * kBlock - 1) / (kTile * kBlock));
+}
+
+// Exclusive prefix of one value a thread over the CTA; *total to all.
+template <int NTHR>
+__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* s_warp, int64_t* total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int64_t x = v;
+#pragma unroll
+    for (int k = 1; k < 32; k <<= 1) {
+        const int64_t y = __shfl_up_sync(~0u, x, k);
+        if (lane >= k) x += y;
     }
     __syncthreads();
-    float top = -INFINITY;
-    for (int j = tid; j < n; j += 128) {
-        const uint8_t* blk = token_at(s, pool, table_b, mine, h, pos, j, err);
-        float v = -INFINITY;
-        if (blk) {
-            const int r = j % kBlock;
-            const uint8_t* row = blk + r * row_bytes(s.d);
-            const __half* par = reinterpret_cast<const __half*>(blk + kBlock * row_bytes(s.d)) + r * 2 * NG;
-            float acc = 0.0f;
-            for (int c = 0; c < s.d; ++c) {
-                const int g = c >> 5, w = c & 31;
-                const uint32_t byte = row[(w >> 3) * 4 * NG + 4 * g + ((w & 7) >> 1)];
-                acc += s_q[c] * fmaf((float)(c & 1 ? byte >> 4 : byte & 15u), __half2float(par[g]),
-                                     __half2float(par[NG + g]));
-            }
-            v = acc * s.scale;
-            if (s.alpha != 1.0f) v = v != v ? v : (s.alpha - 1.0f) * fminf(fmaxf(v, -10.0f), 10.0f);
-            top = fmaxf(top, v);
-            if (v != v) top = INFINITY;      // a NaN score makes the whole row NaN
-        }
-        sc[j] = v;
+    if (lane == 31) s_warp[warp] = x;
+    __syncthreads();
+    int64_t before = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < NTHR / 32; ++w) {
+        if (w < warp) before += s_warp[w];
+        sum += s_warp[w];
     }
-    top = block_max(top, s_part);
-    float total = 0.0f;
-    if (top > -INFINITY) {
-        float tau = 0.0f;
-        if (s.alpha != 1.0f) {
-            float lo = top - 1.0f, hi = top;
-            const float ex = 1.0f / (s.alpha - 1.0f);
-            for (int it = 0; it < 40; ++it) {
-                const float mid = 0.5f * (lo + hi);
-                float sum = 0.0f;
-                for (int j = tid; j < n; j += 128) sum += sc[j] > mid ? powf(sc[j] - mid, ex) : 0.0f;
-                if (block_sum(sum, s_part) >= 1.0f) lo = mid; else hi = mid;
-            }
-            tau = lo;
-        }
-        float sum = 0.0f;
-        for (int j = tid; j < n; j += 128) {
-            float p;
-            if (s.alpha == 1.0f) p = sc[j] == -INFINITY ? 0.0f : expf(sc[j] - top);
-            else p = sc[j] != sc[j] ? sc[j] : sc[j] > tau ? powf(sc[j] - tau, 1.0f / (s.alpha - 1.0f)) : 0.0f;
-            if (top == INFINITY) p = NAN;
-            sc[j] = p;
-            sum += p;
-        }
-        total = block_sum(sum, s_part);
+    *total = sum;
+    return before + x - v;
+}
+
+// ---- the walk over keys and values ----------------------------------------------
+struct Segment { int u, item, from, n, of; };         // tiles from .. from + n - 1 of an item's `of`
+struct Info { int pos0, pos1, tile, seg; };           // a ring stage: its blocks' first positions, where it belongs
+
+template <int D, int NT, int W>
+struct Smem {
+    static constexpr int kStride = D + 4;             // a float4 of each of 8 rows of lanes: no bank twice
+    alignas(128) uint8_t ring[W][kStages][2 * kTile * block_bytes(D)];
+    float4 o[W / 2][8 * NT][kStride / 4];
+    float m[W][8 * NT], l[W][8 * NT];
+    uint64_t full[W][kStages];
+    Info info[W][kStages];
+    Segment seg[kSegments];
+    int segs;
+    int64_t next;
+    int64_t pref[W * 32 + 1];
+    int64_t scan[W];
+};
+
+template <int D, int NT, int W, int MODE>
+__global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __grid_constant__ Args a) {
+    constexpr int NG = D / 32, ROWS = 8 * NT, NTHR = W * 32, BB = block_bytes(D), NS = (NG + 1) / 2;
+    constexpr int RB = row_bytes(D), PB = par_bytes(D);
+    constexpr int kNone = 0x3fffffff;                 // the first position of a block that is not there
+    extern __shared__ __align__(128) uint8_t smem_raw[];
+    auto& sm = *reinterpret_cast<Smem<D, NT, W>*>(smem_raw);
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, t = lane & 3;
+    const Shape& s = a.s;
+    const int per = a.p.tiles * s.H;                  // items of a unit
+    const int per_page = s.P / kBlock;
+
+    if (lane == 0) {
+        for (int i = 0; i < kStages; ++i) sm100::mbar_init(&sm.full[warp][i], 1);
+        sm100::fence_barrier_init();
     }
-    if (tid >= s.d) return;
-    float acc = 0.0f;
-    if (top > -INFINITY)
-        for (int j = 0; j < n; ++j) {
-            const uint8_t* blk = token_at(s, pool, table_b, mine, h, pos, j, nullptr);
-            if (!blk) continue;
-            blk += s.rec / 2;
-            const int r = j % kBlock, g = tid >> 5, w = tid & 31;
-            const __half* par = reinterpret_cast<const __half*>(blk + kBlock * row_bytes(s.d)) + r * 2 * NG;
-            const uint32_t byte = blk[r * row_bytes(s.d) + (w >> 2) * 2 * NG + 2 * g + ((w & 3) >> 1)];
-            acc += sc[j] * fmaf((float)(tid & 1 ? byte >> 4 : byte & 15u), __half2float(par[g]),
-                                __half2float(par[NG + g]));
+    __syncthreads();
+
+    // this CTA's run [x, x1) of all the items' tiles
+    int64_t x = 0, x1 = 1;
+    int chunk = 0;                                    // the units whose prefix sums are in sm.pref
+    auto load_chunk = [&](int base, int64_t before) -> int64_t {
+        __syncthreads();
+        int64_t sum, v = 0;
+        if (base + tid < a.p.U) {
+            const int n = unit_tiles(a, base + tid);
+            if (n) v = (int64_t)(n + kItemCost) * per;
         }
-    O[(int64_t)blockIdx.x * s.d + tid] = __float2bfloat16(top > -INFINITY ? acc / total : 0.0f);
+        const int64_t e = block_scan<NTHR>(v, sm.scan, &sum);
+        sm.pref[tid] = before + e;
+        if (tid == 0) sm.pref[NTHR] = before + sum;
+        __syncthreads();
+        chunk = base;
+        return before + sum;
+    };
+    if (a.p.split) {
+        int64_t total = 0;
+        for (int base = 0; base < a.p.U; base += NTHR) {
+            total = load_chunk(base, total);
+            if (blockIdx.x == 0 && base + tid < a.p.U) a.w.run[1 + base + tid] = sm.pref[tid];
+        }
+        const int64_t run = max((int64_t)a.p.least, (total + gridDim.x - 1) / gridDim.x);
+        if (blockIdx.x == 0 && tid == 0) a.w.run[0] = run;
+        x = run * blockIdx.x;
+        x1 = min(x + run, total);
+        if (x >= x1) return;
+        if (a.p.U > NTHR) {                           // back to the chunk that the run starts in
+            int64_t before = load_chunk(0, 0);
+            while (x >= before) before = load_chunk(chunk + NTHR, before);
+        }
+    }
+    int stage_in = 0, stage_out = 0;                  // the ring's next stage to fill and to read
+    uint32_t parity = 0;                              // of the stage to read
+    bool lost = false;
+
+    while (x < x1) {
+        // ---- the next segments of the run -----------------------------------------
+        __syncthreads();                              // every warp is done with the last ones
+        if (a.p.split) {
+            while (x >= sm.pref[NTHR]) load_chunk(chunk + NTHR, sm.pref[NTHR]);
+            if (tid == 0) {
+                int lo = 0, hi = NTHR, k = 0;         // the last unit that starts at or before x
+                while (hi - lo > 1) {
+                    const int mid = (lo + hi) >> 1;
+                    if (sm.pref[mid] <= x) lo = mid; else hi = mid;
+                }
+                int64_t y = x;
+                const int64_t stop = min(x1, sm.pref[NTHR]);
+                while (y < stop && k < kSegments) {
+                    while (sm.pref[lo + 1] <= y) ++lo;
+                    const int of = (int)((sm.pref[lo + 1] - sm.pref[lo]) / per) - kItemCost;
+                    const int64_t off = y - sm.pref[lo];
+                    const int item = (int)(off / (of + kItemCost));
+                    const int64_t begin = sm.pref[lo] + (int64_t)item * (of + kItemCost) + kItemCost;
+                    const int from = (int)max((int64_t)0, y - begin), to = (int)min((int64_t)of, stop - begin);
+                    if (to > from) sm.seg[k++] = Segment{chunk + lo, item, from, to - from, of};
+                    y = min(stop, begin + of);
+                }
+                sm.segs = k;
+                sm.next = y;
+            }
+        } else if (tid == 0) {
+            const int u = blockIdx.x / per, of = unit_tiles(a, u);
+            sm.seg[0] = Segment{u, (int)(blockIdx.x % per), 0, of, of};
+            sm.segs = 1;
+            sm.next = 1;
+        }
+        __syncthreads();
+        const int segs = sm.segs;
+        x = sm.next;
+
+        // where the rows of an item stand
+        auto token_of_row = [&](int u, int tile, int row) { return a.list ? u % s.T : (tile * ROWS + row) / s.G; };
+        auto head_of_row = [&](int h, int tile, int row) {
+            return h * s.G + (a.list ? tile * ROWS + row : (tile * ROWS + row) % s.G);
+        };
+        auto position = [&](int u, int tile, int row) -> int {   // -1 before the first key, and past the last row
+            if (tile * ROWS + row >= a.p.R) return -1;
+            const long long len = __ldg(a.lengths + (a.list ? u / s.T : u));
+            return (int)max(-1ll, min(len - s.T + token_of_row(u, tile, row), (long long)s.width * s.P - 1));
+        };
+
+        // ---- the tiles that this warp reads, fetched ahead across segments -----------
+        int ahead = -1, mine = 0, c = 0;              // the segment being fetched, the warp's tiles of it, 32 c of them passed
+        uint32_t there = 0;                           // of the 32 that the lanes have looked up
+        int rec0 = -1, rec1 = -1, pos0 = 0, pos1 = 0; // this lane's: record and first position of its blocks
+        auto locate = [&](const Segment& g, int k) -> bool {
+            rec0 = rec1 = -1;
+            pos0 = pos1 = kNone;
+            if (k >= mine) return false;
+            const int j = g.from + warp + k * W, h = g.item / a.p.tiles, tile = g.item % a.p.tiles;
+            const int64_t item_no = (int64_t)g.u * per + g.item;
+            const int pos_hi = position(g.u, tile, min(ROWS, a.p.R - tile * ROWS) - 1);
+            bool wanted = true;
+            if constexpr (MODE == kValues) {          // only tiles that a threshold leaves weight in
+                const float* top = a.w.top + (item_no * a.p.cap + j) * ROWS;
+                wanted = false;
+#pragma unroll
+                for (int i = 0; i < ROWS; i += 4) {
+                    const float4 y = *reinterpret_cast<const float4*>(top + i);
+                    const float4 z = *reinterpret_cast<const float4*>(a.w.tau + item_no * ROWS + i);
+                    wanted |= !(y.x <= z.x) | !(y.y <= z.y) | !(y.z <= z.z) | !(y.w <= z.w);
+                }
+            }
+            if (wanted) {
+                const int32_t* table_b = a.table + (int64_t)(a.list ? g.u / s.T : g.u) * s.width;
+                const int32_t* list = a.list ? a.list + ((int64_t)g.u * s.H + h) * a.p.keep : nullptr;
+                auto block = [&](int blk, int& rec, int& pos) {
+                    int page = blk / per_page;
+                    if (list) page = page < a.p.keep ? __ldg(list + page) : -1;
+                    if (page < 0 || page >= s.width) return;
+                    const int first = page * s.P + blk % per_page * kBlock;
+                    if (first > pos_hi) return;
+                    const int id = __ldg(table_b + page);
+                    if (id >= 0 && id < s.pages) {
+                        rec = id * s.H + h;
+                        pos = first;
+                    } else if (a.err) {
+                        atomicCAS(a.err, 0, ASA_ERR_INVALID);
+                    }
+                };
+                block(kTile * j, rec0, pos0);
+                if (per_page == 1) {
+                    block(kTile * j + 1, rec1, pos1);
+                } else if (rec0 >= 0) {               // the tile lies in one page
+                    rec1 = rec0;
+                    if (pos0 + kBlock <= pos_hi) pos1 = pos0 + kBlock;
+                }
+            }
+            const bool found = rec0 >= 0 || rec1 >= 0;
+            if constexpr (MODE == kScores)
+                if (!found)
+                    for (int i = 0; i < ROWS; ++i) a.w.top[(item_no * a.p.cap + j) * ROWS + i] = -INFINITY;
+            return found;
+        };
+        int in_flight = 0;
+        auto fetch = [&]() {                          // the next tile that is there, into the ring
+            while (!there) {
+                if (32 * c >= mine) {
+                    if (ahead + 1 >= segs) return;
+                    ++ahead;
+                    c = 0;
+                    mine = sm.seg[ahead].n > warp ? (sm.seg[ahead].n - warp + W - 1) / W : 0;
+                    continue;
+                }
+                there = __ballot_sync(~0u, locate(sm.seg[ahead], 32 * c + lane));
+                ++c;
+            }
+            const int k = __ffs(there) - 1;
+            there &= there - 1;
+            const int r0 = __shfl_sync(~0u, rec0, k), r1 = __shfl_sync(~0u, rec1, k);
+            const int p0 = __shfl_sync(~0u, pos0, k), p1 = __shfl_sync(~0u, pos1, k);
+            if (lane == 0) {
+                const int j = sm.seg[ahead].from + warp + (32 * (c - 1) + k) * W;
+                sm.info[warp][stage_in] = Info{p0, p1, j, ahead};
+                uint8_t* dst = sm.ring[warp][stage_in];
+                uint64_t* bar = &sm.full[warp][stage_in];
+                constexpr int kParts = MODE == kSoftmax ? 2 : 1;
+                if (per_page > 1) {                   // two blocks on end
+                    const uint8_t* src = a.pool + r0 * s.rec + (int64_t)(kTile * j % per_page) * BB;
+                    sm100::mbar_expect_tx(bar, kParts * kTile * BB);
+                    if (MODE != kValues) bulk_load(dst, src, kTile * BB, bar);
+                    if (MODE != kScores) bulk_load(dst + kTile * BB, src + s.rec / 2, kTile * BB, bar);
+                } else {
+                    sm100::mbar_expect_tx(bar, kParts * BB * ((r0 >= 0) + (r1 >= 0)));
+#pragma unroll
+                    for (int i = 0; i < kTile; ++i) {
+                        const int rec = i ? r1 : r0;
+                        if (rec < 0) continue;
+                        const uint8_t* src = a.pool + rec * s.rec;
+                        if (MODE != kValues) bulk_load(dst + i * BB, src, BB, bar);
+                        if (MODE != kScores) bulk_load(dst + (kTile + i) * BB, src + s.rec / 2, BB, bar);
+                    }
+                }
+            }
+            __syncwarp();
+            stage_in = stage_in + 1 == kStages ? 0 : stage_in + 1;
+            ++in_flight;
+        };
+        for (int i = 0; i < kStages; ++i) fetch();
+
+        for (int sg = 0; sg < segs; ++sg) {
+            const Segment g = sm.seg[sg];
+            const int h = g.item / a.p.tiles, tile = g.item % a.p.tiles;
+            const int64_t item_no = (int64_t)g.u * per + g.item;
+            const int b = a.list ? g.u / s.T : g.u;
+            const int rows = min(ROWS, a.p.R - tile * ROWS);
+            const int pos_hi = position(g.u, tile, rows - 1), pos_lo = position(g.u, tile, 0);   // rows stand in order
+
+            // ---- queries as B fragments, a power of two a row -----------------------
+            uint32_t qf[NT][NG][4], qz[NT];
+            float rf[NT][2];                          // scores: the factor of rows 2t, 2t + 1; values: their thresholds
+            int pos[NT][2];
+            float m[NT][2], oz[NT][4], o[NT][2 * NG][4];   // oz: by group the offsets' sums, and the weights'
+            float lift = 0.0f;                        // log2 by which weights are lowered for large scales
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                if constexpr (MODE != kValues) {
+                    const int row = 8 * nt + r;
+                    float q[NG][8], big = 0.0f;
+                    bool bad = false;
+                    const __nv_bfloat16* src =
+                        row < rows ? a.Q + b * a.qs.b + token_of_row(g.u, tile, row) * a.qs.t +
+                                         head_of_row(h, tile, row) * a.qs.h + 8 * t
+                                   : nullptr;
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) {
+                        uint32_t w[4] = {0u, 0u, 0u, 0u};
+                        if (src && a.p.vec) {
+                            const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + 32 * i));
+                            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+                        } else if (src) {
+                            const uint16_t* e = reinterpret_cast<const uint16_t*>(src + 32 * i);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) w[k] = __ldg(e + 2 * k) | (uint32_t)__ldg(e + 2 * k + 1) << 16;
+                        }
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) {
+                            q[i][2 * k] = __uint_as_float(w[k] << 16);
+                            q[i][2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) {
+                            big = fmaxf(big, fabsf(q[i][k]));
+                            bad |= !isfinite(q[i][k]);
+                        }
+                    }
+                    big = fmaxf(big, __shfl_xor_sync(~0u, big, 1));
+                    big = fmaxf(big, __shfl_xor_sync(~0u, big, 2));
+                    const bool row_bad = (__ballot_sync(~0u, bad) >> (lane & 28)) & 15u;
+                    // big * 2^up lies in [2^13, 2^14), but for what is below 2^-113
+                    const int up = big == 0.0f || row_bad ? 0 : 13 - max((int)(__float_as_uint(big) >> 23) - 127, -113);
+                    const float f = pow2i(up), f16 = pow2i(up - 4);
+                    float own = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < NG; ++i) {
+                        if (row_bad) {
+#pragma unroll
+                            for (int k = 0; k < 8; ++k) q[i][k] = NAN;
+                        }
+                        // channels 8t .. 8t + 7 of the group, in the order that masking a word of codes gives
+                        qf[nt][i][0] = pack(q[i][0] * f, q[i][4] * f);
+                        qf[nt][i][1] = pack(q[i][1] * f16, q[i][5] * f16);
+                        qf[nt][i][2] = pack(q[i][2] * f, q[i][6] * f);
+                        qf[nt][i][3] = pack(q[i][3] * f16, q[i][7] * f16);
+                        float v = 0.0f;
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) v += q[i][k] * f16;
+                        v += __shfl_xor_sync(~0u, v, 1);
+                        v += __shfl_xor_sync(~0u, v, 2);
+                        own = t == i ? v : own;
+                    }
+                    const float hi = __half2float(__float2half_rn(own));
+                    qz[nt] = pack(hi, own - hi);
+                    const float back = scalbnf(s.scale * (MODE == kSoftmax ? kLog2e : 1.0f), 24 - up);
+                    rf[nt][0] = __shfl_sync(~0u, back, 8 * t);
+                    rf[nt][1] = __shfl_sync(~0u, back, 8 * t + 4);
+                }
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const int row = 8 * nt + 2 * t + e;
+                    pos[nt][e] = position(g.u, tile, row);
+                    m[nt][e] = MODE == kSoftmax ? kLow : -kTop;
+                    oz[nt][e] = oz[nt][e + 2] = 0.0f;
+                    if constexpr (MODE == kValues) rf[nt][e] = a.w.tau[item_no * ROWS + row];
+                }
+#pragma unroll
+                for (int i = 0; i < 2 * NG; ++i)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) o[nt][i][e] = 0.0f;
+            }
+
+            // ---- the segment's tiles ---------------------------------------------------
+            while (in_flight && sm.info[warp][stage_out].seg == sg) {
+                const Info info = sm.info[warp][stage_out];
+                if (!wait_full(&sm.full[warp][stage_out], parity, s.spins, a.err)) lost = true;
+                __syncwarp();
+                const uint8_t* kb = sm.ring[warp][stage_out];
+                const uint8_t* vb = kb + kTile * BB;
+                // every row sees all of both blocks
+                const bool whole = max(info.pos0, info.pos1) + kBlock - 1 <= pos_lo;
+                const int t0 = token_of(r), t1 = t0 + 8;           // the tokens of this lane's scores, in a block
+                float v[kTile][NT][4];
+
+                if constexpr (MODE != kValues) {
+                    // scores of tokens t0, t1 and rows 2t, 2t + 1, group by group
+#pragma unroll
+                    for (int i = 0; i < kTile; ++i) {
+                        const uint8_t* blk = kb + i * BB;
+                        uint32_t w0[NG], w1[NG], p0[NS], p1[NS];
+                        lds<NG>(blk + t0 * RB + t * 4 * NG, w0);
+                        lds<NG>(blk + t1 * RB + t * 4 * NG, w1);
+                        const uint8_t* par = blk + kBlock * RB;
+                        lds_halves<NG>(par + t0 * PB, p0);
+                        lds_halves<NG>(par + t1 * PB, p1);
+                        // (lanes past the last group read a scale; their part of q's sums is zero)
+                        const int zt = NG == 4 || t < NG ? 2 * (NG + t) : 0;
+                        uint32_t z0 = *reinterpret_cast<const uint16_t*>(par + t0 * PB + zt);
+                        uint32_t z1 = *reinterpret_cast<const uint16_t*>(par + t1 * PB + zt);
+                        z0 = __byte_perm(z0, z0, 0x1010);
+                        z1 = __byte_perm(z1, z1, 0x1010);
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            float cz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                            mma(cz, z0, z1, 0u, 0u, qz[nt], 0u);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[i][nt][e] = cz[e] * 9.5367431640625e-7f;   // 2^-20: codes and halves count 2^-24, 2^-4
+                        }
+#pragma unroll
+                        for (int k = 0; k < NG; ++k) {
+                            const uint32_t x0 = w0[k], y0 = w1[k], x8 = x0 >> 8, y8 = y0 >> 8;
+                            const float2 s0 = unpack(p0[k >> 1]), s1 = unpack(p1[k >> 1]);
+                            const float f0 = k & 1 ? s0.y : s0.x, f1 = k & 1 ? s1.y : s1.x;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                                mma(acc, x0 & 0x000f000fu, y0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x00f000f0u,
+                                    qf[nt][k][0], qf[nt][k][1]);
+                                mma(acc, x8 & 0x000f000fu, y8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x00f000f0u,
+                                    qf[nt][k][2], qf[nt][k][3]);
+                                v[i][nt][0] = fmaf(acc[0], f0, v[i][nt][0]);
+                                v[i][nt][1] = fmaf(acc[1], f0, v[i][nt][1]);
+                                v[i][nt][2] = fmaf(acc[2], f1, v[i][nt][2]);
+                                v[i][nt][3] = fmaf(acc[3], f1, v[i][nt][3]);
+                            }
+                        }
+                    }
+                }
+                if constexpr (MODE == kScores) {
+                    const float am1 = s.alpha - 1.0f;
+                    const int64_t place = item_no * a.p.cap + info.tile;
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        float top[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+                        for (int i = 0; i < kTile; ++i) {
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                const float y = v[i][nt][e] * rf[nt][e & 1];
+                                float z = am1 * fminf(fmaxf(y, -10.0f), 10.0f);
+                                if (y != y) z = NAN;
+                                if (!whole && (i ? info.pos1 : info.pos0) + (e < 2 ? t0 : t1) > pos[nt][e & 1]) z = -INFINITY;
+                                top[e & 1] = fmaxf(top[e & 1], z != z ? INFINITY : z);   // a NaN score: its row is NaN
+                                v[i][nt][e] = z;
+                            }
+                            if (8 * nt + 2 * t < rows)
+                                a.w.score[((place * kTile + i) * NT + nt) * 32 + 8 * t + r] =
+                                    make_float4(v[i][nt][0], v[i][nt][1], v[i][nt][2], v[i][nt][3]);
+                        }
+#pragma unroll
+                        for (int k = 4; k < 32; k <<= 1) {
+                            top[0] = fmaxf(top[0], __shfl_xor_sync(~0u, top[0], k));
+                            top[1] = fmaxf(top[1], __shfl_xor_sync(~0u, top[1], k));
+                        }
+                        // rows past the last take no part
+                        if (8 * nt + 2 * t >= rows) top[0] = -INFINITY;
+                        if (8 * nt + 2 * t + 1 >= rows) top[1] = -INFINITY;
+                        if (r == 0) *reinterpret_cast<float2*>(a.w.top + place * ROWS + 8 * nt + 2 * t) = make_float2(top[0], top[1]);
+                    }
+                } else {
+                    if constexpr (MODE == kValues) {
+                        const int64_t place = item_no * a.p.cap + info.tile;
+#pragma unroll
+                        for (int i = 0; i < kTile; ++i)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                float4 y = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                                if (8 * nt + 2 * t < rows) y = a.w.score[((place * kTile + i) * NT + nt) * 32 + 8 * t + r];
+                                v[i][nt][0] = y.x, v[i][nt][1] = y.y, v[i][nt][2] = y.z, v[i][nt][3] = y.w;
+                            }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < kTile; ++i)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    v[i][nt][e] *= rf[nt][e & 1];
+                                    if (!whole && (i ? info.pos1 : info.pos0) + (e < 2 ? t0 : t1) > pos[nt][e & 1])
+                                        v[i][nt][e] = -INFINITY;
+                                }
+                    }
+                    // the values' scales: tokens ta, tb (k = 2t, 2t + 1) and those 8 on, as pairs a group
+                    const int ta = token_of(2 * t), tb = token_of(2 * t + 1);
+                    uint32_t sp[kTile][NG][2], zp[kTile][2];
+#pragma unroll
+                    for (int i = 0; i < kTile; ++i) {
+                        const uint8_t* par = vb + i * BB + kBlock * RB;
+                        uint32_t ra[NS], rb[NS], rc[NS], rd[NS];
+                        lds_halves<NG>(par + ta * PB, ra);
+                        lds_halves<NG>(par + tb * PB, rb);
+                        lds_halves<NG>(par + (ta + 8) * PB, rc);
+                        lds_halves<NG>(par + (tb + 8) * PB, rd);
+#pragma unroll
+                        for (int k = 0; k < NG; ++k) {
+                            const uint32_t pick = k & 1 ? 0x7632u : 0x5410u;
+                            sp[i][k][0] = __byte_perm(ra[k >> 1], rb[k >> 1], pick);
+                            sp[i][k][1] = __byte_perm(rc[k >> 1], rd[k >> 1], pick);
+                        }
+                        // group r's offsets; row NG of that product is ones, and sums the weights
+                        zp[i][0] = zp[i][1] = r == NG ? 0x3c003c00u : 0u;
+                        if (r < NG) {
+                            const uint8_t* z = par + 2 * NG + 2 * r;
+                            zp[i][0] = *reinterpret_cast<const uint16_t*>(z + ta * PB) | (uint32_t)*reinterpret_cast<const uint16_t*>(z + tb * PB) << 16;
+                            zp[i][1] = *reinterpret_cast<const uint16_t*>(z + (ta + 8) * PB) | (uint32_t)*reinterpret_cast<const uint16_t*>(z + (tb + 8) * PB) << 16;
+                        }
+                    }
+                    if (!whole) {
+                        // Tokens that no row sees may hold anything: their scales and
+                        // offsets become zero.  So do those of tokens that only some rows
+                        // see and that hold a NaN; it goes to the rows that see it by way
+                        // of the offsets' sums.
+#pragma unroll
+                        for (int i = 0; i < kTile; ++i) {
+                            const int first = i ? info.pos1 : info.pos0;
+                            uint32_t bad = 0;         // of group r: the tokens with a NaN, by position
+#pragma unroll
+                            for (int j = 0; j < 2; ++j)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const int tok = (e ? tb : ta) + 8 * j;
+                                    const uint32_t half = 0xffffu << (16 * e), inf = 0x7c00u << (16 * e);
+                                    const bool seen = first + tok <= pos_hi;
+                                    bool nan = (zp[i][j] & inf) == inf;
+#pragma unroll
+                                    for (int k = 0; k < NG; ++k) {
+                                        const bool off = (sp[i][k][j] & inf) == inf;
+                                        if (k == r) nan |= off;
+                                        if (!seen || off) sp[i][k][j] &= ~half;
+                                    }
+                                    if (r < NG && (!seen || nan)) zp[i][j] &= ~half;
+                                    if (r < NG && seen && nan) bad |= 1u << tok;
+                                }
+                            bad |= __shfl_xor_sync(~0u, bad, 1);
+                            bad |= __shfl_xor_sync(~0u, bad, 2);
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    const int see = min(max(pos[nt][e] - first + 1, 0), kBlock);
+                                    if (bad & ((1u << see) - 1u)) oz[nt][e] = NAN;
+                                }
+                        }
+                    }
+                    // weights near 2^14, below 2^(14.5 - lift) at most, scales below 2^(lift + 1),
+                    // so that their products stay within fp16: rescale where a score or a scale
+                    // has outgrown what they were fitted to
+                    uint32_t sbig = hmax2(sp[0][0][0], sp[0][0][1]);
+#pragma unroll
+                    for (int k = 1; k < kTile * NG; ++k) sbig = hmax2(sbig, hmax2(sp[k / NG][k % NG][0], sp[k / NG][k % NG][1]));
+                    const float2 sb = unpack(sbig);
+                    const float smax = fmaxf(sb.x, sb.y);          // NaN aside
+                    bool grow = smax > pow2i((int)lift + 1);
+                    if constexpr (MODE == kSoftmax) {
+                        const float room = kTop + 0.5f - lift;
+#pragma unroll
+                        for (int i = 0; i < kTile; ++i)
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) grow |= v[i][nt][e] - m[nt][e & 1] > room;
+                    }
+                    if (__any_sync(~0u, grow)) {
+                        const uint32_t all = __reduce_max_sync(~0u, __float_as_uint(fminf(smax, kF16Max)));
+                        const float up = fmaxf(lift, (float)((int)(all >> 23) - 127));   // 2^up <= largest scale < 2^(up + 1)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            float f[2];
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                float next = m[nt][e] + (up - lift);
+                                if constexpr (MODE == kSoftmax) {
+                                    float top = fmaxf(fmaxf(v[0][nt][e], v[0][nt][e + 2]), fmaxf(v[1][nt][e], v[1][nt][e + 2]));
+                                    top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
+                                    top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
+                                    top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+                                    next = fmaxf(next, top - kTop + up);
+                                }
+                                f[e] = exp2_fast(m[nt][e] - next);
+                                m[nt][e] = next;
+                                oz[nt][e] *= f[e];
+                            }
+#pragma unroll
+                            for (int i = 0; i < 2 * NG; ++i)
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) o[nt][i][e] *= f[e & 1];
+                        }
+                        lift = up;
+                    }
+                    // P, and P^T as an operand
+                    uint32_t pb[kTile][NT][2];
+#pragma unroll
+                    for (int i = 0; i < kTile; ++i)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt) {
+                            float p[4];
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) {
+                                if constexpr (MODE == kSoftmax) {
+                                    p[e] = exp2_fast(v[i][nt][e] - m[nt][e & 1]);
+                                } else {
+                                    const float y = v[i][nt][e] - rf[nt][e & 1];
+                                    const float k = exp2_fast(-m[nt][e & 1]);
+                                    if (s.alpha == 1.5f) p[e] = y > 0.0f ? y * y * k : 0.0f;
+                                    else p[e] = y > 0.0f ? exp2f(log2f(y) / (s.alpha - 1.0f)) * k : 0.0f;
+                                    if (y != y) p[e] = y;
+                                }
+                            }
+                            pb[i][nt][0] = transpose8(pack(p[0], p[1]));
+                            pb[i][nt][1] = transpose8(pack(p[2], p[3]));
+                            mma(oz[nt], zp[i][0], 0u, zp[i][1], 0u, pb[i][nt][0], pb[i][nt][1]);
+                        }
+                    // the values' codes: a half word of each token and group, four channels
+#pragma unroll
+                    for (int i = 0; i < kTile; ++i) {
+                        uint32_t ca[NS], cb[NS], cc[NS], cd[NS];
+                        const uint8_t* code = vb + i * BB + r * 2 * NG;
+                        lds_halves<NG>(code + ta * RB, ca);
+                        lds_halves<NG>(code + tb * RB, cb);
+                        lds_halves<NG>(code + (ta + 8) * RB, cc);
+                        lds_halves<NG>(code + (tb + 8) * RB, cd);
+#pragma unroll
+                        for (int k = 0; k < NG; ++k) {
+                            const uint32_t pick = k & 1 ? 0x7632u : 0x5410u;
+                            const uint32_t x0 = __byte_perm(ca[k >> 1], cb[k >> 1], pick), x8 = x0 >> 8;
+                            const uint32_t y0 = __byte_perm(cc[k >> 1], cd[k >> 1], pick), y8 = y0 >> 8;
+#pragma unroll
+                            for (int nt = 0; nt < NT; ++nt) {
+                                const uint32_t b0 = hmul2(pb[i][nt][0], sp[i][k][0]), b1 = hmul2(pb[i][nt][1], sp[i][k][1]);
+                                const uint32_t e0 = hrest2(pb[i][nt][0], sp[i][k][0], b0), e1 = hrest2(pb[i][nt][1], sp[i][k][1], b1);
+                                mma(o[nt][2 * k], x0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x000f000fu, y0 & 0x00f000f0u, b0, b1);
+                                mma(o[nt][2 * k + 1], x8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x000f000fu, y8 & 0x00f000f0u, b0, b1);
+                                mma(o[nt][2 * k], x0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x000f000fu, y0 & 0x00f000f0u, e0, e1);
+                                mma(o[nt][2 * k + 1], x8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x000f000fu, y8 & 0x00f000f0u, e0, e1);
+                            }
+                        }
+                    }
+                }
+                __syncwarp();                         // the stage has been read by all lanes
+                if (++stage_out == kStages) stage_out = 0, parity ^= 1u;
+                --in_flight;
+                fetch();
+            }
+
+            // ---- the warps' sums together; the item's output, or this run's part of it ---
+            if constexpr (MODE != kScores) {
+                // a row's weight sum is in the lanes r = NG; scale the sums to one reference a row
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+                        if (r == NG) {
+                            sm.m[warp][8 * nt + 2 * t + e] = m[nt][e];
+                            sm.l[warp][8 * nt + 2 * t + e] = oz[nt][e];
+                        }
+                __syncthreads();                      // (also: sm.o is free again)
+                constexpr int H = W / 2;
+#pragma unroll
+                for (int half = 1; half >= 0; --half) {   // the upper warps hand theirs to the lower ones
+                    if ((warp >= H) == (half == 1)) {
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const int row = 8 * nt + 2 * t + e;
+                                float top = sm.m[0][row];
+#pragma unroll
+                                for (int w = 1; w < W; ++w) top = fmaxf(top, sm.m[w][row]);
+                                const float f = exp2_fast(m[nt][e] - top);
+#pragma unroll
+                                for (int k = 0; k < NG; ++k) {
+                                    const float z = __shfl_sync(~0u, oz[nt][e], 4 * k + t);
+                                    constexpr float k0 = 16777216.0f, k1 = 1048576.0f;   // codes count 2^-24 and 2^-20
+                                    float4 y = make_float4(fmaf(o[nt][2 * k][e], k0, z) * f, fmaf(o[nt][2 * k][e + 2], k1, z) * f,
+                                                           fmaf(o[nt][2 * k + 1][e], k0, z) * f, fmaf(o[nt][2 * k + 1][e + 2], k1, z) * f);
+                                    float4* dst = &sm.o[warp % H][row][8 * k + r];
+                                    if (half == 0) {
+                                        const float4 u = *dst;
+                                        y = make_float4(y.x + u.x, y.y + u.y, y.z + u.z, y.w + u.w);
+                                    }
+                                    *dst = y;
+                                }
+                            }
+                    }
+                    __syncthreads();
+                }
+                const bool all = g.n == g.of;
+                const int64_t slot = 2 * (int64_t)blockIdx.x + (g.from + g.n < g.of ? 1 : 0);
+                for (int i = tid; i < rows * (D / 4); i += NTHR) {
+                    const int row = i / (D / 4), c4 = i % (D / 4);
+                    float top = sm.m[0][row];
+#pragma unroll
+                    for (int w = 1; w < W; ++w) top = fmaxf(top, sm.m[w][row]);
+                    float sum = 0.0f;
+#pragma unroll
+                    for (int w = 0; w < W; ++w) sum = fmaf(sm.l[w][row], exp2_fast(sm.m[w][row] - top), sum);
+                    float4 acc = sm.o[0][row][c4];
+#pragma unroll
+                    for (int w = 1; w < H; ++w) {
+                        const float4 y = sm.o[w][row][c4];
+                        acc = make_float4(acc.x + y.x, acc.y + y.y, acc.z + y.z, acc.w + y.w);
+                    }
+                    if (all) {
+                        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                        __nv_bfloat162 y[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv),
+                                               __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
+                        __nv_bfloat16* dst = a.O + (((int64_t)b * s.T + token_of_row(g.u, tile, row)) * s.HQ +
+                                                    head_of_row(h, tile, row)) * D + 4 * c4;
+                        *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(y);
+                    } else {
+                        *reinterpret_cast<float4*>(a.w.part + (slot * ROWS + row) * D + 4 * c4) = acc;
+                        if (c4 == 0) *reinterpret_cast<float2*>(a.w.part_ml + (slot * ROWS + row) * 2) = make_float2(top, sum);
+                    }
+                }
+                __syncthreads();                      // sm.m, sm.o are free again
+            }
+        }
+        if (!a.p.split) break;
+    }
+    // A wait gave up: nothing of this CTA may be in flight when it ends.  The last
+    // phase of a stage is this round's before stage_out, else the round's before.
+    if (lost)
+        for (int i = 0; i < kStages; ++i) sm100::mbar_drain(&sm.full[warp][i], i < stage_out ? parity : parity ^ 1u);
+}
+
+// ---- joining an item that several CTAs walked -------------------------------------
+// A CTA a row: its warps take the parts in turn, a lane four channels.
+template <int D, int NT>
+__global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Args a) {
+    constexpr int ROWS = 8 * NT;
+    __shared__ float s_top[4], s_sum[4];
+    __shared__ float4 s_acc[4][D / 4];
+    const Shape& s = a.s;
+    const int per = a.p.tiles * s.H, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int row = blockIdx.x % ROWS, item_no = blockIdx.x / ROWS;
+    const int u = item_no / per, item = item_no % per, h = item / a.p.tiles, tile = item % a.p.tiles;
+    if (tile * ROWS + row >= a.p.R) return;
+    const int of = unit_tiles(a, u);
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    float sum = 0.0f;
+    if (of) {
+        const int64_t run = a.w.run[0], x0 = a.w.run[1 + u] + (int64_t)item * (of + kItemCost) + kItemCost;
+        const int64_t c0 = x0 / run, c1 = (x0 + of - 1) / run;
+        if (c0 == c1) return;                         // one CTA had it all, and wrote the output
+        const int n = (int)(c1 - c0) + 1;
+        // the last CTA's part is its first segment, the others' their last
+        auto slot = [&](int i) { return 2 * (c0 + i) + (i + 1 < n ? 1 : 0); };
+        float top = kLow;
+        for (int i = threadIdx.x; i < n; i += 128) top = fmaxf(top, a.w.part_ml[(slot(i) * ROWS + row) * 2]);
+#pragma unroll
+        for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, k));
+        if (lane == 0) s_top[warp] = top;
+        __syncthreads();
+        top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
+#pragma unroll 4
+        for (int i = warp; i < n; i += 4) {
+            const float2 ml = *reinterpret_cast<const float2*>(a.w.part_ml + (slot(i) * ROWS + row) * 2);
+            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            if (lane < D / 4) y = *reinterpret_cast<const float4*>(a.w.part + (slot(i) * ROWS + row) * D + 4 * lane);
+            const float f = exp2_fast(ml.x - top);
+            sum = fmaf(ml.y, f, sum);
+            acc = make_float4(fmaf(y.x, f, acc.x), fmaf(y.y, f, acc.y), fmaf(y.z, f, acc.z), fmaf(y.w, f, acc.w));
+        }
+        if (lane == 0) s_sum[warp] = sum;
+        if (lane < D / 4) s_acc[warp][lane] = acc;
+        __syncthreads();
+        sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
+        if (lane < D / 4) {
+            acc = s_acc[0][lane];
+#pragma unroll
+            for (int w = 1; w < 4; ++w) {
+                const float4 y = s_acc[w][lane];
+                acc = make_float4(acc.x + y.x, acc.y + y.y, acc.z + y.z, acc.w + y.w);
+            }
+        }
+    }
+    if (warp || lane >= D / 4) return;
+    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+    __nv_bfloat162 y[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv), __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
+    const int b = a.list ? u / s.T : u, x = tile * ROWS + row;
+    const int tq = a.list ? u % s.T : x / s.G, g = a.list ? x : x % s.G;
+    *reinterpret_cast<uint2*>(a.O + (((int64_t)b * s.T + tq) * s.HQ + h * s.G + g) * D + 4 * lane) = *reinterpret_cast<uint2*>(y);
+}
+
+// ---- the alpha-entmax threshold ----------------------------------------------------
+// One CTA an item's eight rows, a warp a row in the end.  A row's support lies
+// within 1 of its largest x = (alpha - 1) score: the tiles whose maxima reach
+// that are read once to count and once to collect such scores, in an order that
+// does not depend on timing, and the root of sum (x - tau)_+^(1/(alpha-1)) = 1 is
+// found among them by Newton's steps from the left, kept inside a bracket.
+template <int NT>
+__global__ void __launch_bounds__(256) threshold_kernel(const __grid_constant__ Args a) {
+    constexpr int ROWS = 8 * NT;
+    extern __shared__ float s_list[];                 // [8][kListCap]
+    __shared__ float s_top[8][8], s_sum[8][8][2], s_tau[8];
+    __shared__ int s_count[8][8];                     // [warp][row]
+    const Shape& s = a.s;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, t = lane >> 3;
+    const int per = a.p.tiles * s.H, nt = blockIdx.x % NT;
+    const int64_t item_no = blockIdx.x / NT;
+    const int u = (int)(item_no / per), tile = (int)(item_no % per) % a.p.tiles;
+    const int rows = min(8, a.p.R - tile * ROWS - 8 * nt);
+    float* tau_out = a.w.tau + item_no * ROWS + 8 * nt;
+    if (rows <= 0) {
+        if (tid < 8) tau_out[tid] = INFINITY;
+        return;
+    }
+    const int nb = unit_tiles(a, u);
+    const float* tops = a.w.top + item_no * a.p.cap * ROWS + 8 * nt;
+    const float4* tiles = a.w.score + (item_no * a.p.cap * kTile * NT + nt) * 32;
+    // the rows' maxima
+    {
+        const int row = tid & 7;
+        float top = -INFINITY;
+        for (int j = tid >> 3; j < nb; j += 32) top = fmaxf(top, __ldg(tops + (int64_t)j * ROWS + row));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
+        if (lane < 8) s_top[warp][lane] = row < rows ? top : -INFINITY;
+    }
+    __syncthreads();
+    if (tid < 8) {
+        float top = s_top[0][tid];
+        for (int w = 1; w < 8; ++w) top = fmaxf(top, s_top[w][tid]);
+        s_tau[tid] = top;
+    }
+    __syncthreads();
+    float top[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top[i] = s_tau[i];
+    const float top0 = 2 * t < rows ? s_tau[2 * t] : INFINITY, top1 = 2 * t + 1 < rows ? s_tau[2 * t + 1] : INFINITY;
+    // each warp a stretch of tiles; fn(scores) for those that may hold support
+    const int from = (int)((int64_t)nb * warp / 8), to = (int)((int64_t)nb * (warp + 1) / 8);
+    auto each = [&](auto fn) {
+        for (int base = from; base < to; base += 32) {
+            bool want = false;
+            if (base + lane < to) {
+                const float* p = tops + (int64_t)(base + lane) * ROWS;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) want |= i < rows && __ldg(p + i) > top[i] - 1.0f;
+            }
+            uint32_t votes = __ballot_sync(~0u, want);
+            while (votes) {                           // four at a time, so that their loads overlap
+                float4 y[8];
+#pragma unroll
+                for (int k = 0; k < 8; k += 2) {
+                    y[k] = y[k + 1] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    if (votes) {
+                        const int64_t j = base + __ffs(votes) - 1;
+                        votes &= votes - 1;
+                        if (2 * t < rows) {
+                            y[k] = __ldg(tiles + (j * kTile) * NT * 32 + lane);
+                            y[k + 1] = __ldg(tiles + (j * kTile + 1) * NT * 32 + lane);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int k = 0; k < 8; ++k) fn(y[k]);
+            }
+        }
+    };
+    int c0 = 0, c1 = 0;
+    each([&](float4 y) {
+        c0 += (y.x - top0 > -1.0f) + (y.z - top0 > -1.0f);
+        c1 += (y.y - top1 > -1.0f) + (y.w - top1 > -1.0f);
+    });
+    // places: by warp, then by lane within the row's eight lanes
+    int e0 = c0, e1 = c1;
+#pragma unroll
+    for (int k = 1; k < 8; k <<= 1) {
+        const int f0 = __shfl_up_sync(~0u, e0, k, 8), f1 = __shfl_up_sync(~0u, e1, k, 8);
+        if ((lane & 7) >= k) e0 += f0, e1 += f1;
+    }
+    if ((lane & 7) == 7) s_count[warp][2 * t] = e0, s_count[warp][2 * t + 1] = e1;
+    __syncthreads();
+    e0 -= c0;
+    e1 -= c1;
+    bool fits = true;
+    int mine = 0;                                     // of row `warp`
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        int all = 0;
+        for (int w = 0; w < 8; ++w) {
+            if (w < warp && i == 2 * t) e0 += s_count[w][i];
+            if (w < warp && i == 2 * t + 1) e1 += s_count[w][i];
+            all += s_count[w][i];
+        }
+        fits &= all <= kListCap;
+        if (i == warp) mine = all;
+    }
+    const float ex = 1.0f / (s.alpha - 1.0f);
+    auto gain = [&](float y, float tau, float& f, float& df) {   // y, tau relative to the row's maximum
+        const float d = y - tau;
+        if (!(d > 0.0f)) return;
+        if (s.alpha == 1.5f) {
+            f = fmaf(d, d, f);
+            df = fmaf(2.0f, d, df);
+        } else {
+            const float p = exp2f(log2f(d) * ex);
+            f += p;
+            df += ex * p / d;
+        }
+    };
+    // one step: the bracket [lo, hi] around the root, the next point within it
+    auto step = [](float f, float df, float& lo, float& hi, float& tau) {
+        if (f >= 1.0f) lo = tau; else hi = tau;
+        const float next = tau + (f - 1.0f) / df;
+        const bool inside = next >= lo && next <= hi;
+        const float to_ = inside ? next : 0.5f * (lo + hi);
+        const bool end = fabsf(to_ - tau) <= 1e-7f || hi - lo <= 1e-7f;
+        tau = to_;
+        return end;
+    };
+    if (fits) {
+        each([&](float4 y) {
+            float* l0 = s_list + (2 * t) * kListCap;
+            float* l1 = l0 + kListCap;
+            if (y.x - top0 > -1.0f) l0[e0++] = y.x - top0;
+            if (y.z - top0 > -1.0f) l0[e0++] = y.z - top0;
+            if (y.y - top1 > -1.0f) l1[e1++] = y.y - top1;
+            if (y.w - top1 > -1.0f) l1[e1++] = y.w - top1;
+        });
+        __syncthreads();
+        const float* list = s_list + warp * kListCap;
+        float tau = -1.0f, lo = -1.0f, hi = 0.0f;
+        for (int it = 0; it < 60; ++it) {
+            float f = 0.0f, df = 0.0f;
+            for (int i = lane; i < mine; i += 32) gain(list[i], tau, f, df);
+#pragma unroll
+            for (int k = 16; k; k >>= 1) {
+                f += __shfl_xor_sync(~0u, f, k);
+                df += __shfl_xor_sync(~0u, df, k);
+            }
+            if (step(f, df, lo, hi, tau)) break;
+        }
+        if (lane == 0) s_top[0][warp] = tau;
+    } else {
+        // the lists do not fit: every step reads the tiles again, all rows at once
+        float tau[2] = {-1.0f, -1.0f}, lo[2] = {-1.0f, -1.0f}, hi[2] = {0.0f, 0.0f};
+        for (int it = 0; it < 60; ++it) {
+            float f[2] = {0.0f, 0.0f}, df[2] = {0.0f, 0.0f};
+            each([&](float4 y) {
+                gain(y.x - top0, tau[0], f[0], df[0]);
+                gain(y.z - top0, tau[0], f[0], df[0]);
+                gain(y.y - top1, tau[1], f[1], df[1]);
+                gain(y.w - top1, tau[1], f[1], df[1]);
+            });
+            bool end = true;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+#pragma unroll
+                for (int k = 4; k; k >>= 1) {
+                    f[e] += __shfl_xor_sync(~0u, f[e], k);
+                    df[e] += __shfl_xor_sync(~0u, df[e], k);
+                }
+                if ((lane & 7) == 0) s_sum[warp][2 * t + e][0] = f[e], s_sum[warp][2 * t + e][1] = df[e];
+            }
+            __syncthreads();
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                float sf = 0.0f, sd = 0.0f;
+                for (int w = 0; w < 8; ++w) sf += s_sum[w][2 * t + e][0], sd += s_sum[w][2 * t + e][1];
+                const bool live = (e ? top1 : top0) > -INFINITY && (e ? top1 : top0) < INFINITY;
+                if (live) end &= step(sf, sd, lo[e], hi[e], tau[e]);
+            }
+            if (__syncthreads_and(end)) break;
+        }
+        if (warp == 0 && (lane & 7) == 0) s_top[0][2 * t] = tau[0], s_top[0][2 * t + 1] = tau[1];
+    }
+    __syncthreads();
+    if (tid < 8) {
+        const float y = s_tau[tid];
+        tau_out[tid] = y == -INFINITY ? INFINITY : y == INFINITY ? NAN : y + s_top[0][tid];
+    }
+}
+
+// ---- host --------------------------------------------------------------------------
+template <int NT>
+constexpr int warps_of() { return NT == 1 ? 8 : 4; }
+constexpr int ctas_of(int nt) { return nt == 1 ? 2 : 3; }        // an SM holds
+constexpr int kSms = 148;
+
+int row_tiles(const Shape& s, bool lists) { return (lists ? s.G : s.T * s.G) > 8 ? 2 : 1; }
+
+Plan make_plan(const Shape& s, int keep) {
+    Plan p;
+    const int nt = row_tiles(s, keep > 0);
+    p.U = keep ? s.B * s.T : s.B;
+    p.R = keep ? s.G : s.T * s.G;
+    p.tiles = (p.R + 8 * nt - 1) / (8 * nt);
+    p.keep = keep;
+    p.cap = ((keep ? keep : s.width) * (s.P / kBlock) + kTile - 1) / kTile;
+    // Short caches, and calls with many items a CTA, are left whole: an item's only
+    // CTA writes the output itself and nothing is joined.
+    const int64_t items = (int64_t)p.U * p.tiles * s.H;
+    p.split = p.cap > 32 && items < 8 * kSms * ctas_of(nt);
+    p.least = kItemCost + (nt == 1 ? 8 : 4);
+    p.vec = 0;
+    return p;
+}
+
+size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
+
+// Offsets of the workspace's parts; its size.
+size_t lay_out(const Shape& s, const Plan& p, void* base, Space* w) {
+    const int nt = row_tiles(s, p.keep > 0), rows = 8 * nt;
+    const int64_t items = (int64_t)p.U * p.tiles * s.H, slots = 2ll * kSms * ctas_of(nt);
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        char* q = (char*)base + at;
+        at += up256(bytes);
+        return q;
+    };
+    Space x{};
+    x.run = (int64_t*)take(((size_t)p.U + 1) * 8);
+    if (p.split) {
+        x.part = (float*)take((size_t)slots * rows * s.d * 4);
+        x.part_ml = (float*)take((size_t)slots * 2 * rows * 4);
+    }
+    if (s.alpha != 1.0f) {
+        x.score = (float4*)take((size_t)items * p.cap * kTile * nt * 512);
+        x.top = (float*)take((size_t)items * p.cap * rows * 4);
+        x.tau = (float*)take((size_t)items * rows * 4);
+    }
+    if (w) *w = x;
+    return at;
+}
+
+template <int D, int NT, int MODE>
+cudaError_t launch_walk(const Args& a, cudaStream_t st) {
+    constexpr int W = warps_of<NT>();
+    const int smem = (int)sizeof(Smem<D, NT, W>);
+    auto kernel = walk_kernel<D, NT, W, MODE>;
+    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    const int64_t items = (int64_t)a.p.U * a.p.tiles * a.s.H;
+    const unsigned grid = a.p.split ? kSms * ctas_of(NT) : (unsigned)items;
+    kernel<<<grid, W * 32, smem, st>>>(a);
+    note_launch();
+    return cudaGetLastError();
+}
+
+template <int D, int NT>
+cudaError_t launch(const Args& a, cudaStream_t st) {
+    const int64_t items = (int64_t)a.p.U * a.p.tiles * a.s.H;
+    if (items * 8 * NT > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    cudaError_t e;
+    if (a.s.alpha == 1.0f) {
+        e = launch_walk<D, NT, kSoftmax>(a, st);
+    } else {
+        e = launch_walk<D, NT, kScores>(a, st);
+        if (e != cudaSuccess) return e;
+        const int smem = 8 * kListCap * 4;
+        e = cudaFuncSetAttribute(threshold_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (e != cudaSuccess) return e;
+        threshold_kernel<NT><<<(unsigned)(items * NT), 256, smem, st>>>(a);
+        note_launch();
+        e = cudaGetLastError();
+        if (e == cudaSuccess) e = launch_walk<D, NT, kValues>(a, st);
+    }
+    if (e != cudaSuccess || !a.p.split) return e;
+    combine_kernel<D, NT><<<(unsigned)(items * 8 * NT), 128, 0, st>>>(a);
+    note_launch();
+    return cudaGetLastError();
 }
 
 }  // namespace
 
 size_t attend_workspace(const Shape& s, int keep) {
-    const size_t n = (size_t)(keep ? keep : s.width) * s.P;
-    return (size_t)s.B * s.T * s.HQ * n * 4 + 16;
+    return lay_out(s, make_plan(s, keep), nullptr, nullptr) + 16;
 }
 
 cudaError_t attend(const Shape& s, const void* Q, Strides qs, const uint8_t* pool, const int32_t* table,
                    const int32_t* lengths, const int32_t* list, int keep, void* O, void* ws, int* err,
                    cudaStream_t st) {
-    rows_kernel<<<(unsigned)(s.B * s.T * s.HQ), 128, 0, st>>>(
-        s, (const __nv_bfloat16*)Q, qs, pool, table, lengths, list, keep, (__nv_bfloat16*)O, (float*)ws,
-        (list ? keep : s.width) * s.P, err);
-    note_launch();
-    return cudaGetLastError();
+    Args a;
+    a.s = s;
+    a.p = make_plan(s, keep);
+    lay_out(s, a.p, ws, &a.w);
+    a.qs = qs;
+    a.Q = (const __nv_bfloat16*)Q;
+    a.pool = pool;
+    a.table = table;
+    a.lengths = lengths;
+    a.list = list;
+    a.O = (__nv_bfloat16*)O;
+    a.err = err;
+    a.p.vec = (reinterpret_cast<uintptr_t>(Q) & 15) == 0 && qs.b % 8 == 0 && qs.t % 8 == 0 && qs.h % 8 == 0;
+    const bool two = row_tiles(s, keep > 0) == 2;
+    switch (s.d) {
+        case 32: return two ? launch<32, 2>(a, st) : launch<32, 1>(a, st);
+        case 64: return two ? launch<64, 2>(a, st) : launch<64, 1>(a, st);
+        case 96: return two ? launch<96, 2>(a, st) : launch<96, 1>(a, st);
+        default: return two ? launch<128, 2>(a, st) : launch<128, 1>(a, st);
+    }
 }
 
 }  // namespace cache

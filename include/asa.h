@@ -291,7 +291,10 @@ int asa_cache_select(const asa_cache_params* p, const void* Q, const int64_t q_s
  * position lengths[b] - T + t, sees the keys up to its own position -- with
  * pages (int32 [B, T, kv_heads, keep], no page twice, -1 ignored) only those of
  * its key head's listed pages.  O contiguous [B, T, heads, d] bf16; rows that
- * see no key are zero, rows of a query holding a NaN or an infinity NaN. */
+ * see no key are zero, rows of a query holding a NaN or an infinity NaN.  A NaN
+ * among the keys a query sees makes its row NaN, one among the values their
+ * group's 32 channels (under alpha-entmax surely so only where it has weight);
+ * what a query does not see does not reach it. */
 int asa_cache_attention(const asa_cache_params* p, const void* Q, const int64_t q_strides[3],
                         const void* pool, const int32_t* block_table, const int32_t* lengths,
                         const int32_t* pages, int keep, void* O, void* ws, size_t ws_bytes,

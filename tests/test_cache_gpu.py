@@ -298,6 +298,8 @@ def test_nan_in_places_nobody_sees(cuda, alpha):
     assert torch.isnan(o[:, 2:]).all()                        # NaN keys: NaN scores, a NaN row
     values = torch.zeros(1, 2, H, d, device="cuda").bfloat16()
     sa().cache_write(values, bad, cache, dev(table), dev([88]))
+    if alpha != 1.0:
+        q[:, 2:] = 0.0                                        # equal weights: a NaN of weight 0 need not show
     o = sa().cache_attention(q, cache, dev(table), dev(lengths), alpha=alpha)
     check_attention(o[:, :2], q[:, :2], clean, [88], P, alpha, d ** -0.5)
     assert torch.isnan(o[:, 2:, :, :32]).all() and torch.isfinite(o[:, 2:, :, 32:]).all()
