@@ -54,6 +54,7 @@ struct Plan {
     int cap;                          // tiles an item can have at most
     int split;                        // items are cut into equal runs (else one CTA an item)
     int vec;                          // q rows may be read 16 bytes at a time
+    int page_shift;                   // log2 of the blocks of a page
     int least;                        // tiles a run has at least
 };
 
@@ -87,6 +88,13 @@ __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uin
     asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// The same onto zero.
+__device__ __forceinline__ void mma0(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                     uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
@@ -206,14 +214,24 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* s_warp, int64_
 struct Segment { int u, item, from, n, of; };         // tiles from .. from + n - 1 of an item's `of`
 struct Info { int pos0, pos1, tile, seg; };           // a ring stage: its blocks' first positions, where it belongs
 
+// A segment's query rows, made ready by one warp for all.
+template <int NG, int NT>
+struct Rows {
+    uint32_t q[NT][4 * NG + 1][32];                   // B fragments, and the group sums' halves
+    float factor[8 * NT];                             // a score's, from the product's unit
+    int pos[8 * NT];                                  // the rows' positions, -1 before the first key and past the last row
+    int out[8 * NT];                                  // their rows of O
+};
+
 template <int D, int NT, int W>
 struct Smem {
     static constexpr int kStride = D + 4;             // a float4 of each of 8 rows of lanes: no bank twice
     alignas(128) uint8_t ring[W][kStages][2 * kTile * block_bytes(D)];
     float4 o[W / 2][8 * NT][kStride / 4];
     float m[W][8 * NT], l[W][8 * NT];
-    uint64_t full[W][kStages];
+    Rows<D / 32, NT> rows[2];
     Info info[W][kStages];
+    uint64_t full[W][kStages];
     Segment seg[kSegments];
     int segs;
     int64_t next;
@@ -231,7 +249,6 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, t = lane & 3;
     const Shape& s = a.s;
     const int per = a.p.tiles * s.H;                  // items of a unit
-    const int per_page = s.P / kBlock;
 
     if (lane == 0) {
         for (int i = 0; i < kStages; ++i) sm100::mbar_init(&sm.full[warp][i], 1);
@@ -272,6 +289,19 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
             while (x >= before) before = load_chunk(chunk + NTHR, before);
         }
     }
+    // where this lane's operands lie in a stage: tokens t0, t0 + 8 of a block of keys, ta, tb
+    // and those 8 on of a block of values
+    const int t0 = token_of(r), ta = token_of(2 * t), tb = ta ^ 1;
+    const uint8_t* const ring = sm.ring[warp][0];
+    constexpr int kStage = 2 * kTile * BB;
+    const int at_kc = t0 * RB + t * 4 * NG, at_kp = kBlock * RB + t0 * PB;
+    // (lanes past the last group read a scale; their part of q's sums is zero)
+    const int at_kz = at_kp + (NG == 4 || t < NG ? 2 * (NG + t) : 0);
+    const int at_vc = kTile * BB + r * 2 * NG, at_vp = kTile * BB + kBlock * RB;
+    const int at_vz = at_vp + 2 * NG + 2 * (NG == 4 ? r & 3 : r < NG ? r : 0);
+    // the product with the offsets has a group a row, and a row of ones that sums the weights
+    const uint32_t z_and = r < NG ? ~0u : 0u, z_or = r == NG ? 0x3c003c00u : 0u;
+
     int stage_in = 0, stage_out = 0;                  // the ring's next stage to fill and to read
     uint32_t parity = 0;                              // of the stage to read
     bool lost = false;
@@ -312,28 +342,23 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
         const int segs = sm.segs;
         x = sm.next;
 
-        // where the rows of an item stand
-        auto token_of_row = [&](int u, int tile, int row) { return a.list ? u % s.T : (tile * ROWS + row) / s.G; };
-        auto head_of_row = [&](int h, int tile, int row) {
-            return h * s.G + (a.list ? tile * ROWS + row : (tile * ROWS + row) % s.G);
-        };
-        auto position = [&](int u, int tile, int row) -> int {   // -1 before the first key, and past the last row
-            if (tile * ROWS + row >= a.p.R) return -1;
-            const long long len = __ldg(a.lengths + (a.list ? u / s.T : u));
-            return (int)max(-1ll, min(len - s.T + token_of_row(u, tile, row), (long long)s.width * s.P - 1));
-        };
-
         // ---- the tiles that this warp reads, fetched ahead across segments -----------
+        auto token_of_row = [&](int u, int row) { return a.list ? u % s.T : row / s.G; };
+        auto position = [&](int u, int row) -> int {  // of an item's row (its tile's first row added)
+            const long long len = __ldg(a.lengths + (a.list ? u / s.T : u));
+            return (int)max(-1ll, min(len - s.T + token_of_row(u, row), (long long)s.width * s.P - 1));
+        };
         int ahead = -1, mine = 0, c = 0;              // the segment being fetched, the warp's tiles of it, 32 c of them passed
         uint32_t there = 0;                           // of the 32 that the lanes have looked up
-        int rec0 = -1, rec1 = -1, pos0 = 0, pos1 = 0; // this lane's: record and first position of its blocks
+        const uint8_t *at0 = nullptr, *at1 = nullptr; // this lane's: its blocks' records and first positions
+        int pos0 = 0, pos1 = 0;
         auto locate = [&](const Segment& g, int k) -> bool {
-            rec0 = rec1 = -1;
+            at0 = at1 = nullptr;
             pos0 = pos1 = kNone;
             if (k >= mine) return false;
             const int j = g.from + warp + k * W, h = g.item / a.p.tiles, tile = g.item % a.p.tiles;
             const int64_t item_no = (int64_t)g.u * per + g.item;
-            const int pos_hi = position(g.u, tile, min(ROWS, a.p.R - tile * ROWS) - 1);
+            const int pos_hi = position(g.u, min(tile * ROWS + ROWS, a.p.R) - 1);
             bool wanted = true;
             if constexpr (MODE == kValues) {          // only tiles that a threshold leaves weight in
                 const float* top = a.w.top + (item_no * a.p.cap + j) * ROWS;
@@ -348,29 +373,26 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
             if (wanted) {
                 const int32_t* table_b = a.table + (int64_t)(a.list ? g.u / s.T : g.u) * s.width;
                 const int32_t* list = a.list ? a.list + ((int64_t)g.u * s.H + h) * a.p.keep : nullptr;
-                auto block = [&](int blk, int& rec, int& pos) {
-                    int page = blk / per_page;
+                auto block = [&](int blk, const uint8_t*& at, int& pos) {
+                    int page = blk >> a.p.page_shift;
+                    const int in_page = blk & ((1 << a.p.page_shift) - 1);
                     if (list) page = page < a.p.keep ? __ldg(list + page) : -1;
                     if (page < 0 || page >= s.width) return;
-                    const int first = page * s.P + blk % per_page * kBlock;
+                    const int first = page * s.P + in_page * kBlock;
                     if (first > pos_hi) return;
                     const int id = __ldg(table_b + page);
                     if (id >= 0 && id < s.pages) {
-                        rec = id * s.H + h;
+                        at = a.pool + ((int64_t)id * s.H + h) * s.rec + in_page * BB;
                         pos = first;
                     } else if (a.err) {
                         atomicCAS(a.err, 0, ASA_ERR_INVALID);
                     }
                 };
-                block(kTile * j, rec0, pos0);
-                if (per_page == 1) {
-                    block(kTile * j + 1, rec1, pos1);
-                } else if (rec0 >= 0) {               // the tile lies in one page
-                    rec1 = rec0;
-                    if (pos0 + kBlock <= pos_hi) pos1 = pos0 + kBlock;
-                }
+                block(kTile * j, at0, pos0);
+                if (a.p.page_shift == 0) block(kTile * j + 1, at1, pos1);
+                else if (at0 && pos0 + kBlock <= pos_hi) pos1 = pos0 + kBlock;   // the tile lies in one page
             }
-            const bool found = rec0 >= 0 || rec1 >= 0;
+            const bool found = at0 || at1;
             if constexpr (MODE == kScores)
                 if (!found)
                     for (int i = 0; i < ROWS; ++i) a.w.top[(item_no * a.p.cap + j) * ROWS + i] = -INFINITY;
@@ -391,26 +413,21 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
             }
             const int k = __ffs(there) - 1;
             there &= there - 1;
-            const int r0 = __shfl_sync(~0u, rec0, k), r1 = __shfl_sync(~0u, rec1, k);
-            const int p0 = __shfl_sync(~0u, pos0, k), p1 = __shfl_sync(~0u, pos1, k);
-            if (lane == 0) {
-                const int j = sm.seg[ahead].from + warp + (32 * (c - 1) + k) * W;
-                sm.info[warp][stage_in] = Info{p0, p1, j, ahead};
+            if (lane == k) {                          // the lane that looked it up issues its copies
+                sm.info[warp][stage_in] = Info{pos0, pos1, sm.seg[ahead].from + warp + (32 * (c - 1) + k) * W, ahead};
                 uint8_t* dst = sm.ring[warp][stage_in];
                 uint64_t* bar = &sm.full[warp][stage_in];
                 constexpr int kParts = MODE == kSoftmax ? 2 : 1;
-                if (per_page > 1) {                   // two blocks on end
-                    const uint8_t* src = a.pool + r0 * s.rec + (int64_t)(kTile * j % per_page) * BB;
+                if (a.p.page_shift) {                 // two blocks on end
                     sm100::mbar_expect_tx(bar, kParts * kTile * BB);
-                    if (MODE != kValues) bulk_load(dst, src, kTile * BB, bar);
-                    if (MODE != kScores) bulk_load(dst + kTile * BB, src + s.rec / 2, kTile * BB, bar);
+                    if (MODE != kValues) bulk_load(dst, at0, kTile * BB, bar);
+                    if (MODE != kScores) bulk_load(dst + kTile * BB, at0 + s.rec / 2, kTile * BB, bar);
                 } else {
-                    sm100::mbar_expect_tx(bar, kParts * BB * ((r0 >= 0) + (r1 >= 0)));
+                    sm100::mbar_expect_tx(bar, kParts * BB * ((at0 ? 1 : 0) + (at1 ? 1 : 0)));
 #pragma unroll
                     for (int i = 0; i < kTile; ++i) {
-                        const int rec = i ? r1 : r0;
-                        if (rec < 0) continue;
-                        const uint8_t* src = a.pool + rec * s.rec;
+                        const uint8_t* src = i ? at1 : at0;
+                        if (!src) continue;
                         if (MODE != kValues) bulk_load(dst + i * BB, src, BB, bar);
                         if (MODE != kScores) bulk_load(dst + (kTile + i) * BB, src + s.rec / 2, BB, bar);
                     }
@@ -422,91 +439,102 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
         };
         for (int i = 0; i < kStages; ++i) fetch();
 
+        // ---- queries as B fragments, a power of two a row: n-tile nt of segment sg --------
+        auto make_rows = [&](int sg, int nt) {
+            const Segment g = sm.seg[sg];
+            auto& out = sm.rows[sg & 1];
+            const int h = g.item / a.p.tiles, row = g.item % a.p.tiles * ROWS + 8 * nt + r;
+            const int b = a.list ? g.u / s.T : g.u;
+            const bool real = row < a.p.R;
+            const int tq = token_of_row(g.u, row), hq = h * s.G + (a.list ? row : row % s.G);
+            if (t == 0) {
+                out.pos[8 * nt + r] = real ? position(g.u, row) : -1;
+                out.out[8 * nt + r] = (b * s.T + tq) * s.HQ + hq;
+            }
+            if constexpr (MODE != kValues) {
+                float q[NG][8], big = 0.0f;
+                const __nv_bfloat16* src = a.Q + b * a.qs.b + tq * a.qs.t + hq * a.qs.h + 8 * t;
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    uint32_t w[4] = {0u, 0u, 0u, 0u};
+                    if (real && a.p.vec) {
+                        const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + 32 * i));
+                        w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+                    } else if (real) {
+                        const uint16_t* e = reinterpret_cast<const uint16_t*>(src + 32 * i);
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) w[k] = __ldg(e + 2 * k) | (uint32_t)__ldg(e + 2 * k + 1) << 16;
+                    }
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        q[i][2 * k] = __uint_as_float(w[k] << 16);
+                        q[i][2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
+                        big = fmaxf(big, fmaxf(fabsf(q[i][2 * k]), fabsf(q[i][2 * k + 1])));
+                    }
+                }
+                float sum = 0.0f;                     // a NaN or an infinity makes the sum of 0 * q NaN
+#pragma unroll
+                for (int i = 0; i < NG; ++i)
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) sum = fmaf(q[i][k], 0.0f, sum);
+                big = fmaxf(big, __shfl_xor_sync(~0u, big, 1));
+                big = fmaxf(big, __shfl_xor_sync(~0u, big, 2));
+                const bool bad = (__ballot_sync(~0u, sum != sum) >> (lane & 28)) & 15u;
+                // big * 2^up lies in [2^13, 2^14), but for what is below 2^-113
+                const int up = big == 0.0f || bad ? 0 : 13 - max((int)(__float_as_uint(big) >> 23) - 127, -113);
+                const float f = bad ? NAN : pow2i(up), f16 = bad ? NAN : pow2i(up - 4);
+                float own = 0.0f;
+#pragma unroll
+                for (int i = 0; i < NG; ++i) {
+                    // channels 8t .. 8t + 7 of the group, in the order that masking a word of codes gives
+                    out.q[nt][4 * i][lane] = pack(q[i][0] * f, q[i][4] * f);
+                    out.q[nt][4 * i + 1][lane] = pack(q[i][1] * f16, q[i][5] * f16);
+                    out.q[nt][4 * i + 2][lane] = pack(q[i][2] * f, q[i][6] * f);
+                    out.q[nt][4 * i + 3][lane] = pack(q[i][3] * f16, q[i][7] * f16);
+                    float v = 0.0f;
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) v += q[i][k] * f16;
+                    v += __shfl_xor_sync(~0u, v, 1);
+                    v += __shfl_xor_sync(~0u, v, 2);
+                    own = t == i ? v : own;
+                }
+                const float hi = __half2float(__float2half_rn(own));
+                out.q[nt][4 * NG][lane] = pack(hi, own - hi);
+                if (t == 0) out.factor[8 * nt + r] = scalbnf(s.scale * (MODE == kSoftmax ? kLog2e : 1.0f), 24 - up);
+            }
+        };
+        if (warp < NT && segs) make_rows(0, warp);
+        __syncthreads();
+
         for (int sg = 0; sg < segs; ++sg) {
             const Segment g = sm.seg[sg];
-            const int h = g.item / a.p.tiles, tile = g.item % a.p.tiles;
+            const int tile = g.item % a.p.tiles;
             const int64_t item_no = (int64_t)g.u * per + g.item;
-            const int b = a.list ? g.u / s.T : g.u;
             const int rows = min(ROWS, a.p.R - tile * ROWS);
-            const int pos_hi = position(g.u, tile, rows - 1), pos_lo = position(g.u, tile, 0);   // rows stand in order
-
-            // ---- queries as B fragments, a power of two a row -----------------------
+            const auto& mine_rows = sm.rows[sg & 1];
+            const int pos_hi = mine_rows.pos[rows - 1], pos_lo = mine_rows.pos[0];   // rows stand in order
             uint32_t qf[NT][NG][4], qz[NT];
             float rf[NT][2];                          // scores: the factor of rows 2t, 2t + 1; values: their thresholds
-            int pos[NT][2];
-            float m[NT][2], oz[NT][4], o[NT][2 * NG][4];   // oz: by group the offsets' sums, and the weights'
-            float lift = 0.0f;                        // log2 by which weights are lowered for large scales
+            float m[NT][2], room[NT][2];              // references, and how far above them a score may lie (-inf: unset)
+            float oz[NT][4], o[NT][2 * NG][4];        // oz: by group the offsets' sums, and the weights'
+            int lift = 0;                             // log2 by which weights are lowered for large scales
+            uint32_t s_most = 0x4000u;                // the fp16 scale 2^(lift + 1) that they allow
+            const float* tau = a.w.tau + item_no * ROWS;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 if constexpr (MODE != kValues) {
-                    const int row = 8 * nt + r;
-                    float q[NG][8], big = 0.0f;
-                    bool bad = false;
-                    const __nv_bfloat16* src =
-                        row < rows ? a.Q + b * a.qs.b + token_of_row(g.u, tile, row) * a.qs.t +
-                                         head_of_row(h, tile, row) * a.qs.h + 8 * t
-                                   : nullptr;
 #pragma unroll
-                    for (int i = 0; i < NG; ++i) {
-                        uint32_t w[4] = {0u, 0u, 0u, 0u};
-                        if (src && a.p.vec) {
-                            const uint4 v = __ldg(reinterpret_cast<const uint4*>(src + 32 * i));
-                            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
-                        } else if (src) {
-                            const uint16_t* e = reinterpret_cast<const uint16_t*>(src + 32 * i);
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) w[k] = __ldg(e + 2 * k) | (uint32_t)__ldg(e + 2 * k + 1) << 16;
-                        }
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) {
-                            q[i][2 * k] = __uint_as_float(w[k] << 16);
-                            q[i][2 * k + 1] = __uint_as_float(w[k] & 0xffff0000u);
-                        }
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            big = fmaxf(big, fabsf(q[i][k]));
-                            bad |= !isfinite(q[i][k]);
-                        }
-                    }
-                    big = fmaxf(big, __shfl_xor_sync(~0u, big, 1));
-                    big = fmaxf(big, __shfl_xor_sync(~0u, big, 2));
-                    const bool row_bad = (__ballot_sync(~0u, bad) >> (lane & 28)) & 15u;
-                    // big * 2^up lies in [2^13, 2^14), but for what is below 2^-113
-                    const int up = big == 0.0f || row_bad ? 0 : 13 - max((int)(__float_as_uint(big) >> 23) - 127, -113);
-                    const float f = pow2i(up), f16 = pow2i(up - 4);
-                    float own = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < NG; ++i) {
-                        if (row_bad) {
-#pragma unroll
-                            for (int k = 0; k < 8; ++k) q[i][k] = NAN;
-                        }
-                        // channels 8t .. 8t + 7 of the group, in the order that masking a word of codes gives
-                        qf[nt][i][0] = pack(q[i][0] * f, q[i][4] * f);
-                        qf[nt][i][1] = pack(q[i][1] * f16, q[i][5] * f16);
-                        qf[nt][i][2] = pack(q[i][2] * f, q[i][6] * f);
-                        qf[nt][i][3] = pack(q[i][3] * f16, q[i][7] * f16);
-                        float v = 0.0f;
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) v += q[i][k] * f16;
-                        v += __shfl_xor_sync(~0u, v, 1);
-                        v += __shfl_xor_sync(~0u, v, 2);
-                        own = t == i ? v : own;
-                    }
-                    const float hi = __half2float(__float2half_rn(own));
-                    qz[nt] = pack(hi, own - hi);
-                    const float back = scalbnf(s.scale * (MODE == kSoftmax ? kLog2e : 1.0f), 24 - up);
-                    rf[nt][0] = __shfl_sync(~0u, back, 8 * t);
-                    rf[nt][1] = __shfl_sync(~0u, back, 8 * t + 4);
+                    for (int i = 0; i < 4 * NG; ++i) qf[nt][i / 4][i % 4] = mine_rows.q[nt][i][lane];
+                    qz[nt] = mine_rows.q[nt][4 * NG][lane];
                 }
+                const float2 f2 = MODE == kValues ? *reinterpret_cast<const float2*>(tau + 8 * nt + 2 * t)
+                                                  : *reinterpret_cast<const float2*>(&mine_rows.factor[8 * nt + 2 * t]);
+                rf[nt][0] = f2.x;
+                rf[nt][1] = f2.y;
+                m[nt][0] = m[nt][1] = MODE == kSoftmax ? 0.0f : -kTop;
+                room[nt][0] = room[nt][1] = -INFINITY;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int row = 8 * nt + 2 * t + e;
-                    pos[nt][e] = position(g.u, tile, row);
-                    m[nt][e] = MODE == kSoftmax ? kLow : -kTop;
-                    oz[nt][e] = oz[nt][e + 2] = 0.0f;
-                    if constexpr (MODE == kValues) rf[nt][e] = a.w.tau[item_no * ROWS + row];
-                }
+                for (int e = 0; e < 4; ++e) oz[nt][e] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < 2 * NG; ++i)
 #pragma unroll
@@ -514,38 +542,55 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
             }
 
             // ---- the segment's tiles ---------------------------------------------------
-            while (in_flight && sm.info[warp][stage_out].seg == sg) {
+            while (in_flight) {
                 const Info info = sm.info[warp][stage_out];
-                if (!wait_full(&sm.full[warp][stage_out], parity, s.spins, a.err)) lost = true;
+                if (info.seg != sg) break;
+                if (!sm100::mbar_try(&sm.full[warp][stage_out], parity) &&
+                    !wait_full(&sm.full[warp][stage_out], parity, s.spins, a.err))
+                    lost = true;
                 __syncwarp();
-                const uint8_t* kb = sm.ring[warp][stage_out];
-                const uint8_t* vb = kb + kTile * BB;
+                const uint8_t* const st = ring + stage_out * kStage;
                 // every row sees all of both blocks
                 const bool whole = max(info.pos0, info.pos1) + kBlock - 1 <= pos_lo;
-                const int t0 = token_of(r), t1 = t0 + 8;           // the tokens of this lane's scores, in a block
                 float v[kTile][NT][4];
+                auto each = [&](auto fn) {            // of the scores: (block, n-tile, element, its token)
+#pragma unroll
+                    for (int i = 0; i < kTile; ++i)
+#pragma unroll
+                        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) fn(i, nt, e);
+                };
+                auto mask = [&]() {                   // scores of keys that a row does not see
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const int2 pos = *reinterpret_cast<const int2*>(&mine_rows.pos[8 * nt + 2 * t]);
+#pragma unroll
+                        for (int i = 0; i < kTile; ++i)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e)
+                                if ((i ? info.pos1 : info.pos0) + t0 + (e < 2 ? 0 : 8) > (e & 1 ? pos.y : pos.x))
+                                    v[i][nt][e] = -INFINITY;
+                    }
+                };
 
                 if constexpr (MODE != kValues) {
-                    // scores of tokens t0, t1 and rows 2t, 2t + 1, group by group
+                    // scores of tokens t0, t0 + 8 and rows 2t, 2t + 1, group by group
 #pragma unroll
                     for (int i = 0; i < kTile; ++i) {
-                        const uint8_t* blk = kb + i * BB;
                         uint32_t w0[NG], w1[NG], p0[NS], p1[NS];
-                        lds<NG>(blk + t0 * RB + t * 4 * NG, w0);
-                        lds<NG>(blk + t1 * RB + t * 4 * NG, w1);
-                        const uint8_t* par = blk + kBlock * RB;
-                        lds_halves<NG>(par + t0 * PB, p0);
-                        lds_halves<NG>(par + t1 * PB, p1);
-                        // (lanes past the last group read a scale; their part of q's sums is zero)
-                        const int zt = NG == 4 || t < NG ? 2 * (NG + t) : 0;
-                        uint32_t z0 = *reinterpret_cast<const uint16_t*>(par + t0 * PB + zt);
-                        uint32_t z1 = *reinterpret_cast<const uint16_t*>(par + t1 * PB + zt);
+                        lds<NG>(st + at_kc + i * BB, w0);
+                        lds<NG>(st + at_kc + i * BB + 8 * RB, w1);
+                        lds_halves<NG>(st + at_kp + i * BB, p0);
+                        lds_halves<NG>(st + at_kp + i * BB + 8 * PB, p1);
+                        uint32_t z0 = *reinterpret_cast<const uint16_t*>(st + at_kz + i * BB);
+                        uint32_t z1 = *reinterpret_cast<const uint16_t*>(st + at_kz + i * BB + 8 * PB);
                         z0 = __byte_perm(z0, z0, 0x1010);
                         z1 = __byte_perm(z1, z1, 0x1010);
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
-                            float cz[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                            mma(cz, z0, z1, 0u, 0u, qz[nt], 0u);
+                            float cz[4];
+                            mma0(cz, z0, z1, 0u, 0u, qz[nt], 0u);
 #pragma unroll
                             for (int e = 0; e < 4; ++e) v[i][nt][e] = cz[e] * 9.5367431640625e-7f;   // 2^-20: codes and halves count 2^-24, 2^-4
                         }
@@ -556,9 +601,9 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                             const float f0 = k & 1 ? s0.y : s0.x, f1 = k & 1 ? s1.y : s1.x;
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) {
-                                float acc[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                                mma(acc, x0 & 0x000f000fu, y0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x00f000f0u,
-                                    qf[nt][k][0], qf[nt][k][1]);
+                                float acc[4];
+                                mma0(acc, x0 & 0x000f000fu, y0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x00f000f0u,
+                                     qf[nt][k][0], qf[nt][k][1]);
                                 mma(acc, x8 & 0x000f000fu, y8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x00f000f0u,
                                     qf[nt][k][2], qf[nt][k][3]);
                                 v[i][nt][0] = fmaf(acc[0], f0, v[i][nt][0]);
@@ -572,20 +617,19 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                 if constexpr (MODE == kScores) {
                     const float am1 = s.alpha - 1.0f;
                     const int64_t place = item_no * a.p.cap + info.tile;
+                    each([&](int i, int nt, int e) {
+                        const float y = v[i][nt][e] * rf[nt][e & 1];
+                        v[i][nt][e] = y != y ? y : am1 * fminf(fmaxf(y, -10.0f), 10.0f);
+                    });
+                    if (!whole) mask();
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
                         float top[2] = {-INFINITY, -INFINITY};
 #pragma unroll
                         for (int i = 0; i < kTile; ++i) {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float y = v[i][nt][e] * rf[nt][e & 1];
-                                float z = am1 * fminf(fmaxf(y, -10.0f), 10.0f);
-                                if (y != y) z = NAN;
-                                if (!whole && (i ? info.pos1 : info.pos0) + (e < 2 ? t0 : t1) > pos[nt][e & 1]) z = -INFINITY;
-                                top[e & 1] = fmaxf(top[e & 1], z != z ? INFINITY : z);   // a NaN score: its row is NaN
-                                v[i][nt][e] = z;
-                            }
+                            for (int e = 0; e < 4; ++e)   // a NaN score: its row is NaN
+                                top[e & 1] = fmaxf(top[e & 1], v[i][nt][e] != v[i][nt][e] ? INFINITY : v[i][nt][e]);
                             if (8 * nt + 2 * t < rows)
                                 a.w.score[((place * kTile + i) * NT + nt) * 32 + 8 * t + r] =
                                     make_float4(v[i][nt][0], v[i][nt][1], v[i][nt][2], v[i][nt][3]);
@@ -601,6 +645,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                         if (r == 0) *reinterpret_cast<float2*>(a.w.top + place * ROWS + 8 * nt + 2 * t) = make_float2(top[0], top[1]);
                     }
                 } else {
+                    // v: a score less its row's reference (softmax), or less its threshold
                     if constexpr (MODE == kValues) {
                         const int64_t place = item_no * a.p.cap + info.tile;
 #pragma unroll
@@ -609,44 +654,34 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                             for (int nt = 0; nt < NT; ++nt) {
                                 float4 y = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
                                 if (8 * nt + 2 * t < rows) y = a.w.score[((place * kTile + i) * NT + nt) * 32 + 8 * t + r];
-                                v[i][nt][0] = y.x, v[i][nt][1] = y.y, v[i][nt][2] = y.z, v[i][nt][3] = y.w;
+                                v[i][nt][0] = y.x - rf[nt][0], v[i][nt][1] = y.y - rf[nt][1];
+                                v[i][nt][2] = y.z - rf[nt][0], v[i][nt][3] = y.w - rf[nt][1];
                             }
                     } else {
-#pragma unroll
-                        for (int i = 0; i < kTile; ++i)
-#pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    v[i][nt][e] *= rf[nt][e & 1];
-                                    if (!whole && (i ? info.pos1 : info.pos0) + (e < 2 ? t0 : t1) > pos[nt][e & 1])
-                                        v[i][nt][e] = -INFINITY;
-                                }
+                        each([&](int i, int nt, int e) { v[i][nt][e] = fmaf(v[i][nt][e], rf[nt][e & 1], -m[nt][e & 1]); });
+                        if (!whole) mask();
                     }
-                    // the values' scales: tokens ta, tb (k = 2t, 2t + 1) and those 8 on, as pairs a group
-                    const int ta = token_of(2 * t), tb = token_of(2 * t + 1);
+                    // the values' scales of tokens ta, tb (k = 2t, 2t + 1) and those 8 on, as pairs a group
                     uint32_t sp[kTile][NG][2], zp[kTile][2];
 #pragma unroll
                     for (int i = 0; i < kTile; ++i) {
-                        const uint8_t* par = vb + i * BB + kBlock * RB;
                         uint32_t ra[NS], rb[NS], rc[NS], rd[NS];
-                        lds_halves<NG>(par + ta * PB, ra);
-                        lds_halves<NG>(par + tb * PB, rb);
-                        lds_halves<NG>(par + (ta + 8) * PB, rc);
-                        lds_halves<NG>(par + (tb + 8) * PB, rd);
+                        const uint8_t *pa = st + at_vp + ta * PB + i * BB, *pb_ = st + at_vp + tb * PB + i * BB;
+                        lds_halves<NG>(pa, ra);
+                        lds_halves<NG>(pb_, rb);
+                        lds_halves<NG>(pa + 8 * PB, rc);
+                        lds_halves<NG>(pb_ + 8 * PB, rd);
 #pragma unroll
                         for (int k = 0; k < NG; ++k) {
                             const uint32_t pick = k & 1 ? 0x7632u : 0x5410u;
                             sp[i][k][0] = __byte_perm(ra[k >> 1], rb[k >> 1], pick);
                             sp[i][k][1] = __byte_perm(rc[k >> 1], rd[k >> 1], pick);
                         }
-                        // group r's offsets; row NG of that product is ones, and sums the weights
-                        zp[i][0] = zp[i][1] = r == NG ? 0x3c003c00u : 0u;
-                        if (r < NG) {
-                            const uint8_t* z = par + 2 * NG + 2 * r;
-                            zp[i][0] = *reinterpret_cast<const uint16_t*>(z + ta * PB) | (uint32_t)*reinterpret_cast<const uint16_t*>(z + tb * PB) << 16;
-                            zp[i][1] = *reinterpret_cast<const uint16_t*>(z + (ta + 8) * PB) | (uint32_t)*reinterpret_cast<const uint16_t*>(z + (tb + 8) * PB) << 16;
-                        }
+                        const uint8_t *za = st + at_vz + ta * PB + i * BB, *zb = st + at_vz + tb * PB + i * BB;
+                        zp[i][0] = __byte_perm(*reinterpret_cast<const uint16_t*>(za), *reinterpret_cast<const uint16_t*>(zb), 0x5410);
+                        zp[i][1] = __byte_perm(*reinterpret_cast<const uint16_t*>(za + 8 * PB), *reinterpret_cast<const uint16_t*>(zb + 8 * PB), 0x5410);
+                        zp[i][0] = (zp[i][0] & z_and) | z_or;
+                        zp[i][1] = (zp[i][1] & z_and) | z_or;
                     }
                     if (!whole) {
                         // Tokens that no row sees may hold anything: their scales and
@@ -680,7 +715,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                             for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                                 for (int e = 0; e < 2; ++e) {
-                                    const int see = min(max(pos[nt][e] - first + 1, 0), kBlock);
+                                    const int see = min(max(mine_rows.pos[8 * nt + 2 * t + e] - first + 1, 0), kBlock);
                                     if (bad & ((1u << see) - 1u)) oz[nt][e] = NAN;
                                 }
                         }
@@ -691,36 +726,39 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                     uint32_t sbig = hmax2(sp[0][0][0], sp[0][0][1]);
 #pragma unroll
                     for (int k = 1; k < kTile * NG; ++k) sbig = hmax2(sbig, hmax2(sp[k / NG][k % NG][0], sp[k / NG][k % NG][1]));
-                    const float2 sb = unpack(sbig);
-                    const float smax = fmaxf(sb.x, sb.y);          // NaN aside
-                    bool grow = smax > pow2i((int)lift + 1);
+                    sbig = max(sbig & 0xffffu, sbig >> 16);        // of fp16 numbers not below zero
+                    bool grow = sbig > s_most;
                     if constexpr (MODE == kSoftmax) {
-                        const float room = kTop + 0.5f - lift;
 #pragma unroll
-                        for (int i = 0; i < kTile; ++i)
+                        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) grow |= v[i][nt][e] - m[nt][e & 1] > room;
+                            for (int e = 0; e < 2; ++e)
+                                grow |= fmaxf(fmaxf(v[0][nt][e], v[0][nt][e + 2]), fmaxf(v[1][nt][e], v[1][nt][e + 2])) > room[nt][e];
                     }
                     if (__any_sync(~0u, grow)) {
-                        const uint32_t all = __reduce_max_sync(~0u, __float_as_uint(fminf(smax, kF16Max)));
-                        const float up = fmaxf(lift, (float)((int)(all >> 23) - 127));   // 2^up <= largest scale < 2^(up + 1)
+                        // NaN scales aside: what they touch is NaN whatever the weights
+                        const uint32_t all = __reduce_max_sync(~0u, min(sbig, 0x7bffu));
+                        const int up = max(lift, (int)(all >> 10) - 15);   // 2^up <= largest scale < 2^(up + 1)
 #pragma unroll
                         for (int nt = 0; nt < NT; ++nt) {
                             float f[2];
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
-                                float next = m[nt][e] + (up - lift);
+                                float by = (float)(up - lift);     // what the reference rises by
                                 if constexpr (MODE == kSoftmax) {
                                     float top = fmaxf(fmaxf(v[0][nt][e], v[0][nt][e + 2]), fmaxf(v[1][nt][e], v[1][nt][e + 2]));
                                     top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
                                     top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
                                     top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-                                    next = fmaxf(next, top - kTop + up);
+                                    const float to = top - kTop + (float)up;
+                                    if (room[nt][e] > -INFINITY) by = fmaxf(by, to);
+                                    else by = top > -INFINITY ? to : 0.0f;
+                                    if (room[nt][e] > -INFINITY || top > -INFINITY) room[nt][e] = kTop + 0.5f - (float)up;
+#pragma unroll
+                                    for (int i = 0; i < kTile; ++i) v[i][nt][e] -= by, v[i][nt][e + 2] -= by;
                                 }
-                                f[e] = exp2_fast(m[nt][e] - next);
-                                m[nt][e] = next;
+                                f[e] = exp2_fast(-by);
+                                m[nt][e] += by;
                                 oz[nt][e] *= f[e];
                             }
 #pragma unroll
@@ -729,6 +767,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                                 for (int e = 0; e < 4; ++e) o[nt][i][e] *= f[e & 1];
                         }
                         lift = up;
+                        s_most = (uint32_t)(up + 16) << 10;
                     }
                     // P, and P^T as an operand
                     uint32_t pb[kTile][NT][2];
@@ -739,13 +778,13 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                             float p[4];
 #pragma unroll
                             for (int e = 0; e < 4; ++e) {
+                                const float y = v[i][nt][e];
                                 if constexpr (MODE == kSoftmax) {
-                                    p[e] = exp2_fast(v[i][nt][e] - m[nt][e & 1]);
+                                    p[e] = exp2_fast(y);
                                 } else {
-                                    const float y = v[i][nt][e] - rf[nt][e & 1];
-                                    const float k = exp2_fast(-m[nt][e & 1]);
-                                    if (s.alpha == 1.5f) p[e] = y > 0.0f ? y * y * k : 0.0f;
-                                    else p[e] = y > 0.0f ? exp2f(log2f(y) / (s.alpha - 1.0f)) * k : 0.0f;
+                                    const float unit = exp2_fast(-m[nt][e & 1]);
+                                    if (s.alpha == 1.5f) p[e] = y > 0.0f ? y * y * unit : 0.0f;
+                                    else p[e] = y > 0.0f ? exp2f(log2f(y) / (s.alpha - 1.0f)) * unit : 0.0f;
                                     if (y != y) p[e] = y;
                                 }
                             }
@@ -757,11 +796,11 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
 #pragma unroll
                     for (int i = 0; i < kTile; ++i) {
                         uint32_t ca[NS], cb[NS], cc[NS], cd[NS];
-                        const uint8_t* code = vb + i * BB + r * 2 * NG;
-                        lds_halves<NG>(code + ta * RB, ca);
-                        lds_halves<NG>(code + tb * RB, cb);
-                        lds_halves<NG>(code + (ta + 8) * RB, cc);
-                        lds_halves<NG>(code + (tb + 8) * RB, cd);
+                        const uint8_t *qa = st + at_vc + ta * RB + i * BB, *qb = st + at_vc + tb * RB + i * BB;
+                        lds_halves<NG>(qa, ca);
+                        lds_halves<NG>(qb, cb);
+                        lds_halves<NG>(qa + 8 * RB, cc);
+                        lds_halves<NG>(qb + 8 * RB, cd);
 #pragma unroll
                         for (int k = 0; k < NG; ++k) {
                             const uint32_t pick = k & 1 ? 0x7632u : 0x5410u;
@@ -784,19 +823,29 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                 --in_flight;
                 fetch();
             }
-
-            // ---- the warps' sums together; the item's output, or this run's part of it ---
-            if constexpr (MODE != kScores) {
-                // a row's weight sum is in the lanes r = NG; scale the sums to one reference a row
+            if constexpr (MODE == kSoftmax)
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
-                        if (r == NG) {
+                        if (!(room[nt][e] > -INFINITY)) m[nt][e] = kLow;
+            // the next segment's rows, by the warps that may be first done
+            if (warp >= W - NT && sg + 1 < segs) make_rows(sg + 1, warp - (W - NT));
+
+            // ---- the warps' sums together; the item's output, or this run's part of it ---
+            if constexpr (MODE == kScores) {
+                __syncthreads();
+            } else {
+                // a row's weight sum is in the lanes r = NG; scale the sums to one reference a row
+                if (r == NG)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) {
                             sm.m[warp][8 * nt + 2 * t + e] = m[nt][e];
                             sm.l[warp][8 * nt + 2 * t + e] = oz[nt][e];
                         }
-                __syncthreads();                      // (also: sm.o is free again)
+                __syncthreads();
                 constexpr int H = W / 2;
 #pragma unroll
                 for (int half = 1; half >= 0; --half) {   // the upper warps hand theirs to the lower ones
@@ -809,13 +858,12 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                                 float top = sm.m[0][row];
 #pragma unroll
                                 for (int w = 1; w < W; ++w) top = fmaxf(top, sm.m[w][row]);
-                                const float f = exp2_fast(m[nt][e] - top);
+                                const float f = exp2_fast(m[nt][e] - top), k0 = 16777216.0f * f, k1 = 1048576.0f * f;   // codes count 2^-24 and 2^-20
 #pragma unroll
                                 for (int k = 0; k < NG; ++k) {
-                                    const float z = __shfl_sync(~0u, oz[nt][e], 4 * k + t);
-                                    constexpr float k0 = 16777216.0f, k1 = 1048576.0f;   // codes count 2^-24 and 2^-20
-                                    float4 y = make_float4(fmaf(o[nt][2 * k][e], k0, z) * f, fmaf(o[nt][2 * k][e + 2], k1, z) * f,
-                                                           fmaf(o[nt][2 * k + 1][e], k0, z) * f, fmaf(o[nt][2 * k + 1][e + 2], k1, z) * f);
+                                    const float z = __shfl_sync(~0u, oz[nt][e], 4 * k + t) * f;
+                                    float4 y = make_float4(fmaf(o[nt][2 * k][e], k0, z), fmaf(o[nt][2 * k][e + 2], k1, z),
+                                                           fmaf(o[nt][2 * k + 1][e], k0, z), fmaf(o[nt][2 * k + 1][e + 2], k1, z));
                                     float4* dst = &sm.o[warp % H][row][8 * k + r];
                                     if (half == 0) {
                                         const float4 u = *dst;
@@ -847,15 +895,13 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                         const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
                         __nv_bfloat162 y[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv),
                                                __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
-                        __nv_bfloat16* dst = a.O + (((int64_t)b * s.T + token_of_row(g.u, tile, row)) * s.HQ +
-                                                    head_of_row(h, tile, row)) * D + 4 * c4;
-                        *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<uint2*>(y);
+                        *reinterpret_cast<uint2*>(a.O + (int64_t)mine_rows.out[row] * D + 4 * c4) = *reinterpret_cast<uint2*>(y);
                     } else {
                         *reinterpret_cast<float4*>(a.w.part + (slot * ROWS + row) * D + 4 * c4) = acc;
                         if (c4 == 0) *reinterpret_cast<float2*>(a.w.part_ml + (slot * ROWS + row) * 2) = make_float2(top, sum);
                     }
                 }
-                __syncthreads();                      // sm.m, sm.o are free again
+                __syncthreads();                      // sm.m, sm.o and the rows are free again
             }
         }
         if (!a.p.split) break;
@@ -1138,6 +1184,8 @@ Plan make_plan(const Shape& s, int keep) {
     p.split = p.cap > 32 && items < 8 * kSms * ctas_of(nt);
     p.least = kItemCost + (nt == 1 ? 8 : 4);
     p.vec = 0;
+    p.page_shift = 0;
+    while (kBlock << p.page_shift < s.P) ++p.page_shift;
     return p;
 }
 
