@@ -726,7 +726,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                     uint32_t sbig = hmax2(sp[0][0][0], sp[0][0][1]);
 #pragma unroll
                     for (int k = 1; k < kTile * NG; ++k) sbig = hmax2(sbig, hmax2(sp[k / NG][k % NG][0], sp[k / NG][k % NG][1]));
-                    sbig = max(sbig & 0xffffu, sbig >> 16);        // of fp16 numbers not below zero
+                    sbig = max(sbig & 0x7fffu, sbig >> 16 & 0x7fffu);   // (no scale is far below zero)
                     bool grow = sbig > s_most;
                     if constexpr (MODE == kSoftmax) {
 #pragma unroll

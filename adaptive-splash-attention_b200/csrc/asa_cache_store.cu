@@ -2,7 +2,7 @@
 // keeping the pages' bounds, and reading both back.
 //
 // Per group of 32 channels: offset z = fp16(min), scale s = fp16((max - z) * fl(1/15)),
-// code n = rint((x - z)/s) clipped to 0..15; a value reads back as z + n s (one
+// not below 0, code n = rint((x - z)/s) clipped to 0..15; a value reads back as z + n s (one
 // rounding to fp32: n s is exact there), then as bf16 where asked.
 #include "asa_cache.h"
 
@@ -10,75 +10,152 @@ namespace asa {
 namespace cache {
 namespace {
 
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+
+// Eight neighbouring channels as they lie in memory, and as fp32.
 template <typename X>
-__device__ __forceinline__ void load4(const X* p, float (&x)[4]);
+struct Eight;
 template <>
-__device__ __forceinline__ void load4(const float* p, float (&x)[4]) {
+struct Eight<float> {
+    float x[8];
+    __device__ __forceinline__ void load(const float* p, bool vec) {
+        if (vec) {
+            const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
+            x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+        } else {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = __ldg(p + i);
-}
+            for (int i = 0; i < 8; ++i) x[i] = __ldg(p + i);
+        }
+    }
+    __device__ __forceinline__ float2 pair(int i) const { return make_float2(x[2 * i], x[2 * i + 1]); }
+    // smallest and largest, NaN if there is one
+    __device__ __forceinline__ void range(float& lo, float& hi) const {
+        lo = hi = x[0];
+        bool nan = x[0] != x[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) lo = fminf(lo, x[i]), hi = fmaxf(hi, x[i]), nan |= x[i] != x[i];
+        if (nan) lo = hi = NAN;
+    }
+};
 template <>
-__device__ __forceinline__ void load4(const __nv_bfloat16* p, float (&x)[4]) {
+struct Eight<__nv_bfloat16> {
+    uint32_t w[4];
+    __device__ __forceinline__ void load(const __nv_bfloat16* p, bool vec) {
+        if (vec) {
+            const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
+            w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
+        } else {
+            const uint16_t* e = reinterpret_cast<const uint16_t*>(p);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) x[i] = __bfloat162float(p[i]);
+            for (int i = 0; i < 4; ++i) w[i] = __ldg(e + 2 * i) | (uint32_t)__ldg(e + 2 * i + 1) << 16;
+        }
+    }
+    __device__ __forceinline__ float2 pair(int i) const {
+        return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    }
+    __device__ __forceinline__ void range(float& lo, float& hi) const {
+        const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(w);
+        const float2 a = __bfloat1622float2(__hmin2_nan(__hmin2_nan(v[0], v[1]), __hmin2_nan(v[2], v[3])));
+        const float2 b = __bfloat1622float2(__hmax2_nan(__hmax2_nan(v[0], v[1]), __hmax2_nan(v[2], v[3])));
+        lo = a.x != a.x ? a.x : a.y != a.y ? a.y : fminf(a.x, a.y);
+        hi = b.x != b.x ? b.x : b.y != b.y ? b.y : fmaxf(b.x, b.y);
+    }
+};
+
+// The fp16 a code is counted in, from a group's smallest and largest.
+struct Grid { float z, s; uint32_t bits; };           // bits: s, then z
+__device__ __forceinline__ Grid grid_of(float lo, float hi) {
+    Grid g;
+    const __half z = __float2half_rn(lo);
+    g.z = __half2float(z);
+    // (below zero where a group of equal numbers has its offset rounded up)
+    const __half s = __float2half_rn(fmaxf(__fmul_rn(hi - g.z, kFifteenth), 0.0f));
+    g.s = __half2float(s);
+    g.bits = __half_as_ushort(s) | (uint32_t)__half_as_ushort(z) << 16;
+    return g;
 }
 
-// One token's row of one key head by one warp: lane l has channels 4l..4l+3, a
-// group is eight lanes.  Writes the codes (two bytes a lane) and, from each
-// group's first lane, its scale and offset.
-template <int D, bool KEY>
-__device__ __forceinline__ void quantise_row(const float (&raw)[4], uint8_t* codes, __half* par) {
-    constexpr int NG = D / 32;
-    const int lane = threadIdx.x & 31;
-    float x[4], lo = INFINITY, hi = -INFINITY;
-    bool nan = false;
+// Codes of eight channels, the first in the lowest four bits.  The quotient is
+// approximated by a product with 1 / s (within 2^-21 of it for codes up to 15) and
+// rounded by adding 1.5 * 2^23; where it comes within 2^-18 of a half, or a code
+// could leave 0..15, `sure` is lowered and exact_codes decides.
+template <typename X>
+__device__ __forceinline__ uint32_t quick_codes(const Eight<X>& x, const Grid& g, bool& sure) {
+    const float inv = g.s > 0.0f ? __frcp_rn(g.s) : 0.0f, magic = 12582912.0f;
+    float worst = 0.0f, r[8];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        nan |= raw[i] != raw[i];
-        x[i] = fminf(fmaxf(raw[i], -kF16Max), kF16Max);
-        lo = fminf(lo, x[i]);
-        hi = fmaxf(hi, x[i]);
+        const float2 v = __fmul2_rn(__fadd2_rn(x.pair(i), make_float2(-g.z, -g.z)), make_float2(inv, inv));
+        const float2 f = __fadd2_rn(__fadd2_rn(v, make_float2(magic, magic)), make_float2(-magic, -magic));
+        const float2 d = __fadd2_rn(v, make_float2(-f.x, -f.y));
+        worst = fmaxf(worst, fmaxf(fabsf(d.x), fabsf(d.y)));
+        r[2 * i] = f.x;
+        r[2 * i + 1] = f.y;
     }
+    sure &= worst < 0.5f - 3.8147e-6f;
+    uint32_t out = 0;
 #pragma unroll
-    for (int m = 1; m < 8; m <<= 1) {
+    for (int i = 0; i < 8; i += 4) {
+        const float sum = fmaf(fmaf(fmaf(r[i + 3], 16.0f, r[i + 2]), 16.0f, r[i + 1]), 16.0f, r[i]);
+        out |= (__float_as_uint(sum + magic) & 0xffffu) << (4 * i);
+    }
+    return out;
+}
+template <typename X>
+__device__ __noinline__ uint32_t exact_codes(const Eight<X>& x, float z, float s) {
+    uint32_t out = 0;
+    for (int i = 0; i < 4; ++i) {
+        const float2 v = x.pair(i);
+        for (int e = 0; e < 2; ++e) {
+            const float c = fminf(fmaxf(e ? v.y : v.x, -kF16Max), kF16Max);
+            const float n = s > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(c - z, s)), 0.0f), 15.0f) : 0.0f;
+            out |= (uint32_t)n << (4 * (2 * i + e));
+        }
+    }
+    return out;
+}
+
+// A row's part in one lane: codes and grid of its eight channels; the group is
+// four lanes.  All lanes take part.
+template <typename X>
+__device__ __forceinline__ uint32_t quantise(const Eight<X>& x, uint32_t& grid, bool& nan) {
+    float lo, hi;
+    x.range(lo, hi);
+    nan = lo != lo;
+#pragma unroll
+    for (int m = 1; m < 4; m <<= 1) {
         lo = fminf(lo, __shfl_xor_sync(~0u, lo, m));
         hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, m));
     }
-    nan = (__ballot_sync(~0u, nan) >> (lane & 24)) & 0xff;
-    const __half z = __float2half_rn(lo);
-    const float zf = __half2float(z);
-    const __half s = __float2half_rn(__fmul_rn(hi - zf, kFifteenth));
-    const float sf = __half2float(s);
-    uint32_t n[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-        n[i] = sf > 0.0f ? (uint32_t)fminf(fmaxf(rintf(__fdiv_rn(x[i] - zf, sf)), 0.0f), 15.0f) : 0u;
-    const int g = lane >> 3, w = lane & 7;
-    if (g >= NG) return;
-    const uint16_t two = (uint16_t)(n[0] | n[1] << 4 | n[2] << 8 | n[3] << 12);
-    const int at = KEY ? (w >> 1) * 4 * NG + 4 * g + 2 * (w & 1) : w * 2 * NG + 2 * g;
-    *reinterpret_cast<uint16_t*>(codes + at) = two;
-    if (w == 0) {
-        const __half bad = __ushort_as_half(0x7fff);
-        par[g] = nan ? bad : s;
-        par[NG + g] = nan ? bad : z;
-    }
+    const uint32_t group_nan = (__ballot_sync(~0u, nan) >> (threadIdx.x & 28)) & 15u;
+    bool sure = lo >= -kF16Max && hi <= kF16Max;
+    lo = fminf(fmaxf(lo, -kF16Max), kF16Max);
+    hi = fminf(fmaxf(hi, -kF16Max), kF16Max);
+    const Grid g = grid_of(lo, hi);
+    // with the offset rounded up far enough, or the scale rounded down, codes would leave 0..15
+    sure &= lo - g.z >= -0.25f * g.s && hi - g.z <= 15.25f * g.s;
+    uint32_t codes = quick_codes<X>(x, g, sure);
+    if (__any_sync(~0u, !sure)) codes = exact_codes<X>(x, g.z, g.s);
+    grid = group_nan ? 0x7fff7fffu : g.bits;
+    return codes;
 }
 
-__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
-
-// One CTA a (sequence, touched page, key head): its tokens, then the page's bounds.
-template <typename X, int D>
-__global__ void __launch_bounds__(256) write_kernel(Shape s, const X* __restrict__ K, const X* __restrict__ V,
-                                                    Strides ks, Strides vs, uint8_t* __restrict__ pool,
-                                                    int8_t* __restrict__ bounds, const int32_t* __restrict__ table,
-                                                    const int32_t* __restrict__ start,
-                                                    const int32_t* __restrict__ count, int touched, int* err) {
-    constexpr int NG = D / 32, W = 8;
-    __shared__ float s_hi[W][D], s_lo[W][D];
+// One CTA a (sequence, touched page, key head): its tokens' keys and values, then
+// the page's bounds.  A row is D/8 lanes of eight channels, so that a warp
+// reads 512 bytes of bf16 at a time.
+template <typename X, int D, int W>
+__global__ void __launch_bounds__(W * 32) write_kernel(Shape s, const X* __restrict__ K, const X* __restrict__ V,
+                                                       Strides ks, Strides vs, int vec, uint8_t* __restrict__ pool,
+                                                       int8_t* __restrict__ bounds, const int32_t* __restrict__ table,
+                                                       const int32_t* __restrict__ start,
+                                                       const int32_t* __restrict__ count, int touched, int* err) {
+    constexpr int NG = D / 32, LR = D / 8, RW = 32 / LR, RB = row_bytes(D), NTHR = W * 32;
+    __shared__ float s_hi[W * RW][D], s_lo[W * RW][D];
     __shared__ float s_m[W];
     const int h = blockIdx.x % s.H, j = blockIdx.x / s.H % touched, b = blockIdx.x / s.H / touched;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int sub = lane / LR, at = lane % LR, g = at >> 2, q = at & 3;   // row of the warp, channels 32 g + 8 q ..
+    const bool lane_in = sub < RW;                    // (96 channels leave eight lanes over)
     const long long begin = __ldg(start + b);
     const long long n = count ? min(max(__ldg(count + b), 0), s.T) : s.T;
     if (n == 0) return;
@@ -93,54 +170,84 @@ __global__ void __launch_bounds__(256) write_kernel(Shape s, const X* __restrict
         return;
     }
     uint8_t* rec = pool + ((int64_t)id * s.H + h) * s.rec;
-    float hi[4], lo[4];
+    const int64_t t0 = first - begin;
+    const int rows = (int)(last - first), slot0 = (int)(first - page_no * s.P);
+    const X* kp = K + b * ks.b + t0 * ks.t + h * ks.h + 8 * at;
+    const X* vp = V + b * vs.b + t0 * vs.t + h * vs.h + 8 * at;
+    float hi[8], lo[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) hi[i] = -INFINITY, lo[i] = INFINITY;
-    for (long long pos = first + warp; pos < last; pos += W) {
-        const int slot = (int)(pos - page_no * s.P);
-        const int64_t t = pos - begin;
-        float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (4 * lane < D) {
-            load4<X>(K + b * ks.b + t * ks.t + h * ks.h + 4 * lane, x);
-            load4<X>(V + b * vs.b + t * vs.t + h * vs.h + 4 * lane, y);
+    for (int i = 0; i < 8; ++i) hi[i] = -INFINITY, lo[i] = INFINITY;
+    constexpr int U = 2;                              // rows in flight a lane
+    for (int i0 = warp * RW; i0 < rows; i0 += U * W * RW) {
+        Eight<X> k[U], v[U];
+        bool in[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * W * RW + sub;
+            in[u] = lane_in && i < rows;
+            k[u] = v[u] = Eight<X>{};
+            if (in[u]) {
+                k[u].load(kp + i * ks.t, vec);
+                v[u].load(vp + i * vs.t, vec);
+            }
         }
-        uint8_t* kb = rec + (int64_t)(slot / kBlock) * block_bytes(D);
-        uint8_t* vb = kb + s.rec / 2;
-        const int r = slot % kBlock;
-        quantise_row<D, true>(x, kb + r * row_bytes(D),
-                              reinterpret_cast<__half*>(kb + kBlock * row_bytes(D)) + r * 2 * NG);
-        quantise_row<D, false>(y, vb + r * row_bytes(D),
-                               reinterpret_cast<__half*>(vb + kBlock * row_bytes(D)) + r * 2 * NG);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float c = x[i] != x[i] ? 0.0f : fminf(fmaxf(x[i], -kF16Max), kF16Max);
-            hi[i] = fmaxf(hi[i], c);
-            lo[i] = fminf(lo[i], c);
+        for (int u = 0; u < U; ++u) {
+            if (i0 + u * W * RW >= rows) break;
+            const int slot = slot0 + i0 + u * W * RW + sub, r = slot % kBlock;
+            uint8_t* kb = rec + (int64_t)(slot / kBlock) * block_bytes(D);
+            uint8_t* vb = kb + s.rec / 2;
+            uint32_t kg, vg;
+            bool k_nan, v_nan;
+            const uint32_t kc = quantise<X>(k[u], kg, k_nan), vc = quantise<X>(v[u], vg, v_nan);
+            if (!in[u]) continue;
+            *reinterpret_cast<uint32_t*>(kb + r * RB + q * 4 * NG + 4 * g) = kc;
+            uint8_t* vr = vb + r * RB + 2 * q * 2 * NG + 2 * g;
+            *reinterpret_cast<uint16_t*>(vr) = (uint16_t)vc;
+            *reinterpret_cast<uint16_t*>(vr + 2 * NG) = (uint16_t)(vc >> 16);
+            // the group's lanes store the key's scale and offset, the value's scale and offset
+            uint8_t* par = (q < 2 ? kb : vb) + kBlock * RB + r * par_bytes(D) + 2 * g + (q & 1 ? 2 * NG : 0);
+            const uint32_t pv = q < 2 ? kg : vg;
+            *reinterpret_cast<uint16_t*>(par) = (uint16_t)(q & 1 ? pv >> 16 : pv);
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                float2 y = k[u].pair(c);
+                if (k_nan) y.x = y.x != y.x ? 0.0f : y.x, y.y = y.y != y.y ? 0.0f : y.y;
+                hi[2 * c] = fmaxf(hi[2 * c], y.x);
+                lo[2 * c] = fminf(lo[2 * c], y.x);
+                hi[2 * c + 1] = fmaxf(hi[2 * c + 1], y.y);
+                lo[2 * c + 1] = fminf(lo[2 * c + 1], y.y);
+            }
         }
     }
-    if (4 * lane < D)
+    if (lane_in)
 #pragma unroll
-        for (int i = 0; i < 4; ++i) s_hi[warp][4 * lane + i] = hi[i], s_lo[warp][4 * lane + i] = lo[i];
+        for (int i = 0; i < 8; ++i) s_hi[warp * RW + sub][8 * at + i] = hi[i], s_lo[warp * RW + sub][8 * at + i] = lo[i];
     __syncthreads();
     int8_t* rb = bounds + ((int64_t)id * s.H + h) * bounds_bytes(D);
-    const int c = threadIdx.x;
-    float top = 0.0f, low = 0.0f;
-    if (c < D) {
-        top = s_hi[0][c];
-        low = s_lo[0][c];
+    constexpr int C = (D + NTHR - 1) / NTHR;          // channels a thread
+    float top[C], low[C], m = 0.0f;
+    const bool grown = slot0 > 0;                     // begun by an earlier call: its bounds stand
+    const float unit = grown ? pow2(min(max(*reinterpret_cast<const int*>(rb + 2 * D), -126), 127)) : 0.0f;
 #pragma unroll
-        for (int w = 1; w < W; ++w) top = fmaxf(top, s_hi[w][c]), low = fminf(low, s_lo[w][c]);
-        if (first > page_no * s.P) {         // begun by an earlier call: its bounds stand
-            const float unit = pow2(min(max(*reinterpret_cast<const int*>(rb + 2 * D), -126), 127));
-            top = fmaxf(top, (float)rb[c] * unit);
-            low = fminf(low, (float)rb[D + c] * unit);
-        }
+    for (int i = 0; i < C; ++i) {
+        const int c = threadIdx.x + i * NTHR;
+        top[i] = low[i] = 0.0f;
+        if (c >= D) continue;
+        float a = s_hi[0][c], z = s_lo[0][c];
+        for (int w = 1; w < W * RW; ++w) a = fmaxf(a, s_hi[w][c]), z = fminf(z, s_lo[w][c]);
+        a = fminf(a, kF16Max);
+        z = fmaxf(z, -kF16Max);
+        a = fmaxf(a, -kF16Max);
+        z = fminf(z, kF16Max);
+        if (grown) a = fmaxf(a, (float)rb[c] * unit), z = fminf(z, (float)rb[D + c] * unit);
+        top[i] = a;
+        low[i] = z;
+        m = fmaxf(m, fmaxf(fabsf(a), fabsf(z)));
     }
-    float m = fmaxf(fabsf(top), fabsf(low));
-#pragma unroll
-    for (int k = 16; k; k >>= 1) m = fmaxf(m, __shfl_xor_sync(~0u, m, k));
+    m = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(m)));
     if (lane == 0) s_m[warp] = m;
-    __syncthreads();                         // also: every old bound has been read
+    __syncthreads();                                  // also: every old bound has been read
     m = s_m[0];
 #pragma unroll
     for (int w = 1; w < W; ++w) m = fmaxf(m, s_m[w]);
@@ -150,11 +257,15 @@ __global__ void __launch_bounds__(256) write_kernel(Shape s, const X* __restrict
         e = max(e - 7 + (f > 127.0f / 128.0f ? 1 : 0), -126);
     }
     const float inv = pow2(-e);
-    if (c < D) {
-        rb[c] = (int8_t)ceilf(top * inv);
-        rb[D + c] = (int8_t)floorf(low * inv);
+#pragma unroll
+    for (int i = 0; i < C; ++i) {
+        const int c = threadIdx.x + i * NTHR;
+        if (c < D) {
+            rb[c] = (int8_t)ceilf(top[i] * inv);
+            rb[D + c] = (int8_t)floorf(low[i] * inv);
+        }
     }
-    if (c == 0) *reinterpret_cast<int*>(rb + 2 * D) = e;
+    if (threadIdx.x == 0) *reinterpret_cast<int*>(rb + 2 * D) = e;
 }
 
 template <typename X>
@@ -248,8 +359,18 @@ cudaError_t write_as(const Shape& s, const void* K, const void* V, Strides ks, S
     const int touched = (s.T + s.P - 2) / s.P + 1;
     const long long grid = (long long)s.B * touched * s.H;
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    write_kernel<X, D><<<(unsigned)grid, 256, 0, st>>>(s, (const X*)K, (const X*)V, ks, vs, pool, bounds,
-                                                       table, start, count, touched, err);
+    constexpr int64_t kVec = 16 / (int64_t)sizeof(X);     // elements of a 16-byte load
+    const auto fits = [](const void* p, Strides x) {
+        return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && x.b % kVec == 0 && x.t % kVec == 0 && x.h % kVec == 0;
+    };
+    const int vec = fits(K, ks) && fits(V, vs);
+    // A step writes a token or a few of each sequence: two warps a page then start sooner than eight.
+    if (s.T <= 4)
+        write_kernel<X, D, 2><<<(unsigned)grid, 64, 0, st>>>(s, (const X*)K, (const X*)V, ks, vs, vec, pool, bounds,
+                                                             table, start, count, touched, err);
+    else
+        write_kernel<X, D, 8><<<(unsigned)grid, 256, 0, st>>>(s, (const X*)K, (const X*)V, ks, vs, vec, pool,
+                                                              bounds, table, start, count, touched, err);
     note_launch();
     return cudaGetLastError();
 }

@@ -210,8 +210,8 @@ int asa_stable_backward(const asa_params* p, const void* Q, const void* K, const
  *            of 16 tokens.  A block holds 16 rows of d/2 bytes of codes, then 16
  *            rows of 2*d/32 fp16: the scales of the row's d/32 groups of 32
  *            channels, then their offsets.  A value is offset + code * scale
- *            (code 0..15), offset = fp16(min), scale = fp16((max - offset) * r)
- *            with r the fp32 number nearest 1/15, code = rint((x - offset)/scale)
+ *            (code 0..15), offset = fp16(min), scale = fp16((max - offset) * r),
+ *            not below 0, r the fp32 number nearest 1/15, code = rint((x - offset)/scale)
  *            clipped to 0..15, all in fp32, after x is clipped to +-65504.  A group holding a NaN reads back as NaN.
  *            A row of codes lists, run by run over the groups, the bytes of a
  *            run of 8 (keys) or 4 (values) channels: channel c = 32 g + w of a
