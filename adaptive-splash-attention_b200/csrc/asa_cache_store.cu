@@ -6,20 +6,24 @@
 // rounding to fp32: n s is exact there), then as bf16 where asked.
 #include "asa_cache.h"
 
+#include <type_traits>
+
 namespace asa {
 namespace cache {
 namespace {
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 
-// Eight neighbouring channels as they lie in memory, and as fp32.
+// Eight neighbouring channels: words as they lie in memory, values as fp32, and the
+// lane-wise larger and smaller of two (NaN aside).
 template <typename X>
 struct Eight;
 template <>
 struct Eight<float> {
     float x[8];
-    __device__ __forceinline__ void load(const float* p, bool vec) {
-        if (vec) {
+    template <bool VEC>
+    __device__ __forceinline__ void load(const float* p) {
+        if constexpr (VEC) {
             const float4 a = __ldg(reinterpret_cast<const float4*>(p)), b = __ldg(reinterpret_cast<const float4*>(p) + 1);
             x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
         } else {
@@ -27,21 +31,36 @@ struct Eight<float> {
             for (int i = 0; i < 8; ++i) x[i] = __ldg(p + i);
         }
     }
-    __device__ __forceinline__ float2 pair(int i) const { return make_float2(x[2 * i], x[2 * i + 1]); }
-    // smallest and largest, NaN if there is one
-    __device__ __forceinline__ void range(float& lo, float& hi) const {
-        lo = hi = x[0];
-        bool nan = x[0] != x[0];
+    __device__ __forceinline__ void fill(float v) {
 #pragma unroll
-        for (int i = 1; i < 8; ++i) lo = fminf(lo, x[i]), hi = fmaxf(hi, x[i]), nan |= x[i] != x[i];
-        if (nan) lo = hi = NAN;
+        for (int i = 0; i < 8; ++i) x[i] = v;
+    }
+    __device__ __forceinline__ float at(int i) const { return x[i]; }
+    __device__ __forceinline__ bool nan() const {
+        bool n = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) n |= x[i] != x[i];
+        return n;
+    }
+    __device__ __forceinline__ void raise(const Eight& o) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = fmaxf(x[i], o.x[i]);
+    }
+    __device__ __forceinline__ void lower(const Eight& o) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = fminf(x[i], o.x[i]);
+    }
+    __device__ __forceinline__ void nan_to_zero() {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = x[i] != x[i] ? 0.0f : x[i];
     }
 };
 template <>
 struct Eight<__nv_bfloat16> {
     uint32_t w[4];
-    __device__ __forceinline__ void load(const __nv_bfloat16* p, bool vec) {
-        if (vec) {
+    template <bool VEC>
+    __device__ __forceinline__ void load(const __nv_bfloat16* p) {
+        if constexpr (VEC) {
             const uint4 v = __ldg(reinterpret_cast<const uint4*>(p));
             w[0] = v.x, w[1] = v.y, w[2] = v.z, w[3] = v.w;
         } else {
@@ -50,180 +69,193 @@ struct Eight<__nv_bfloat16> {
             for (int i = 0; i < 4; ++i) w[i] = __ldg(e + 2 * i) | (uint32_t)__ldg(e + 2 * i + 1) << 16;
         }
     }
-    __device__ __forceinline__ float2 pair(int i) const {
-        return make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+    __device__ __forceinline__ void fill(float x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = __byte_perm(__float_as_uint(x), 0u, 0x3232);
     }
-    __device__ __forceinline__ void range(float& lo, float& hi) const {
-        const __nv_bfloat162* v = reinterpret_cast<const __nv_bfloat162*>(w);
-        const float2 a = __bfloat1622float2(__hmin2_nan(__hmin2_nan(v[0], v[1]), __hmin2_nan(v[2], v[3])));
-        const float2 b = __bfloat1622float2(__hmax2_nan(__hmax2_nan(v[0], v[1]), __hmax2_nan(v[2], v[3])));
-        lo = a.x != a.x ? a.x : a.y != a.y ? a.y : fminf(a.x, a.y);
-        hi = b.x != b.x ? b.x : b.y != b.y ? b.y : fmaxf(b.x, b.y);
+    __device__ __forceinline__ float at(int i) const {
+        return __uint_as_float(i & 1 ? w[i / 2] & 0xffff0000u : w[i / 2] << 16);
+    }
+    __device__ __forceinline__ bool nan() const {     // a magnitude above infinity's carries into the sign
+        uint32_t n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) n |= (w[i] & 0x7fff7fffu) + 0x007f007fu;
+        return (n & 0x80008000u) != 0u;
+    }
+    __device__ __forceinline__ void raise(const Eight& o) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 c = __hmax2(reinterpret_cast<const __nv_bfloat162&>(w[i]), reinterpret_cast<const __nv_bfloat162&>(o.w[i]));
+            w[i] = reinterpret_cast<const uint32_t&>(c);
+        }
+    }
+    __device__ __forceinline__ void lower(const Eight& o) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const __nv_bfloat162 c = __hmin2(reinterpret_cast<const __nv_bfloat162&>(w[i]), reinterpret_cast<const __nv_bfloat162&>(o.w[i]));
+            w[i] = reinterpret_cast<const uint32_t&>(c);
+        }
+    }
+    __device__ __forceinline__ void nan_to_zero() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if ((w[i] & 0x7fffu) > 0x7f80u) w[i] &= 0xffff0000u;
+            if ((w[i] & 0x7fff0000u) > 0x7f800000u) w[i] &= 0xffffu;
+        }
     }
 };
 
-// The fp16 a code is counted in, from a group's smallest and largest.
-struct Grid { float z, s; uint32_t bits; };           // bits: s, then z
-__device__ __forceinline__ Grid grid_of(float lo, float hi) {
-    Grid g;
-    const __half z = __float2half_rn(lo);
-    g.z = __half2float(z);
-    // (below zero where a group of equal numbers has its offset rounded up)
-    const __half s = __float2half_rn(fmaxf(__fmul_rn(hi - g.z, kFifteenth), 0.0f));
-    g.s = __half2float(s);
-    g.bits = __half_as_ushort(s) | (uint32_t)__half_as_ushort(z) << 16;
-    return g;
-}
-
-// Codes of eight channels, the first in the lowest four bits.  The quotient is
-// approximated by a product with 1 / s (within 2^-21 of it for codes up to 15) and
-// rounded by adding 1.5 * 2^23; where it comes within 2^-18 of a half, or a code
-// could leave 0..15, `sure` is lowered and exact_codes decides.
+// A group of 32 channels, all in one lane: codes (the first channel in the lowest
+// four bits of the first word) and scale (low half) and offset.
+//
+// (x - z) / s is formed as Markstein does it (IBM J. Res. Dev. 34, 1990): with the
+// correctly rounded reciprocal, a product, its exact remainder and one correction
+// give the correctly rounded quotient.  So halves, which are not rare between
+// numbers of few bits, go to the even code as the format's division has them.
+// Adding 1.5 * 2^23 rounds to whole numbers.
 template <typename X>
-__device__ __forceinline__ uint32_t quick_codes(const Eight<X>& x, const Grid& g, bool& sure) {
-    const float inv = g.s > 0.0f ? __frcp_rn(g.s) : 0.0f, magic = 12582912.0f;
-    float worst = 0.0f, r[8];
+__device__ __forceinline__ void quantise(const Eight<X> (&x)[4], uint32_t (&codes)[4], uint32_t& grid) {
+    constexpr float kMagic = 12582912.0f;
+    Eight<X> least = x[0], most = x[0];
+    bool nan = x[0].nan();
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 v = __fmul2_rn(__fadd2_rn(x.pair(i), make_float2(-g.z, -g.z)), make_float2(inv, inv));
-        const float2 f = __fadd2_rn(__fadd2_rn(v, make_float2(magic, magic)), make_float2(-magic, -magic));
-        const float2 d = __fadd2_rn(v, make_float2(-f.x, -f.y));
-        worst = fmaxf(worst, fmaxf(fabsf(d.x), fabsf(d.y)));
-        r[2 * i] = f.x;
-        r[2 * i + 1] = f.y;
+    for (int i = 1; i < 4; ++i) {
+        least.lower(x[i]);
+        most.raise(x[i]);
+        nan |= x[i].nan();
     }
-    sure &= worst < 0.5f - 3.8147e-6f;
-    uint32_t out = 0;
+    float lo = least.at(0), hi = most.at(0);
 #pragma unroll
-    for (int i = 0; i < 8; i += 4) {
-        const float sum = fmaf(fmaf(fmaf(r[i + 3], 16.0f, r[i + 2]), 16.0f, r[i + 1]), 16.0f, r[i]);
-        out |= (__float_as_uint(sum + magic) & 0xffffu) << (4 * i);
-    }
-    return out;
-}
-template <typename X>
-__device__ __noinline__ uint32_t exact_codes(const Eight<X>& x, float z, float s) {
-    uint32_t out = 0;
-    for (int i = 0; i < 4; ++i) {
-        const float2 v = x.pair(i);
-        for (int e = 0; e < 2; ++e) {
-            const float c = fminf(fmaxf(e ? v.y : v.x, -kF16Max), kF16Max);
-            const float n = s > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(c - z, s)), 0.0f), 15.0f) : 0.0f;
-            out |= (uint32_t)n << (4 * (2 * i + e));
-        }
-    }
-    return out;
-}
-
-// A row's part in one lane: codes and grid of its eight channels; the group is
-// four lanes.  All lanes take part.
-template <typename X>
-__device__ __forceinline__ uint32_t quantise(const Eight<X>& x, uint32_t& grid, bool& nan) {
-    float lo, hi;
-    x.range(lo, hi);
-    nan = lo != lo;
-#pragma unroll
-    for (int m = 1; m < 4; m <<= 1) {
-        lo = fminf(lo, __shfl_xor_sync(~0u, lo, m));
-        hi = fmaxf(hi, __shfl_xor_sync(~0u, hi, m));
-    }
-    const uint32_t group_nan = (__ballot_sync(~0u, nan) >> (threadIdx.x & 28)) & 15u;
-    bool sure = lo >= -kF16Max && hi <= kF16Max;
+    for (int i = 1; i < 8; ++i) lo = fminf(lo, least.at(i)), hi = fmaxf(hi, most.at(i));
+    bool plain = lo >= -kF16Max && hi <= kF16Max;
     lo = fminf(fmaxf(lo, -kF16Max), kF16Max);
     hi = fminf(fmaxf(hi, -kF16Max), kF16Max);
-    const Grid g = grid_of(lo, hi);
+    const __half zh = __float2half_rn(lo);
+    const float z = __half2float(zh);
+    // (below zero where a group of equal numbers has its offset rounded up)
+    const __half sh = __float2half_rn(fmaxf(__fmul_rn(hi - z, kFifteenth), 0.0f));
+    const float s = __half2float(sh), inv = s > 0.0f ? __frcp_rn(s) : 0.0f;
+    grid = nan ? 0x7fff7fffu : __half_as_ushort(sh) | (uint32_t)__half_as_ushort(zh) << 16;
     // with the offset rounded up far enough, or the scale rounded down, codes would leave 0..15
-    sure &= lo - g.z >= -0.25f * g.s && hi - g.z <= 15.25f * g.s;
-    uint32_t codes = quick_codes<X>(x, g, sure);
-    if (__any_sync(~0u, !sure)) codes = exact_codes<X>(x, g.z, g.s);
-    grid = group_nan ? 0x7fff7fffu : g.bits;
-    return codes;
+    plain &= lo - z >= -0.25f * s && hi - z <= 15.25f * s;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        float r[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const float y = x[i].at(j) - z, q = y * inv;
+            r[j] = (fmaf(fmaf(-q, s, y), inv, q) + kMagic) - kMagic;
+        }
+        if (!plain)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float c = fminf(fmaxf(x[i].at(j), -kF16Max), kF16Max);
+                r[j] = s > 0.0f ? fminf(fmaxf(rintf(__fdiv_rn(c - z, s)), 0.0f), 15.0f) : 0.0f;
+            }
+        uint32_t out = 0;
+#pragma unroll
+        for (int j = 0; j < 8; j += 4) {
+            const float sum = fmaf(fmaf(fmaf(r[j + 3], 16.0f, r[j + 2]), 16.0f, r[j + 1]), 16.0f, r[j]);
+            out |= (__float_as_uint(sum + kMagic) & 0xffffu) << (4 * j);
+        }
+        codes[i] = out;
+    }
 }
 
-// One CTA a (sequence, touched page, key head): its tokens' keys and values, then
-// the page's bounds.  A row is D/8 lanes of eight channels, so that a warp
-// reads 512 bytes of bf16 at a time.
-template <typename X, int D, int W>
-__global__ void __launch_bounds__(W * 32) write_kernel(Shape s, const X* __restrict__ K, const X* __restrict__ V,
-                                                       Strides ks, Strides vs, int vec, uint8_t* __restrict__ pool,
-                                                       int8_t* __restrict__ bounds, const int32_t* __restrict__ table,
-                                                       const int32_t* __restrict__ start,
-                                                       const int32_t* __restrict__ count, int touched, int* err) {
-    constexpr int NG = D / 32, LR = D / 8, RW = 32 / LR, RB = row_bytes(D), NTHR = W * 32;
-    __shared__ float s_hi[W * RW][D], s_lo[W * RW][D];
+// One CTA a (sequence, touched page, key head): its tokens' keys and values, a
+// group of 32 channels a lane at a time, laid out in shared memory as in the
+// record and copied from there 16 bytes a lane; then the page's bounds, from the
+// keys (in L1 by then).
+template <typename X, int D, int NTHR>
+__global__ void __launch_bounds__(NTHR) write_kernel(Shape s, const X* __restrict__ K, const X* __restrict__ V,
+                                                     Strides ks, Strides vs, int vec, uint8_t* __restrict__ pool,
+                                                     int8_t* __restrict__ bounds, const int32_t* __restrict__ table,
+                                                     const int32_t* __restrict__ start,
+                                                     const int32_t* __restrict__ count, int touched, int page_shift,
+                                                     int* err) {
+    constexpr int NG = D / 32, LR = D / 8, RB = row_bytes(D), PB = par_bytes(D), W = NTHR / 32;
+    constexpr int SETS = NTHR / LR;                   // token sets that bounds are first taken over
+    extern __shared__ __align__(16) uint8_t s_rec[];  // rows of codes and of scales: [2][page][RB], [2][page][PB]
+    __shared__ float s_hi[SETS][D], s_lo[SETS][D];
     __shared__ float s_m[W];
-    const int h = blockIdx.x % s.H, j = blockIdx.x / s.H % touched, b = blockIdx.x / s.H / touched;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int sub = lane / LR, at = lane % LR, g = at >> 2, q = at & 3;   // row of the warp, channels 32 g + 8 q ..
-    const bool lane_in = sub < RW;                    // (96 channels leave eight lanes over)
-    const long long begin = __ldg(start + b);
-    const long long n = count ? min(max(__ldg(count + b), 0), s.T) : s.T;
-    if (n == 0) return;
-    // the pages that positions begin .. begin + n - 1 lie in, the j-th of them
-    const long long page_no = (begin >= 0 ? begin / s.P : -((-begin + s.P - 1) / s.P)) + j;
-    const long long first = max(begin, page_no * s.P), last = min(begin + n, (page_no + 1) * s.P);
-    if (first >= last) return;
+    const unsigned bj = blockIdx.x / (unsigned)s.H;
+    const int h = blockIdx.x - bj * s.H, b = bj / (unsigned)touched, j = bj - b * touched;
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int begin = __ldg(start + b), n = count ? min(max(__ldg(count + b), 0), s.T) : s.T;
+    // the j-th of the pages that positions begin .. begin + n - 1 lie in, and the tokens there:
+    // `from` of the call's, `rows` of them, the first in slot `slot0`
+    const int page_no = (begin >> page_shift) + j, into = (begin & (s.P - 1)) - j * s.P;   // (begin - the page's first)
+    const int from = max(0, -into), slot0 = max(0, into), rows = min(n - from, s.P - slot0);
+    if (rows <= 0) return;
     int id = -1;
     if (page_no >= 0 && page_no < s.width) id = __ldg(table + (int64_t)b * s.width + page_no);
     if (id < 0 || id >= s.pages) {
-        if (threadIdx.x == 0 && err) atomicCAS(err, 0, ASA_ERR_INVALID);
+        if (tid == 0 && err) atomicCAS(err, 0, ASA_ERR_INVALID);
         return;
     }
     uint8_t* rec = pool + ((int64_t)id * s.H + h) * s.rec;
-    const int64_t t0 = first - begin;
-    const int rows = (int)(last - first), slot0 = (int)(first - page_no * s.P);
-    const X* kp = K + b * ks.b + t0 * ks.t + h * ks.h + 8 * at;
-    const X* vp = V + b * vs.b + t0 * vs.t + h * vs.h + 8 * at;
-    float hi[8], lo[8];
+    const X* kp = K + b * ks.b + (int64_t)from * ks.t + h * ks.h;
+    const X* vp = V + b * vs.b + (int64_t)from * vs.t + h * vs.h;
+    uint8_t* const s_par = s_rec + 2 * s.P * RB;
+    auto body = [&](auto vec_c) {
+        constexpr bool VEC = decltype(vec_c)::value;
+        for (int i = tid; i < 2 * rows * NG; i += NTHR) {
+            const int g = i % NG, row = i / NG, part = row >= rows, r = part ? row - rows : row;
+            const X* src = (part ? vp + r * vs.t : kp + r * ks.t) + 32 * g;
+            Eight<X> x[4];
+            uint32_t codes[4], grid;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) hi[i] = -INFINITY, lo[i] = INFINITY;
-    constexpr int U = 2;                              // rows in flight a lane
-    for (int i0 = warp * RW; i0 < rows; i0 += U * W * RW) {
-        Eight<X> k[U], v[U];
-        bool in[U];
+            for (int k = 0; k < 4; ++k) x[k].template load<VEC>(src + 8 * k);
+            quantise<X>(x, codes, grid);
+            uint8_t* to = s_rec + (part * s.P + r) * RB;
 #pragma unroll
-        for (int u = 0; u < U; ++u) {
-            const int i = i0 + u * W * RW + sub;
-            in[u] = lane_in && i < rows;
-            k[u] = v[u] = Eight<X>{};
-            if (in[u]) {
-                k[u].load(kp + i * ks.t, vec);
-                v[u].load(vp + i * vs.t, vec);
+            for (int k = 0; k < 4; ++k) {
+                if (part) {
+                    *reinterpret_cast<uint16_t*>(to + 2 * k * 2 * NG + 2 * g) = (uint16_t)codes[k];
+                    *reinterpret_cast<uint16_t*>(to + (2 * k + 1) * 2 * NG + 2 * g) = (uint16_t)(codes[k] >> 16);
+                } else {
+                    *reinterpret_cast<uint32_t*>(to + k * 4 * NG + 4 * g) = codes[k];
+                }
+            }
+            uint16_t* par = reinterpret_cast<uint16_t*>(s_par + (part * s.P + r) * PB) + g;
+            par[0] = (uint16_t)grid;
+            par[NG] = (uint16_t)(grid >> 16);
+        }
+        // bounds of this thread's eight channels over its set of tokens
+        const int set = tid / LR, c8 = tid % LR;
+        if (set < SETS) {
+            Eight<X> hi, lo;
+            hi.fill(-INFINITY);
+            lo.fill(INFINITY);
+#pragma unroll 4
+            for (int r = set; r < rows; r += SETS) {
+                Eight<X> x;
+                x.template load<VEC>(kp + r * ks.t + 8 * c8);
+                if (x.nan()) x.nan_to_zero();
+                hi.raise(x);
+                lo.lower(x);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; i += 4) {
+                *reinterpret_cast<float4*>(&s_hi[set][8 * c8 + i]) = make_float4(hi.at(i), hi.at(i + 1), hi.at(i + 2), hi.at(i + 3));
+                *reinterpret_cast<float4*>(&s_lo[set][8 * c8 + i]) = make_float4(lo.at(i), lo.at(i + 1), lo.at(i + 2), lo.at(i + 3));
             }
         }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
-            if (i0 + u * W * RW >= rows) break;
-            const int slot = slot0 + i0 + u * W * RW + sub, r = slot % kBlock;
-            uint8_t* kb = rec + (int64_t)(slot / kBlock) * block_bytes(D);
-            uint8_t* vb = kb + s.rec / 2;
-            uint32_t kg, vg;
-            bool k_nan, v_nan;
-            const uint32_t kc = quantise<X>(k[u], kg, k_nan), vc = quantise<X>(v[u], vg, v_nan);
-            if (!in[u]) continue;
-            *reinterpret_cast<uint32_t*>(kb + r * RB + q * 4 * NG + 4 * g) = kc;
-            uint8_t* vr = vb + r * RB + 2 * q * 2 * NG + 2 * g;
-            *reinterpret_cast<uint16_t*>(vr) = (uint16_t)vc;
-            *reinterpret_cast<uint16_t*>(vr + 2 * NG) = (uint16_t)(vc >> 16);
-            // the group's lanes store the key's scale and offset, the value's scale and offset
-            uint8_t* par = (q < 2 ? kb : vb) + kBlock * RB + r * par_bytes(D) + 2 * g + (q & 1 ? 2 * NG : 0);
-            const uint32_t pv = q < 2 ? kg : vg;
-            *reinterpret_cast<uint16_t*>(par) = (uint16_t)(q & 1 ? pv >> 16 : pv);
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                float2 y = k[u].pair(c);
-                if (k_nan) y.x = y.x != y.x ? 0.0f : y.x, y.y = y.y != y.y ? 0.0f : y.y;
-                hi[2 * c] = fmaxf(hi[2 * c], y.x);
-                lo[2 * c] = fminf(lo[2 * c], y.x);
-                hi[2 * c + 1] = fmaxf(hi[2 * c + 1], y.y);
-                lo[2 * c + 1] = fminf(lo[2 * c + 1], y.y);
-            }
-        }
-    }
-    if (lane_in)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) s_hi[warp * RW + sub][8 * at + i] = hi[i], s_lo[warp * RW + sub][8 * at + i] = lo[i];
+    };
+    if (vec) body(std::true_type{}); else body(std::false_type{});
     __syncthreads();
+    // rows to the record
+    constexpr int CW = RB / 16;                       // 16-byte pieces of a row of codes
+    for (int i = tid; i < 2 * rows * CW; i += NTHR) {
+        const int piece = i % CW, row = i / CW, part = row >= rows, r = part ? row - rows : row, slot = slot0 + r;
+        *reinterpret_cast<uint4*>(rec + part * (s.rec / 2) + slot / kBlock * block_bytes(D) + slot % kBlock * RB + 16 * piece) =
+            *reinterpret_cast<const uint4*>(s_rec + (part * s.P + r) * RB + 16 * piece);
+    }
+    for (int i = tid; i < 2 * rows * NG; i += NTHR) {
+        const int piece = i % NG, row = i / NG, part = row >= rows, r = part ? row - rows : row, slot = slot0 + r;
+        *reinterpret_cast<uint32_t*>(rec + part * (s.rec / 2) + slot / kBlock * block_bytes(D) + kBlock * RB + slot % kBlock * PB + 4 * piece) =
+            *reinterpret_cast<const uint32_t*>(s_par + (part * s.P + r) * PB + 4 * piece);
+    }
     int8_t* rb = bounds + ((int64_t)id * s.H + h) * bounds_bytes(D);
     constexpr int C = (D + NTHR - 1) / NTHR;          // channels a thread
     float top[C], low[C], m = 0.0f;
@@ -231,15 +263,14 @@ __global__ void __launch_bounds__(W * 32) write_kernel(Shape s, const X* __restr
     const float unit = grown ? pow2(min(max(*reinterpret_cast<const int*>(rb + 2 * D), -126), 127)) : 0.0f;
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-        const int c = threadIdx.x + i * NTHR;
+        const int c = tid + i * NTHR;
         top[i] = low[i] = 0.0f;
         if (c >= D) continue;
         float a = s_hi[0][c], z = s_lo[0][c];
-        for (int w = 1; w < W * RW; ++w) a = fmaxf(a, s_hi[w][c]), z = fminf(z, s_lo[w][c]);
-        a = fminf(a, kF16Max);
-        z = fmaxf(z, -kF16Max);
-        a = fmaxf(a, -kF16Max);
-        z = fminf(z, kF16Max);
+#pragma unroll
+        for (int w = 1; w < SETS; ++w) a = fmaxf(a, s_hi[w][c]), z = fminf(z, s_lo[w][c]);
+        a = fmaxf(fminf(a, kF16Max), -kF16Max);
+        z = fmaxf(fminf(z, kF16Max), -kF16Max);
         if (grown) a = fmaxf(a, (float)rb[c] * unit), z = fminf(z, (float)rb[D + c] * unit);
         top[i] = a;
         low[i] = z;
@@ -259,13 +290,13 @@ __global__ void __launch_bounds__(W * 32) write_kernel(Shape s, const X* __restr
     const float inv = pow2(-e);
 #pragma unroll
     for (int i = 0; i < C; ++i) {
-        const int c = threadIdx.x + i * NTHR;
+        const int c = tid + i * NTHR;
         if (c < D) {
             rb[c] = (int8_t)ceilf(top[i] * inv);
             rb[D + c] = (int8_t)floorf(low[i] * inv);
         }
     }
-    if (threadIdx.x == 0) *reinterpret_cast<int*>(rb + 2 * D) = e;
+    if (tid == 0) *reinterpret_cast<int*>(rb + 2 * D) = e;
 }
 
 template <typename X>
@@ -283,52 +314,70 @@ __device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&x)[8]) {
     *reinterpret_cast<uint4*>(p) = *reinterpret_cast<uint4*>(v);
 }
 
-// A thread an eight-channel run of a token: its key and its value.
+// A thread takes eight-channel runs of tokens' keys and values, kReadRows at a
+// time: the places of all, then their codes, scales and offsets, then the outputs,
+// so that the loads of several are under way at once.
+constexpr int kReadRows = 4;
 template <typename X, int D>
 __global__ void __launch_bounds__(256) read_kernel(Shape s, const uint8_t* __restrict__ pool,
                                                    const int32_t* __restrict__ table,
                                                    const int32_t* __restrict__ start,
                                                    const int32_t* __restrict__ count, X* __restrict__ K,
-                                                   X* __restrict__ V, int* err) {
-    constexpr int NG = D / 32, R = D / 8;
-    const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-    const int64_t row = i / R;                       // (b, t, h)
-    if (row >= (int64_t)s.B * s.T * s.H) return;
-    const int run = (int)(i % R), h = (int)(row % s.H);
-    const int64_t bt = row / s.H;
-    const int t = (int)(bt % s.T), b = (int)(bt / s.T);
-    float k[8], v[8];
+                                                   X* __restrict__ V, unsigned chunks, int page_shift, int* err) {
+    constexpr int NG = D / 32, R = D / 8, RB = row_bytes(D), ROWS = 256 / R;   // rows of the CTA at a time
+    const unsigned b = blockIdx.x / chunks, chunk = blockIdx.x - b * chunks;
+    const unsigned run = threadIdx.x % R, first = chunk * (kReadRows * ROWS) + threadIdx.x / R;
+    if (threadIdx.x / R >= ROWS) return;              // (96 channels leave four threads over)
+    const unsigned of = (unsigned)s.T * s.H;          // rows (token, head) of the sequence
+    const int begin = __ldg(start + b), n = count ? __ldg(count + b) : s.T;
+    const int g = run >> 2, q = run & 3;              // channels 32 g + 8 q ..
+    const uint8_t* at[kReadRows];
 #pragma unroll
-    for (int c = 0; c < 8; ++c) k[c] = v[c] = 0.0f;
-    const int n = count ? __ldg(count + b) : s.T;
-    if (t < n) {
-        const long long pos = (long long)__ldg(start + b) + t;
+    for (int u = 0; u < kReadRows; ++u) {
+        const unsigned row = first + u * ROWS, t = row / (unsigned)s.H, h = row - t * s.H;
+        at[u] = nullptr;
+        if (row >= of || (int)t >= n) continue;
+        const long long pos = (long long)begin + t;
         int id = -1;
-        if (pos >= 0 && pos / s.P < s.width) id = __ldg(table + (int64_t)b * s.width + pos / s.P);
+        if (pos >= 0 && pos >> page_shift < s.width) id = __ldg(table + (int64_t)b * s.width + (pos >> page_shift));
         if (id >= 0 && id < s.pages) {
-            const int slot = (int)(pos % s.P), r = slot % kBlock;
-            const uint8_t* kb = pool + ((int64_t)id * s.H + h) * s.rec + (int64_t)(slot / kBlock) * block_bytes(D);
-            const uint8_t* vb = kb + s.rec / 2;
-            const int g = run >> 2, q = run & 3;     // channels 32 g + 8 q ..
-            const __half* kp = reinterpret_cast<const __half*>(kb + kBlock * row_bytes(D)) + r * 2 * NG;
-            const __half* vp = reinterpret_cast<const __half*>(vb + kBlock * row_bytes(D)) + r * 2 * NG;
-            const uint8_t* vr = vb + r * row_bytes(D);
-            const uint32_t kw = *reinterpret_cast<const uint32_t*>(kb + r * row_bytes(D) + q * 4 * NG + 4 * g);
-            const uint32_t vw = *reinterpret_cast<const uint16_t*>(vr + 2 * q * 2 * NG + 2 * g) |
-                                (uint32_t)*reinterpret_cast<const uint16_t*>(vr + (2 * q + 1) * 2 * NG + 2 * g) << 16;
-            const float ksc = __half2float(kp[g]), kz = __half2float(kp[NG + g]);
-            const float vsc = __half2float(vp[g]), vz = __half2float(vp[NG + g]);
-#pragma unroll
-            for (int c = 0; c < 8; ++c) {
-                k[c] = fmaf((float)((kw >> (4 * c)) & 15u), ksc, kz);
-                v[c] = fmaf((float)((vw >> (4 * c)) & 15u), vsc, vz);
-            }
+            const unsigned slot = (unsigned)pos & (s.P - 1);
+            at[u] = pool + ((int64_t)id * s.H + h) * s.rec + slot / kBlock * block_bytes(D) + slot % kBlock;
         } else if (err) {
             atomicCAS(err, 0, ASA_ERR_INVALID);
         }
     }
-    store8<X>(K + row * D + 8 * run, k);
-    store8<X>(V + row * D + 8 * run, v);
+    uint32_t kw[kReadRows], vw[kReadRows], kp[kReadRows], vp[kReadRows];
+#pragma unroll
+    for (int u = 0; u < kReadRows; ++u) {
+        kw[u] = vw[u] = kp[u] = vp[u] = 0u;
+        if (!at[u]) continue;
+        const uint32_t r = (uint32_t)(reinterpret_cast<uintptr_t>(at[u]) & (kBlock - 1));   // (records are 16-byte aligned)
+        const uint8_t *kb = at[u] - r, *vb = kb + s.rec / 2;
+        const uint16_t* kh = reinterpret_cast<const uint16_t*>(kb + kBlock * RB + r * par_bytes(D)) + g;
+        const uint16_t* vh = reinterpret_cast<const uint16_t*>(vb + kBlock * RB + r * par_bytes(D)) + g;
+        const uint8_t* vr = vb + r * RB + 2 * q * 2 * NG + 2 * g;
+        kw[u] = __ldg(reinterpret_cast<const uint32_t*>(kb + r * RB + q * 4 * NG + 4 * g));
+        vw[u] = __ldg(reinterpret_cast<const uint16_t*>(vr)) | (uint32_t)__ldg(reinterpret_cast<const uint16_t*>(vr + 2 * NG)) << 16;
+        kp[u] = __ldg(kh) | (uint32_t)__ldg(kh + NG) << 16;
+        vp[u] = __ldg(vh) | (uint32_t)__ldg(vh + NG) << 16;
+    }
+#pragma unroll
+    for (int u = 0; u < kReadRows; ++u) {
+        const unsigned row = first + u * ROWS;
+        if (row >= of) break;
+        const float2 ks = __half22float2(*reinterpret_cast<const __half2*>(&kp[u]));
+        const float2 vs = __half22float2(*reinterpret_cast<const __half2*>(&vp[u]));
+        float k[8], v[8];
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+            k[c] = fmaf((float)((kw[u] >> (4 * c)) & 15u), ks.x, ks.y);
+            v[c] = fmaf((float)((vw[u] >> (4 * c)) & 15u), vs.x, vs.y);
+        }
+        const int64_t to = ((int64_t)b * of + row) * D + 8 * run;
+        store8<X>(K + to, k);
+        store8<X>(V + to, v);
+    }
 }
 
 __global__ void __launch_bounds__(256) bounds_kernel(Shape s, const int8_t* __restrict__ bounds,
@@ -357,6 +406,8 @@ cudaError_t write_as(const Shape& s, const void* K, const void* V, Strides ks, S
                      int8_t* bounds, const int32_t* table, const int32_t* start, const int32_t* count,
                      int* err, cudaStream_t st) {
     const int touched = (s.T + s.P - 2) / s.P + 1;
+    int page_shift = 4;
+    while (1 << page_shift < s.P) ++page_shift;
     const long long grid = (long long)s.B * touched * s.H;
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
     constexpr int64_t kVec = 16 / (int64_t)sizeof(X);     // elements of a 16-byte load
@@ -364,13 +415,14 @@ cudaError_t write_as(const Shape& s, const void* K, const void* V, Strides ks, S
         return (reinterpret_cast<uintptr_t>(p) & 15) == 0 && x.b % kVec == 0 && x.t % kVec == 0 && x.h % kVec == 0;
     };
     const int vec = fits(K, ks) && fits(V, vs);
+    const size_t smem = (size_t)2 * s.P * (row_bytes(D) + par_bytes(D));   // 20 KB at most
     // A step writes a token or a few of each sequence: two warps a page then start sooner than eight.
     if (s.T <= 4)
-        write_kernel<X, D, 2><<<(unsigned)grid, 64, 0, st>>>(s, (const X*)K, (const X*)V, ks, vs, vec, pool, bounds,
-                                                             table, start, count, touched, err);
+        write_kernel<X, D, 64><<<(unsigned)grid, 64, smem, st>>>(s, (const X*)K, (const X*)V, ks, vs, vec, pool, bounds,
+                                                                 table, start, count, touched, page_shift, err);
     else
-        write_kernel<X, D, 8><<<(unsigned)grid, 256, 0, st>>>(s, (const X*)K, (const X*)V, ks, vs, vec, pool,
-                                                              bounds, table, start, count, touched, err);
+        write_kernel<X, D, 256><<<(unsigned)grid, 256, smem, st>>>(s, (const X*)K, (const X*)V, ks, vs, vec, pool,
+                                                                   bounds, table, start, count, touched, page_shift, err);
     note_launch();
     return cudaGetLastError();
 }
@@ -378,10 +430,13 @@ cudaError_t write_as(const Shape& s, const void* K, const void* V, Strides ks, S
 template <typename X, int D>
 cudaError_t read_as(const Shape& s, const uint8_t* pool, const int32_t* table, const int32_t* start,
                     const int32_t* count, void* K, void* V, int* err, cudaStream_t st) {
-    const long long threads = (long long)s.B * s.T * s.H * (D / 8);
-    const long long grid = (threads + 255) / 256;
+    constexpr int kRows = kReadRows * (256 / (D / 8));     // a CTA
+    const long long chunks = ((long long)s.T * s.H + kRows - 1) / kRows, grid = chunks * s.B;
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    read_kernel<X, D><<<(unsigned)grid, 256, 0, st>>>(s, pool, table, start, count, (X*)K, (X*)V, err);
+    int page_shift = 4;
+    while (1 << page_shift < s.P) ++page_shift;
+    read_kernel<X, D><<<(unsigned)grid, 256, 0, st>>>(s, pool, table, start, count, (X*)K, (X*)V, (unsigned)chunks,
+                                                      page_shift, err);
     note_launch();
     return cudaGetLastError();
 }
