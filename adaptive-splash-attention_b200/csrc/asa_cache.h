@@ -44,6 +44,31 @@ __host__ __device__ constexpr int bounds_bytes(int d) { return 2 * d + ASA_CACHE
 
 struct Strides { int64_t b, t, h; };
 
+// The cache's kernels follow one another closely (a step is four to six of them), so
+// each may be set up on the SMs while the one before it drains: a kernel first waits
+// for the memory of all before it, then lets the next be set up.
+#ifdef __CUDACC__
+__device__ __forceinline__ void follow() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, A&&... args) {
+    cudaLaunchConfig_t c{};
+    c.gridDim = dim3(grid);
+    c.blockDim = dim3(block);
+    c.dynamicSmemBytes = smem;
+    c.stream = st;
+    cudaLaunchAttribute at{};
+    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at.val.programmaticStreamSerializationAllowed = 1;
+    c.attrs = &at;
+    c.numAttrs = 1;
+    note_launch();
+    return cudaLaunchKernelEx(&c, kernel, P(args)...);
+}
+#endif
+
 cudaError_t write(const Shape& s, const void* K, const void* V, Strides ks, Strides vs, uint8_t* pool,
                   int8_t* bounds, const int32_t* table, const int32_t* start, const int32_t* count,
                   int* err, cudaStream_t st);

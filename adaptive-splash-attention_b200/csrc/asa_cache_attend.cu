@@ -43,7 +43,6 @@ constexpr int kTile = 2;              // blocks of a tile
 constexpr int kStages = 2;            // tiles a warp has in flight
 constexpr int kItemCost = 8;          // what starting an item costs, in tiles of one CTA
 constexpr int kSegments = 32;         // segments a CTA lines up at a time
-constexpr int kListCap = 2048;        // scores a row keeps in shared memory while its threshold is solved
 
 enum Mode { kSoftmax = 0, kScores = 1, kValues = 2 };
 
@@ -254,6 +253,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
         for (int i = 0; i < kStages; ++i) sm100::mbar_init(&sm.full[warp][i], 1);
         sm100::fence_barrier_init();
     }
+    follow();
     __syncthreads();
 
     // this CTA's run [x, x1) of all the items' tiles
@@ -919,6 +919,7 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Ar
     constexpr int ROWS = 8 * NT;
     __shared__ float s_top[4], s_sum[4];
     __shared__ float4 s_acc[4][D / 4];
+    follow();
     const Shape& s = a.s;
     const int per = a.p.tiles * s.H, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int row = blockIdx.x % ROWS, item_no = blockIdx.x / ROWS;
@@ -973,16 +974,27 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Ar
 
 // ---- the alpha-entmax threshold ----------------------------------------------------
 // One CTA an item's eight rows, a warp a row in the end.  A row's support lies
-// within 1 of its largest x = (alpha - 1) score: the tiles whose maxima reach
-// that are read once to count and once to collect such scores, in an order that
-// does not depend on timing, and the root of sum (x - tau)_+^(1/(alpha-1)) = 1 is
-// found among them by Newton's steps from the left, kept inside a bracket.
+// within 1 of its largest x = (alpha - 1) score: of the tiles whose maxima reach that
+// (listed first) each such x is put on its row's list, every warp in a stretch of its
+// own and in order, so that no sum depends on timing; the stretches are closed up, and
+// the root of sum (x - tau)_+^(1/(alpha-1)) = 1 is found among them by Newton's steps
+// from the left, kept inside a bracket.  Rows with more than a list holds (a flat
+// row, a small alpha) have every step read the tiles again.
+constexpr int kTauThreads = 512, kTauWarps = kTauThreads / 32;
+constexpr int kTileList = 2048;       // tiles listed
+constexpr int kListCap = 1024;        // of a row, closed up
+constexpr int kPart = 96;             // of a row and warp
+constexpr int kTauSmem = (kTileList + 8 * kListCap + 8 * kTauWarps * kPart) * 4;
+
 template <int NT>
-__global__ void __launch_bounds__(256) threshold_kernel(const __grid_constant__ Args a) {
-    constexpr int ROWS = 8 * NT;
-    extern __shared__ float s_list[];                 // [8][kListCap]
-    __shared__ float s_top[8][8], s_sum[8][8][2], s_tau[8];
-    __shared__ int s_count[8][8];                     // [warp][row]
+__global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_constant__ Args a) {
+    constexpr int ROWS = 8 * NT, W = kTauWarps;
+    extern __shared__ int s_tiles[];
+    float* const s_list = reinterpret_cast<float*>(s_tiles + kTileList);     // [8][kListCap]
+    float* const s_part = s_list + 8 * kListCap;                             // [8][W][kPart]
+    __shared__ float s_max[W][8], s_top[8], s_sum[W][8][2], s_tau[8];
+    __shared__ int s_count[W], s_rows[W][8];
+    follow();
     const Shape& s = a.s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, t = lane >> 3;
     const int per = a.p.tiles * s.H, nt = blockIdx.x % NT;
@@ -997,85 +1009,131 @@ __global__ void __launch_bounds__(256) threshold_kernel(const __grid_constant__ 
     const int nb = unit_tiles(a, u);
     const float* tops = a.w.top + item_no * a.p.cap * ROWS + 8 * nt;
     const float4* tiles = a.w.score + (item_no * a.p.cap * kTile * NT + nt) * 32;
-    // the rows' maxima
-    {
-        const int row = tid & 7;
-        float top = -INFINITY;
-        for (int j = tid >> 3; j < nb; j += 32) top = fmaxf(top, __ldg(tops + (int64_t)j * ROWS + row));
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-        if (lane < 8) s_top[warp][lane] = row < rows ? top : -INFINITY;
+    auto tops_of = [&](int j, float (&y)[8]) {
+        const float4 x = __ldg(reinterpret_cast<const float4*>(tops + (int64_t)j * ROWS));
+        const float4 z = __ldg(reinterpret_cast<const float4*>(tops + (int64_t)j * ROWS) + 1);
+        y[0] = x.x, y[1] = x.y, y[2] = x.z, y[3] = x.w, y[4] = z.x, y[5] = z.y, y[6] = z.z, y[7] = z.w;
+    };
+    // the rows' maxima (-inf in rows past the last)
+    float top[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top[i] = -INFINITY;
+#pragma unroll 4
+    for (int j = tid; j < nb; j += kTauThreads) {
+        float y[8];
+        tops_of(j, y);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) top[i] = fmaxf(top[i], y[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+#pragma unroll
+        for (int k = 16; k; k >>= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], k));
+        if (lane == 0) s_max[warp][i] = top[i];
     }
     __syncthreads();
     if (tid < 8) {
-        float top = s_top[0][tid];
-        for (int w = 1; w < 8; ++w) top = fmaxf(top, s_top[w][tid]);
-        s_tau[tid] = top;
+        float y = s_max[0][tid];
+        for (int w = 1; w < W; ++w) y = fmaxf(y, s_max[w][tid]);
+        s_top[tid] = y;
     }
     __syncthreads();
-    float top[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top[i] = s_tau[i];
-    const float top0 = 2 * t < rows ? s_tau[2 * t] : INFINITY, top1 = 2 * t + 1 < rows ? s_tau[2 * t + 1] : INFINITY;
-    // each warp a stretch of tiles; fn(scores) for those that may hold support
-    const int from = (int)((int64_t)nb * warp / 8), to = (int)((int64_t)nb * (warp + 1) / 8);
+    for (int i = 0; i < 8; ++i) top[i] = s_top[i];
+    const float top0 = 2 * t < rows ? s_top[2 * t] : INFINITY, top1 = 2 * t + 1 < rows ? s_top[2 * t + 1] : INFINITY;
+    // the tiles that may hold support, in order
+    int listed = 0;
+    for (int base = 0; base < nb; base += kTauThreads) {
+        bool want = false;
+        if (base + tid < nb) {
+            float y[8];
+            tops_of(base + tid, y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) want |= y[i] > top[i] - 1.0f;
+        }
+        const uint32_t votes = __ballot_sync(~0u, want);
+        if (lane == 0) s_count[warp] = __popc(votes);
+        __syncthreads();
+        int at = listed + __popc(votes & ((1u << lane) - 1u));
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            at += w < warp ? s_count[w] : 0;
+            listed += s_count[w];
+        }
+        if (want && at < kTileList) s_tiles[at] = base + tid;
+        __syncthreads();
+    }
+    // the warp's share of them, several tiles' loads at a time; fn(four scores of rows 2t, 2t + 1)
     auto each = [&](auto fn) {
-        for (int base = from; base < to; base += 32) {
-            bool want = false;
-            if (base + lane < to) {
-                const float* p = tops + (int64_t)(base + lane) * ROWS;
+        constexpr int U = 4;
+        const bool all = listed > kTileList;          // (then every tile is read)
+        const int n = all ? nb : listed;
+        for (int i0 = warp; i0 < n; i0 += U * W) {
+            float4 y[2 * U];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) want |= i < rows && __ldg(p + i) > top[i] - 1.0f;
-            }
-            uint32_t votes = __ballot_sync(~0u, want);
-            while (votes) {                           // four at a time, so that their loads overlap
-                float4 y[8];
+            for (int k = 0; k < U; ++k) {
+                const int i = i0 + k * W;
+                y[2 * k] = y[2 * k + 1] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                if (i < n && 2 * t < rows) {
+                    const int64_t j = all ? i : s_tiles[i];
+                    bool read = true;
+                    if (all) {                        // (a tile that is not there has no scores)
+                        float z[8];
+                        tops_of((int)j, z);
+                        read = false;
 #pragma unroll
-                for (int k = 0; k < 8; k += 2) {
-                    y[k] = y[k + 1] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
-                    if (votes) {
-                        const int64_t j = base + __ffs(votes) - 1;
-                        votes &= votes - 1;
-                        if (2 * t < rows) {
-                            y[k] = __ldg(tiles + (j * kTile) * NT * 32 + lane);
-                            y[k + 1] = __ldg(tiles + (j * kTile + 1) * NT * 32 + lane);
-                        }
+                        for (int e = 0; e < 8; ++e) read |= z[e] > top[e] - 1.0f;
+                    }
+                    if (read) {
+                        y[2 * k] = __ldg(tiles + j * kTile * NT * 32 + lane);
+                        y[2 * k + 1] = __ldg(tiles + (j * kTile + 1) * NT * 32 + lane);
                     }
                 }
-#pragma unroll
-                for (int k = 0; k < 8; ++k) fn(y[k]);
             }
+#pragma unroll
+            for (int k = 0; k < 2 * U; ++k) fn(y[k]);
         }
     };
-    int c0 = 0, c1 = 0;
-    each([&](float4 y) {
-        c0 += (y.x - top0 > -1.0f) + (y.z - top0 > -1.0f);
-        c1 += (y.y - top1 > -1.0f) + (y.w - top1 > -1.0f);
-    });
-    // places: by warp, then by lane within the row's eight lanes
-    int e0 = c0, e1 = c1;
-#pragma unroll
-    for (int k = 1; k < 8; k <<= 1) {
-        const int f0 = __shfl_up_sync(~0u, e0, k, 8), f1 = __shfl_up_sync(~0u, e1, k, 8);
-        if ((lane & 7) >= k) e0 += f0, e1 += f1;
+    int n0 = 0, n1 = 0;                               // on the lists of rows 2t, 2t + 1, of this warp
+    {
+        float* l0 = s_part + (2 * t * W + warp) * kPart;
+        float* l1 = l0 + W * kPart;
+        const int shift = 8 * t;
+        auto put = [&](float y, float* list, int& n) {
+            const bool in = y > -1.0f;
+            const uint32_t votes = __ballot_sync(~0u, in) >> shift & 255u;
+            const int at = n + __popc(votes & ((1u << (lane & 7)) - 1u));
+            if (in && at < kPart) list[at] = y;
+            n += __popc(votes);
+        };
+        each([&](float4 y) {
+            put(y.x - top0, l0, n0);
+            put(y.z - top0, l0, n0);
+            put(y.y - top1, l1, n1);
+            put(y.w - top1, l1, n1);
+        });
     }
-    if ((lane & 7) == 7) s_count[warp][2 * t] = e0, s_count[warp][2 * t + 1] = e1;
+    if ((lane & 7) == 0) s_rows[warp][2 * t] = n0, s_rows[warp][2 * t + 1] = n1;
     __syncthreads();
-    e0 -= c0;
-    e1 -= c1;
     bool fits = true;
-    int mine = 0;                                     // of row `warp`
+    int mine = 0;                                     // on the list of row `warp`
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        int all = 0;
-        for (int w = 0; w < 8; ++w) {
-            if (w < warp && i == 2 * t) e0 += s_count[w][i];
-            if (w < warp && i == 2 * t + 1) e1 += s_count[w][i];
-            all += s_count[w][i];
+        int all = 0, at = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w) {
+            const int n = s_rows[w][i];
+            fits &= n <= kPart;
+            if (w < warp) at += n;
+            all += n;
         }
         fits &= all <= kListCap;
         if (i == warp) mine = all;
+        const int n = min(s_rows[warp][i], kPart);    // the warp's stretch to its place
+        for (int k = lane; k < n; k += 32)
+            if (at + k < kListCap) s_list[i * kListCap + at + k] = s_part[(i * W + warp) * kPart + k];
     }
+    __syncthreads();
     const float ex = 1.0f / (s.alpha - 1.0f);
     auto gain = [&](float y, float tau, float& f, float& df) {   // y, tau relative to the row's maximum
         const float d = y - tau;
@@ -1100,30 +1158,22 @@ __global__ void __launch_bounds__(256) threshold_kernel(const __grid_constant__ 
         return end;
     };
     if (fits) {
-        each([&](float4 y) {
-            float* l0 = s_list + (2 * t) * kListCap;
-            float* l1 = l0 + kListCap;
-            if (y.x - top0 > -1.0f) l0[e0++] = y.x - top0;
-            if (y.z - top0 > -1.0f) l0[e0++] = y.z - top0;
-            if (y.y - top1 > -1.0f) l1[e1++] = y.y - top1;
-            if (y.w - top1 > -1.0f) l1[e1++] = y.w - top1;
-        });
-        __syncthreads();
-        const float* list = s_list + warp * kListCap;
-        float tau = -1.0f, lo = -1.0f, hi = 0.0f;
-        for (int it = 0; it < 60; ++it) {
-            float f = 0.0f, df = 0.0f;
-            for (int i = lane; i < mine; i += 32) gain(list[i], tau, f, df);
+        if (warp < 8) {
+            const float* list = s_list + warp * kListCap;
+            float tau = -1.0f, lo = -1.0f, hi = 0.0f;
+            for (int it = 0; it < 60; ++it) {
+                float f = 0.0f, df = 0.0f;
+                for (int i = lane; i < mine; i += 32) gain(list[i], tau, f, df);
 #pragma unroll
-            for (int k = 16; k; k >>= 1) {
-                f += __shfl_xor_sync(~0u, f, k);
-                df += __shfl_xor_sync(~0u, df, k);
+                for (int k = 16; k; k >>= 1) {
+                    f += __shfl_xor_sync(~0u, f, k);
+                    df += __shfl_xor_sync(~0u, df, k);
+                }
+                if (step(f, df, lo, hi, tau)) break;
             }
-            if (step(f, df, lo, hi, tau)) break;
+            if (lane == 0) s_tau[warp] = tau;
         }
-        if (lane == 0) s_top[0][warp] = tau;
     } else {
-        // the lists do not fit: every step reads the tiles again, all rows at once
         float tau[2] = {-1.0f, -1.0f}, lo[2] = {-1.0f, -1.0f}, hi[2] = {0.0f, 0.0f};
         for (int it = 0; it < 60; ++it) {
             float f[2] = {0.0f, 0.0f}, df[2] = {0.0f, 0.0f};
@@ -1147,18 +1197,18 @@ __global__ void __launch_bounds__(256) threshold_kernel(const __grid_constant__ 
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 float sf = 0.0f, sd = 0.0f;
-                for (int w = 0; w < 8; ++w) sf += s_sum[w][2 * t + e][0], sd += s_sum[w][2 * t + e][1];
-                const bool live = (e ? top1 : top0) > -INFINITY && (e ? top1 : top0) < INFINITY;
-                if (live) end &= step(sf, sd, lo[e], hi[e], tau[e]);
+                for (int w = 0; w < W; ++w) sf += s_sum[w][2 * t + e][0], sd += s_sum[w][2 * t + e][1];
+                const float y = e ? top1 : top0;
+                if (y > -INFINITY && y < INFINITY) end &= step(sf, sd, lo[e], hi[e], tau[e]);
             }
             if (__syncthreads_and(end)) break;
         }
-        if (warp == 0 && (lane & 7) == 0) s_top[0][2 * t] = tau[0], s_top[0][2 * t + 1] = tau[1];
+        if (warp == 0 && (lane & 7) == 0) s_tau[2 * t] = tau[0], s_tau[2 * t + 1] = tau[1];
     }
     __syncthreads();
     if (tid < 8) {
-        const float y = s_tau[tid];
-        tau_out[tid] = y == -INFINITY ? INFINITY : y == INFINITY ? NAN : y + s_top[0][tid];
+        const float y = s_top[tid];
+        tau_out[tid] = y == -INFINITY ? INFINITY : y == INFINITY ? NAN : y + s_tau[tid];
     }
 }
 
@@ -1225,13 +1275,11 @@ cudaError_t launch_walk(const Args& a, cudaStream_t st) {
     if (e != cudaSuccess) return e;
     const int64_t items = (int64_t)a.p.U * a.p.tiles * a.s.H;
     const unsigned grid = a.p.split ? kSms * ctas_of(NT) : (unsigned)items;
-    kernel<<<grid, W * 32, smem, st>>>(a);
-    note_launch();
-    return cudaGetLastError();
+    return launch(kernel, grid, W * 32, smem, st, a);
 }
 
 template <int D, int NT>
-cudaError_t launch(const Args& a, cudaStream_t st) {
+cudaError_t attend_as(const Args& a, cudaStream_t st) {
     const int64_t items = (int64_t)a.p.U * a.p.tiles * a.s.H;
     if (items * 8 * NT > 0x7fffffff) return cudaErrorInvalidConfiguration;
     cudaError_t e;
@@ -1240,18 +1288,13 @@ cudaError_t launch(const Args& a, cudaStream_t st) {
     } else {
         e = launch_walk<D, NT, kScores>(a, st);
         if (e != cudaSuccess) return e;
-        const int smem = 8 * kListCap * 4;
-        e = cudaFuncSetAttribute(threshold_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        e = cudaFuncSetAttribute(threshold_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTauSmem);
         if (e != cudaSuccess) return e;
-        threshold_kernel<NT><<<(unsigned)(items * NT), 256, smem, st>>>(a);
-        note_launch();
-        e = cudaGetLastError();
+        e = launch(threshold_kernel<NT>, (unsigned)(items * NT), kTauThreads, kTauSmem, st, a);
         if (e == cudaSuccess) e = launch_walk<D, NT, kValues>(a, st);
     }
     if (e != cudaSuccess || !a.p.split) return e;
-    combine_kernel<D, NT><<<(unsigned)(items * 8 * NT), 128, 0, st>>>(a);
-    note_launch();
-    return cudaGetLastError();
+    return launch(combine_kernel<D, NT>, (unsigned)(items * 8 * NT), 128, 0, st, a);
 }
 
 }  // namespace
@@ -1278,10 +1321,10 @@ cudaError_t attend(const Shape& s, const void* Q, Strides qs, const uint8_t* poo
     a.p.vec = (reinterpret_cast<uintptr_t>(Q) & 15) == 0 && qs.b % 8 == 0 && qs.t % 8 == 0 && qs.h % 8 == 0;
     const bool two = row_tiles(s, keep > 0) == 2;
     switch (s.d) {
-        case 32: return two ? launch<32, 2>(a, st) : launch<32, 1>(a, st);
-        case 64: return two ? launch<64, 2>(a, st) : launch<64, 1>(a, st);
-        case 96: return two ? launch<96, 2>(a, st) : launch<96, 1>(a, st);
-        default: return two ? launch<128, 2>(a, st) : launch<128, 1>(a, st);
+        case 32: return two ? attend_as<32, 2>(a, st) : attend_as<32, 1>(a, st);
+        case 64: return two ? attend_as<64, 2>(a, st) : attend_as<64, 1>(a, st);
+        case 96: return two ? attend_as<96, 2>(a, st) : attend_as<96, 1>(a, st);
+        default: return two ? attend_as<128, 2>(a, st) : attend_as<128, 1>(a, st);
     }
 }
 

@@ -133,6 +133,7 @@ int asa_cache_select(const asa_cache_params* p, const void* Q, const int64_t q_s
     int rc = check(p, &s, true);
     if (rc) return rc;
     if (keep < 1) return ASA_ERR_INVALID;
+    if (s.G > 256) return ASA_ERR_UNSUPPORTED;           // a query's heads are held in shared memory
     if (!s.B || !s.T) return ASA_OK;
     if ((long long)s.B * s.T * s.H * keep > (1LL << 40)) return ASA_ERR_UNSUPPORTED;
     if (!Q || !q_strides || !lengths || !pages || (s.width && !block_table) || (s.pages && !bounds))

@@ -44,7 +44,6 @@ struct Query {
     const int32_t* table;
     const int32_t* lengths;
     int keep;
-    int vec;                          // q rows may be read 16 bytes at a time
     int* err;
 };
 
@@ -54,85 +53,80 @@ __device__ __forceinline__ int pages_seen(const Query& a, int b, int t) {
     return pos < 0 ? 0 : (int)(pos / a.s.P) + 1;
 }
 
-// Keys of pages from .. to - 1 (ordered scores; put(page, key)) by the warps of a CTA, 16 pages each.
+// A query's whole numbers for one key head, heads rounded up to eights: upper parts
+// (max(n, 0)), then lower ones, and the units.
+template <int D>
+__device__ __forceinline__ void make_query(const Query& a, int b, int t, int h, int8_t* s_q, float* s_unit) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+    const int heads = (a.s.G + 7) & ~7;
+    for (int g = warp; g < heads; g += warps) {
+        const __nv_bfloat16* src = a.Q + b * a.qs.b + t * a.qs.t + (int64_t)(h * a.s.G + g) * a.qs.h;
+        float x[D / 32], big = 0.0f;
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            x[i] = g < a.s.G ? __bfloat162float(src[lane + 32 * i]) : 0.0f;
+            big = fmaxf(big, fabsf(x[i]));
+            bad |= x[i] != x[i];
+        }
+        big = __uint_as_float(__reduce_max_sync(~0u, __float_as_uint(big)));
+        const float unit = __any_sync(~0u, bad) ? NAN : __fmul_rn(big, k127th);
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) {
+            const int n = unit > 0.0f ? (int)rintf(__fdiv_rn(x[i], unit)) : 0;
+            s_q[g * 2 * D + lane + 32 * i] = (int8_t)max(n, 0);
+            s_q[g * 2 * D + D + lane + 32 * i] = (int8_t)min(n, 0);
+        }
+        if (lane == 0) s_unit[g] = unit;
+    }
+}
+
+// Keys of pages from .. to - 1 (ordered scores; put(page, key, whether earlier heads had a say)) by
+// the warps of a CTA, 16 pages each.
 template <int D, typename Put>
-__device__ __forceinline__ void score_pages(const Query& a, int b, int t, int h, int from, int to, int warps, Put put) {
+__device__ __forceinline__ void score_pages(const Query& a, int b, int h, int from, int to, int warps, const int8_t* s_q,
+                                            const float* s_unit, Put put) {
     constexpr int SEG = 2 * D / 64;                   // 64-byte stretches of a page's bounds
     const Shape& s = a.s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, q4 = lane & 3;
-    if (from + 16 * warp >= to) return;
     for (int tile = 0; tile * 8 < s.G; ++tile) {
-        // the lane's part of head 8 tile + r: channels 16 q4 .. + 15 of each stretch, whole numbers
-        const int g = 8 * tile + r;
-        uint32_t raw[SEG][8], w[SEG][4];
-        float big = 0.0f;
-        bool bad = false;
-        const __nv_bfloat16* src = a.Q + b * a.qs.b + t * a.qs.t + (int64_t)(h * s.G + g) * a.qs.h;
+        uint4 w[SEG];
 #pragma unroll
-        for (int k = 0; k < SEG; ++k) {               // (the lower codes' stretches have the upper ones' channels)
-            const uint16_t* e = reinterpret_cast<const uint16_t*>(src + (64 * k + 16 * q4) % D);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) raw[k][i] = 0u;
-            if (g < s.G && a.vec) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint4 v = __ldg(reinterpret_cast<const uint4*>(e) + i);
-                    raw[k][4 * i] = v.x, raw[k][4 * i + 1] = v.y, raw[k][4 * i + 2] = v.z, raw[k][4 * i + 3] = v.w;
-                }
-            } else if (g < s.G) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i) raw[k][i] = __ldg(e + 2 * i) | (uint32_t)__ldg(e + 2 * i + 1) << 16;
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float x = __uint_as_float(raw[k][i] << 16), y = __uint_as_float(raw[k][i] & 0xffff0000u);
-                big = fmaxf(big, fmaxf(fabsf(x), fabsf(y)));
-                bad |= x != x || y != y;
-            }
-        }
-        big = fmaxf(big, __shfl_xor_sync(~0u, big, 1));
-        big = fmaxf(big, __shfl_xor_sync(~0u, big, 2));
-        const bool row_bad = (__ballot_sync(~0u, bad) >> (lane & 28)) & 15u;
-        const float unit = row_bad ? NAN : __fmul_rn(big, k127th);
-#pragma unroll
-        for (int k = 0; k < SEG; ++k) {
-            const bool upper = 64 * k + 16 * q4 < D;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                uint32_t word = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const uint32_t two = raw[k][2 * j + i / 2];
-                    const float x = __uint_as_float(i & 1 ? two & 0xffff0000u : two << 16);
-                    const int n = unit > 0.0f ? (int)rintf(__fdiv_rn(x, unit)) : 0;
-                    word |= (uint32_t)((upper ? max(n, 0) : min(n, 0)) & 255) << (8 * i);
-                }
-                w[k][j] = word;
-            }
-        }
-        const float u0 = __shfl_sync(~0u, unit, 8 * q4), u1 = __shfl_sync(~0u, unit, 8 * q4 + 4);
+        for (int k = 0; k < SEG; ++k)
+            w[k] = *reinterpret_cast<const uint4*>(s_q + (8 * tile + r) * 2 * D + 64 * k + 16 * q4);
+        const float u0 = s_unit[8 * tile + 2 * q4], u1 = s_unit[8 * tile + 2 * q4 + 1];
         const bool in0 = 8 * tile + 2 * q4 < s.G, in1 = 8 * tile + 2 * q4 + 1 < s.G;
-        for (int p0 = from + 16 * warp; p0 < to; p0 += 16 * warps) {
-            const int8_t* rec[2];
-            float scale[2];
+        int next[2];                                  // the pages' ids, looked up an iteration ahead
+        auto look_up = [&](int p0) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int page = p0 + r + 8 * e;
-                const int id = page < to ? __ldg(a.table + (int64_t)b * s.width + page) : -1;
+                next[e] = page < to ? __ldg(a.table + (int64_t)b * s.width + page) : -1;
+            }
+        };
+        look_up(from + 16 * warp);
+        for (int p0 = from + 16 * warp; p0 < to; p0 += 16 * warps) {
+            const int8_t* rec[2];
+            float scale[2];
+            uint4 x[2][SEG];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int id = next[e];
                 rec[e] = nullptr;
                 scale[e] = 0.0f;
                 if (id >= 0 && id < s.pages) rec[e] = a.bounds + ((int64_t)id * s.H + h) * bounds_bytes(D);
-                else if (page < to && q4 == 0 && a.err) atomicCAS(a.err, 0, ASA_ERR_INVALID);
+                else if (p0 + r + 8 * e < to && q4 == 0 && a.err) atomicCAS(a.err, 0, ASA_ERR_INVALID);
+#pragma unroll
+                for (int k = 0; k < SEG; ++k)
+                    x[e][k] = rec[e] ? __ldg(reinterpret_cast<const uint4*>(rec[e] + 64 * k + 16 * q4)) : make_uint4(0u, 0u, 0u, 0u);
                 if (rec[e]) scale[e] = __int_as_float((min(max(__ldg(reinterpret_cast<const int*>(rec[e] + 2 * D)), -126), 127) + 127) << 23);
             }
+            look_up(p0 + 16 * warps);
             int acc[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int k = 0; k < SEG; ++k) {
-                const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
-                const uint4 x = rec[0] ? __ldg(reinterpret_cast<const uint4*>(rec[0] + 64 * k + 16 * q4)) : zero;
-                const uint4 y = rec[1] ? __ldg(reinterpret_cast<const uint4*>(rec[1] + 64 * k + 16 * q4)) : zero;
-                mma_s8(acc, x.x, y.x, x.y, y.y, w[k][0], w[k][1]);
-                mma_s8(acc, x.z, y.z, x.w, y.w, w[k][2], w[k][3]);
+                mma_s8(acc, x[0][k].x, x[1][k].x, x[0][k].y, x[1][k].y, w[k].x, w[k].y);
+                mma_s8(acc, x[0][k].z, x[1][k].z, x[0][k].w, x[1][k].w, w[k].z, w[k].w);
             }
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -151,14 +145,18 @@ __device__ __forceinline__ void score_pages(const Query& a, int b, int t, int h,
 // Keys of an item's pages, kChunk a CTA, for items whose keys do not fit in shared memory.
 template <int D>
 __global__ void __launch_bounds__(256) score_kernel(const __grid_constant__ Query a, uint32_t* __restrict__ keys, int chunks) {
+    follow();
     const int item = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
     const int h = item % a.s.H, bt = item / a.s.H, t = bt % a.s.T, b = bt / a.s.T;
     const int n = pages_seen(a, b, t);
     if (n <= a.keep) return;
     uint32_t* key = keys + (int64_t)item * a.s.width;
-    score_pages<D>(a, b, t, h, chunk * kChunk, min((chunk + 1) * kChunk, n - 1), 8, [&](int page, uint32_t k, bool more) {
-        key[page] = more ? max(key[page], k) : k;
-    });
+    extern __shared__ __align__(16) int8_t s_q[];
+    float* s_unit = reinterpret_cast<float*>(s_q + ((a.s.G + 7) & ~7) * 2 * D);
+    make_query<D>(a, b, t, h, s_q, s_unit);
+    __syncthreads();
+    score_pages<D>(a, b, h, chunk * kChunk, min((chunk + 1) * kChunk, n - 1), 8, s_q, s_unit,
+                   [&](int page, uint32_t k, bool more) { key[page] = more ? max(key[page], k) : k; });
 }
 
 // One CTA a (query, key head): its keys (scored here, where they fit in shared
@@ -166,10 +164,13 @@ __global__ void __launch_bounds__(256) score_kernel(const __grid_constant__ Quer
 template <int D, bool SHARED>
 __global__ void __launch_bounds__(kThreads) pick_kernel(const __grid_constant__ Query a, const uint32_t* __restrict__ keys,
                                                         int32_t* __restrict__ pages) {
-    extern __shared__ uint32_t s_key[];
+    extern __shared__ __align__(16) int8_t s_q[];    // the query, its units, the keys
     __shared__ int s_count[2][kWarps];
+    float* s_unit = reinterpret_cast<float*>(s_q + ((a.s.G + 7) & ~7) * 2 * D);
+    uint32_t* s_key = reinterpret_cast<uint32_t*>(s_unit + ((a.s.G + 7) & ~7));
     const Shape& s = a.s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, keep = a.keep;
+    follow();
     const int h = blockIdx.x % s.H, bt = blockIdx.x / s.H, t = bt % s.T, b = bt / s.T;
     int32_t* out = pages + (int64_t)blockIdx.x * keep;
     const int n = pages_seen(a, b, t);
@@ -179,9 +180,10 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const __grid_constant__ 
     }
     const int m = n - 1;                              // those that are weighed; the query's own is taken
     if constexpr (SHARED) {
-        score_pages<D>(a, b, t, h, 0, m, kWarps, [&](int page, uint32_t k, bool more) {
-            s_key[page] = more ? max(s_key[page], k) : k;
-        });
+        make_query<D>(a, b, t, h, s_q, s_unit);
+        __syncthreads();
+        score_pages<D>(a, b, h, 0, m, kWarps, s_q, s_unit,
+                       [&](int page, uint32_t k, bool more) { s_key[page] = more ? max(s_key[page], k) : k; });
         __syncthreads();
     }
     const uint32_t* key = SHARED ? s_key : keys + (int64_t)blockIdx.x * s.width;
@@ -253,19 +255,22 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const __grid_constant__ 
 template <int D>
 cudaError_t select_as(const Query& a, int32_t* pages, void* ws, cudaStream_t st) {
     const unsigned items = (unsigned)(a.s.B * a.s.T * a.s.H);
+    const size_t query = (size_t)((a.s.G + 7) & ~7) * (2 * D + 4) /* 67 KB at most */, keys = (size_t)a.s.width * 4;
     if (a.s.width <= kShared) {
-        pick_kernel<D, true><<<items, kThreads, (size_t)a.s.width * 4, st>>>(a, nullptr, pages);
-    } else {
-        const int chunks = (a.s.width + kChunk - 1) / kChunk;
-        if ((int64_t)items * chunks > 0x7fffffff) return cudaErrorInvalidConfiguration;
-        score_kernel<D><<<items * chunks, 256, 0, st>>>(a, (uint32_t*)ws, chunks);
-        note_launch();
-        cudaError_t e = cudaGetLastError();
-        if (e != cudaSuccess) return e;
-        pick_kernel<D, false><<<items, kThreads, 0, st>>>(a, (const uint32_t*)ws, pages);
+        if (query + keys > 48 * 1024) {
+            const cudaError_t e = cudaFuncSetAttribute(pick_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 116 * 1024);
+            if (e != cudaSuccess) return e;
+        }
+        return launch(pick_kernel<D, true>, items, kThreads, query + keys, st, a, (const uint32_t*)nullptr, pages);
     }
-    note_launch();
-    return cudaGetLastError();
+    const int chunks = (a.s.width + kChunk - 1) / kChunk;
+    if ((int64_t)items * chunks > 0x7fffffff) return cudaErrorInvalidConfiguration;
+    if (query > 48 * 1024) {
+        const cudaError_t e = cudaFuncSetAttribute(score_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+        if (e != cudaSuccess) return e;
+    }
+    const cudaError_t e = launch(score_kernel<D>, items * chunks, 256, query, st, a, (uint32_t*)ws, chunks);
+    return e != cudaSuccess ? e : launch(pick_kernel<D, false>, items, kThreads, 0, st, a, (const uint32_t*)ws, pages);
 }
 
 }  // namespace
@@ -277,8 +282,7 @@ size_t select_workspace(const Shape& s) {
 
 cudaError_t select(const Shape& s, const void* Q, Strides qs, const int8_t* bounds, const int32_t* table,
                    const int32_t* lengths, int keep, int32_t* pages, void* ws, int* err, cudaStream_t st) {
-    const int vec = (reinterpret_cast<uintptr_t>(Q) & 15) == 0 && qs.b % 8 == 0 && qs.t % 8 == 0 && qs.h % 8 == 0;
-    const Query a{s, (const __nv_bfloat16*)Q, qs, bounds, table, lengths, keep, vec, err};
+    const Query a{s, (const __nv_bfloat16*)Q, qs, bounds, table, lengths, keep, err};
     switch (s.d) {
         case 32: return select_as<32>(a, pages, ws, st);
         case 64: return select_as<64>(a, pages, ws, st);

@@ -178,6 +178,7 @@ __global__ void __launch_bounds__(NTHR) write_kernel(Shape s, const X* __restric
     extern __shared__ __align__(16) uint8_t s_rec[];  // rows of codes and of scales: [2][page][RB], [2][page][PB]
     __shared__ float s_hi[SETS][D], s_lo[SETS][D];
     __shared__ float s_m[W];
+    follow();
     const unsigned bj = blockIdx.x / (unsigned)s.H;
     const int h = blockIdx.x - bj * s.H, b = bj / (unsigned)touched, j = bj - b * touched;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -325,6 +326,7 @@ __global__ void __launch_bounds__(256) read_kernel(Shape s, const uint8_t* __res
                                                    const int32_t* __restrict__ count, X* __restrict__ K,
                                                    X* __restrict__ V, unsigned chunks, int page_shift, int* err) {
     constexpr int NG = D / 32, R = D / 8, RB = row_bytes(D), ROWS = 256 / R;   // rows of the CTA at a time
+    follow();
     const unsigned b = blockIdx.x / chunks, chunk = blockIdx.x - b * chunks;
     const unsigned run = threadIdx.x % R, first = chunk * (kReadRows * ROWS) + threadIdx.x / R;
     if (threadIdx.x / R >= ROWS) return;              // (96 channels leave four threads over)
@@ -384,6 +386,7 @@ __global__ void __launch_bounds__(256) bounds_kernel(Shape s, const int8_t* __re
                                                      const int32_t* __restrict__ pages, int n,
                                                      float* __restrict__ upper, float* __restrict__ lower,
                                                      int* err) {
+    follow();
     const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
     if (i >= (int64_t)n * s.H * s.d) return;
     const int c = (int)(i % s.d), h = (int)(i / s.d % s.H);
@@ -417,14 +420,9 @@ cudaError_t write_as(const Shape& s, const void* K, const void* V, Strides ks, S
     const int vec = fits(K, ks) && fits(V, vs);
     const size_t smem = (size_t)2 * s.P * (row_bytes(D) + par_bytes(D));   // 20 KB at most
     // A step writes a token or a few of each sequence: two warps a page then start sooner than eight.
-    if (s.T <= 4)
-        write_kernel<X, D, 64><<<(unsigned)grid, 64, smem, st>>>(s, (const X*)K, (const X*)V, ks, vs, vec, pool, bounds,
-                                                                 table, start, count, touched, page_shift, err);
-    else
-        write_kernel<X, D, 256><<<(unsigned)grid, 256, smem, st>>>(s, (const X*)K, (const X*)V, ks, vs, vec, pool,
-                                                                   bounds, table, start, count, touched, page_shift, err);
-    note_launch();
-    return cudaGetLastError();
+    const auto kernel = s.T <= 4 ? write_kernel<X, D, 64> : write_kernel<X, D, 256>;
+    return launch(kernel, (unsigned)grid, s.T <= 4 ? 64 : 256, smem, st, s, (const X*)K, (const X*)V, ks, vs, vec, pool,
+                  bounds, table, start, count, touched, page_shift, err);
 }
 
 template <typename X, int D>
@@ -435,10 +433,8 @@ cudaError_t read_as(const Shape& s, const uint8_t* pool, const int32_t* table, c
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
     int page_shift = 4;
     while (1 << page_shift < s.P) ++page_shift;
-    read_kernel<X, D><<<(unsigned)grid, 256, 0, st>>>(s, pool, table, start, count, (X*)K, (X*)V, (unsigned)chunks,
-                                                      page_shift, err);
-    note_launch();
-    return cudaGetLastError();
+    return launch(read_kernel<X, D>, (unsigned)grid, 256, 0, st, s, pool, table, start, count, (X*)K, (X*)V,
+                  (unsigned)chunks, page_shift, err);
 }
 
 }  // namespace
@@ -469,9 +465,7 @@ cudaError_t read_bounds(const Shape& s, const int8_t* bounds, const int32_t* pag
                         float* lower, int* err, cudaStream_t st) {
     const long long grid = ((long long)n * s.H * s.d + 255) / 256;
     if (grid > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    bounds_kernel<<<(unsigned)grid, 256, 0, st>>>(s, bounds, pages, n, upper, lower, err);
-    note_launch();
-    return cudaGetLastError();
+    return launch(bounds_kernel, (unsigned)grid, 256, 0, st, s, bounds, pages, n, upper, lower, err);
 }
 
 }  // namespace cache

@@ -282,7 +282,7 @@ int asa_cache_bounds(const asa_cache_params* p, const void* bounds, const int32_
  * score is max over the group's heads of unit_q * 2^e * sum_c max(n_c upper_c,
  * n_c lower_c), n = rint(q / unit_q), unit_q = max|q| * r with r the fp32
  * number nearest 1/127: sums of whole numbers, the same in any order.  Ties go to the lower page; a NaN scores
- * lowest.  Q [B, T, heads, d] bf16, pages int32 [B, T, kv_heads, keep]. */
+ * lowest.  At most 256 query heads a key head.  Q [B, T, heads, d] bf16, pages int32 [B, T, kv_heads, keep]. */
 int asa_cache_select(const asa_cache_params* p, const void* Q, const int64_t q_strides[3],
                      const void* bounds, const int32_t* block_table, const int32_t* lengths,
                      int keep, int32_t* pages, void* ws, size_t ws_bytes, asa_stream_t stream);
