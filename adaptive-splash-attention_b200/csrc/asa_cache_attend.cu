@@ -975,25 +975,24 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Ar
 // ---- the alpha-entmax threshold ----------------------------------------------------
 // One CTA an item's eight rows, a warp a row in the end.  A row's support lies
 // within 1 of its largest x = (alpha - 1) score: of the tiles whose maxima reach that
-// (listed first) each such x is put on its row's list, every warp in a stretch of its
-// own and in order, so that no sum depends on timing; the stretches are closed up, and
-// the root of sum (x - tau)_+^(1/(alpha-1)) = 1 is found among them by Newton's steps
+// (listed first) each such x is put on its row's list, every lane in a stretch of its
+// own, so that no sum depends on timing; the stretches are closed up, and the root of sum (x - tau)_+^(1/(alpha-1)) = 1 is found among them by Newton's steps
 // from the left, kept inside a bracket.  Rows with more than a list holds (a flat
 // row, a small alpha) have every step read the tiles again.
 constexpr int kTauThreads = 512, kTauWarps = kTauThreads / 32;
 constexpr int kTileList = 2048;       // tiles listed
 constexpr int kListCap = 1024;        // of a row, closed up
-constexpr int kPart = 96;             // of a row and warp
-constexpr int kTauSmem = (kTileList + 8 * kListCap + 8 * kTauWarps * kPart) * 4;
+constexpr int kPart = 13;             // of a row and lane (odd: no bank twice)
+constexpr int kTauSmem = (kTileList + 8 * kListCap + 8 * kTauWarps * 8 * kPart) * 4;
 
 template <int NT>
 __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_constant__ Args a) {
     constexpr int ROWS = 8 * NT, W = kTauWarps;
     extern __shared__ int s_tiles[];
     float* const s_list = reinterpret_cast<float*>(s_tiles + kTileList);     // [8][kListCap]
-    float* const s_part = s_list + 8 * kListCap;                             // [8][W][kPart]
+    float* const s_part = s_list + 8 * kListCap;                             // [8][W * 8][kPart]
     __shared__ float s_max[W][8], s_top[8], s_sum[W][8][2], s_tau[8];
-    __shared__ int s_count[W], s_rows[W][8];
+    __shared__ int s_count[W], s_rows[8][W * 8], s_mine[8];
     follow();
     const Shape& s = a.s;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, t = lane >> 3;
@@ -1094,44 +1093,49 @@ __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_con
             for (int k = 0; k < 2 * U; ++k) fn(y[k]);
         }
     };
-    int n0 = 0, n1 = 0;                               // on the lists of rows 2t, 2t + 1, of this warp
-    {
-        float* l0 = s_part + (2 * t * W + warp) * kPart;
-        float* l1 = l0 + W * kPart;
-        const int shift = 8 * t;
-        auto put = [&](float y, float* list, int& n) {
-            const bool in = y > -1.0f;
-            const uint32_t votes = __ballot_sync(~0u, in) >> shift & 255u;
-            const int at = n + __popc(votes & ((1u << (lane & 7)) - 1u));
-            if (in && at < kPart) list[at] = y;
-            n += __popc(votes);
-        };
-        each([&](float4 y) {
-            put(y.x - top0, l0, n0);
-            put(y.z - top0, l0, n0);
-            put(y.y - top1, l1, n1);
-            put(y.w - top1, l1, n1);
-        });
-    }
-    if ((lane & 7) == 0) s_rows[warp][2 * t] = n0, s_rows[warp][2 * t + 1] = n1;
-    __syncthreads();
-    bool fits = true;
-    int mine = 0;                                     // on the list of row `warp`
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        int all = 0, at = 0;
-#pragma unroll
-        for (int w = 0; w < W; ++w) {
-            const int n = s_rows[w][i];
-            fits &= n <= kPart;
-            if (w < warp) at += n;
-            all += n;
+    int n0 = 0, n1 = 0;                               // on the lane's stretches of rows 2t, 2t + 1
+    const int stretch = warp * 8 + (lane & 7);
+    float* const l0 = s_part + (2 * t * W * 8 + stretch) * kPart;
+    float* const l1 = l0 + W * 8 * kPart;
+    auto put = [&](float y, float* list, int& n) {
+        if (y > -1.0f) {
+            if (n < kPart) list[n] = y;
+            ++n;
         }
-        fits &= all <= kListCap;
-        if (i == warp) mine = all;
-        const int n = min(s_rows[warp][i], kPart);    // the warp's stretch to its place
-        for (int k = lane; k < n; k += 32)
-            if (at + k < kListCap) s_list[i * kListCap + at + k] = s_part[(i * W + warp) * kPart + k];
+    };
+    each([&](float4 y) {
+        put(y.x - top0, l0, n0);
+        put(y.z - top0, l0, n0);
+        put(y.y - top1, l1, n1);
+        put(y.w - top1, l1, n1);
+    });
+    s_rows[2 * t][stretch] = n0;
+    s_rows[2 * t + 1][stretch] = n1;
+    __syncthreads();
+    if (warp < 8) {                                   // where row `warp`'s stretches go
+        int n[W / 4], sum = 0;
+#pragma unroll
+        for (int k = 0; k < W / 4; ++k) n[k] = s_rows[warp][lane * (W / 4) + k], sum += n[k];
+        int at = sum;
+#pragma unroll
+        for (int k = 1; k < 32; k <<= 1) {
+            const int y = __shfl_up_sync(~0u, at, k);
+            if (lane >= k) at += y;
+        }
+        if (lane == 31) s_mine[warp] = at;
+        at -= sum;
+#pragma unroll
+        for (int k = 0; k < W / 4; ++k) s_rows[warp][lane * (W / 4) + k] = at, at += n[k];
+    }
+    bool fits = n0 <= kPart && n1 <= kPart;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) fits &= s_mine[i] <= kListCap;
+    fits = __syncthreads_and(fits);
+    const int mine = s_mine[warp & 7];                // on the list of row `warp`
+    if (fits) {
+        for (int k = 0; k < n0; ++k) s_list[2 * t * kListCap + s_rows[2 * t][stretch] + k] = l0[k];
+        for (int k = 0; k < n1; ++k) s_list[(2 * t + 1) * kListCap + s_rows[2 * t + 1][stretch] + k] = l1[k];
     }
     __syncthreads();
     const float ex = 1.0f / (s.alpha - 1.0f);

@@ -159,6 +159,17 @@ __global__ void __launch_bounds__(256) score_kernel(const __grid_constant__ Quer
                    [&](int page, uint32_t k, bool more) { key[page] = more ? max(key[page], k) : k; });
 }
 
+// Sum of a number a warp over the CTA, and over the warps before this one.  One
+// barrier; `slot` must not be written again before another.
+__device__ __forceinline__ int cta_sum(int v, int* slot, int* before = nullptr) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) slot[warp] = v;
+    __syncthreads();
+    const int of = lane < kWarps ? slot[lane] : 0;
+    if (before) *before = __reduce_add_sync(~0u, lane < warp ? of : 0);
+    return __reduce_add_sync(~0u, of);
+}
+
 // One CTA a (query, key head): its keys (scored here, where they fit in shared
 // memory), the edge between taken and left, and the taken pages in ascending order.
 template <int D, bool SHARED>
@@ -192,19 +203,14 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const __grid_constant__ 
     uint32_t edge = 0;
     int above = m;                                    // keys that reach it
     if (need == 0) edge = ~0u, above = -1;            // (none is taken)
-    for (int bit = 31, turn = 0; bit >= 0 && above != need && need; --bit, turn ^= 1) {
+    int turn = 0;
+    for (int bit = 31; bit >= 0 && above != need && need; --bit, turn ^= 1) {
         const uint32_t next = edge | 1u << bit;
         int count = 0;
         for (int i = tid; i < m; i += kThreads) count += key[i] >= next;
-        count = __reduce_add_sync(~0u, count);
-        if (lane == 0) s_count[turn][warp] = count;
-        __syncthreads();
-        count = 0;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) count += s_count[turn][w];
+        count = cta_sum(__reduce_add_sync(~0u, count), s_count[turn]);
         if (count >= need) edge = next, above = count;
     }
-    __syncthreads();
     // Keys beyond the edge are taken, and of those on it the first; where exactly
     // `need` reach it, all are.
     int before = 0, tied = 0, ties = 0;
@@ -212,13 +218,8 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const __grid_constant__ 
     if (!all && need) {
         int count = 0;
         for (int i = tid; i < m; i += kThreads) count += key[i] > edge;
-        count = __reduce_add_sync(~0u, count);
-        if (lane == 0) s_count[0][warp] = count;
-        __syncthreads();
-        ties = need;
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) ties -= s_count[0][w];
-        __syncthreads();
+        ties = need - cta_sum(__reduce_add_sync(~0u, count), s_count[turn]);
+        turn ^= 1;
     }
     for (int base = 0; base < m; base += kThreads) {
         const int i = base + tid;
@@ -227,27 +228,19 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const __grid_constant__ 
         if (ties) {                                   // (the same in all threads)
             const bool tie = i < m && k == edge;
             const uint32_t votes = __ballot_sync(~0u, tie);
-            if (lane == 0) s_count[0][warp] = __popc(votes);
-            __syncthreads();
-            int rank = tied + __popc(votes & ((1u << lane) - 1u));
-#pragma unroll
-            for (int w = 0; w < kWarps; ++w) {
-                rank += w < warp ? s_count[0][w] : 0;
-                tied += s_count[0][w];
-            }
+            int rank;
+            const int sum = cta_sum(__popc(votes), s_count[turn], &rank);
+            turn ^= 1;
+            rank += tied + __popc(votes & ((1u << lane) - 1u));
+            tied += sum;
             take |= tie && rank < ties;
         }
         const uint32_t votes = __ballot_sync(~0u, take);
-        if (lane == 0) s_count[1][warp] = __popc(votes);
-        __syncthreads();
-        int at = before + __popc(votes & ((1u << lane) - 1u));
-#pragma unroll
-        for (int w = 0; w < kWarps; ++w) {
-            at += w < warp ? s_count[1][w] : 0;
-            before += s_count[1][w];
-        }
-        if (take) out[at] = i;
-        __syncthreads();
+        int at;
+        const int sum = cta_sum(__popc(votes), s_count[turn], &at);
+        turn ^= 1;
+        if (take) out[before + at + __popc(votes & ((1u << lane) - 1u))] = i;
+        before += sum;
     }
     if (tid == 0) out[keep - 1] = m;
 }
