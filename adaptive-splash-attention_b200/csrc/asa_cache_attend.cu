@@ -29,57 +29,19 @@
 // neither a small weight nor a small scale falls among fp16's subnormals; a running
 // exponent lowers it where scales above 2 would overflow.  Sums, maxima and
 // accumulators are fp32.
-#include "asa_cache.h"
-#include "asa_sm100.cuh"
+#include "asa_cache_attend.cuh"
 
 namespace asa {
 namespace cache {
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kTop = 14.0f;         // log2 of the weight that a row's largest score gets
-constexpr float kLow = -1.0e30f;      // below any score
 constexpr int kTile = 2;              // blocks of a tile
 constexpr int kStages = 2;            // tiles a warp has in flight
-constexpr int kItemCost = 8;          // what starting an item costs, in tiles of one CTA
+constexpr int kItemCost = 8;          // Plan::item_cost
 constexpr int kSegments = 32;         // segments a CTA lines up at a time
 
+
 enum Mode { kSoftmax = 0, kScores = 1, kValues = 2 };
-
-// How a call's rows are tiled and its work cut.
-struct Plan {
-    int U, R, tiles;                  // units of rows (sequences; with lists, query tokens), rows each, tiles each
-    int keep;                         // pages listed a query and key head (0: all of the table)
-    int cap;                          // tiles an item can have at most
-    int split;                        // items are cut into equal runs (else one CTA an item)
-    int vec;                          // q rows may be read 16 bytes at a time
-    int page_shift;                   // log2 of the blocks of a page
-    int least;                        // tiles a run has at least
-};
-
-// The workspace: [run length | prefix per unit | partials | scores, tile maxima, thresholds]
-struct Space {
-    int64_t* run;                     // [1 + U]
-    float* part;                      // [2 * CTAs][rows][D]
-    float* part_ml;                   // [2 * CTAs][2][rows]
-    float4* score;                    // [items][cap][2][NT][32]
-    float* top;                       // [items][cap][8 NT]
-    float* tau;                       // [items][8 NT]
-};
-
-struct Args {
-    Shape s;
-    Plan p;
-    Space w;
-    Strides qs;
-    const __nv_bfloat16* Q;
-    const uint8_t* pool;
-    const int32_t* table;
-    const int32_t* lengths;
-    const int32_t* list;
-    __nv_bfloat16* O;
-    int* err;
-};
 
 // ---- small pieces --------------------------------------------------------------
 __device__ __forceinline__ void mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
@@ -121,29 +83,6 @@ __device__ __forceinline__ uint32_t hmax2(uint32_t a, uint32_t b) {
     const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
-__device__ __forceinline__ float exp2_fast(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ float pow2i(int e) { return __int_as_float((e + 127) << 23); }   // e in -126..127
-
-__device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                 ::"r"(sm100::smem_u32(dst)), "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar)) : "memory");
-}
-// Bounded wait for a block's copy.  An error word set by something else than a
-// wait that gave up (a page outside the pool) does not cut it short.
-__device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity, long long spins, int* err) {
-    if (sm100::mbar_try(bar, parity)) return true;
-    for (long long i = 0; i < spins; ++i) {
-        if (sm100::mbar_try(bar, parity)) return true;
-        if ((i & 1023) == 1023 && err && *reinterpret_cast<volatile int*>(err) == ASA_ERR_DEVICE_TIMEOUT) return false;
-    }
-    if (err) atomicExch(err, ASA_ERR_DEVICE_TIMEOUT);
-    return false;
-}
-
 // The token (0..7) that stands at index m of an 8-token half block in the
 // fragments: neighbours 2, 3 and 6, 7 trade places, which spreads the values' rows
 // over the shared-memory banks.
@@ -178,35 +117,6 @@ __device__ __forceinline__ void lds_halves(const uint8_t* p, uint32_t (&w)[(NH +
     } else {
         w[0] = *reinterpret_cast<const uint16_t*>(p);
     }
-}
-
-__device__ __forceinline__ int unit_tiles(const Args& a, int u) {
-    if (a.list) return a.p.cap;
-    const long long n = min((long long)max(__ldg(a.lengths + u), 0), (long long)a.s.width * a.s.P);
-    return (int)((n + kTile * kBlock - 1) / (kTile * kBlock));
-}
-
-// Exclusive prefix of one value a thread over the CTA; *total to all.
-template <int NTHR>
-__device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* s_warp, int64_t* total) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int64_t x = v;
-#pragma unroll
-    for (int k = 1; k < 32; k <<= 1) {
-        const int64_t y = __shfl_up_sync(~0u, x, k);
-        if (lane >= k) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) s_warp[warp] = x;
-    __syncthreads();
-    int64_t before = 0, sum = 0;
-#pragma unroll
-    for (int w = 0; w < NTHR / 32; ++w) {
-        if (w < warp) before += s_warp[w];
-        sum += s_warp[w];
-    }
-    *total = sum;
-    return before + x - v;
 }
 
 // ---- the walk over keys and values ----------------------------------------------
@@ -264,7 +174,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
         int64_t sum, v = 0;
         if (base + tid < a.p.U) {
             const int n = unit_tiles(a, base + tid);
-            if (n) v = (int64_t)(n + kItemCost) * per;
+            if (n) v = (int64_t)(n + a.p.item_cost) * per;
         }
         const int64_t e = block_scan<NTHR>(v, sm.scan, &sum);
         sm.pref[tid] = before + e;
@@ -321,10 +231,10 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                 const int64_t stop = min(x1, sm.pref[NTHR]);
                 while (y < stop && k < kSegments) {
                     while (sm.pref[lo + 1] <= y) ++lo;
-                    const int of = (int)((sm.pref[lo + 1] - sm.pref[lo]) / per) - kItemCost;
+                    const int of = (int)((sm.pref[lo + 1] - sm.pref[lo]) / per) - a.p.item_cost;
                     const int64_t off = y - sm.pref[lo];
-                    const int item = (int)(off / (of + kItemCost));
-                    const int64_t begin = sm.pref[lo] + (int64_t)item * (of + kItemCost) + kItemCost;
+                    const int item = (int)(off / (of + a.p.item_cost));
+                    const int64_t begin = sm.pref[lo] + (int64_t)item * (of + a.p.item_cost) + a.p.item_cost;
                     const int from = (int)max((int64_t)0, y - begin), to = (int)min((int64_t)of, stop - begin);
                     if (to > from) sm.seg[k++] = Segment{chunk + lo, item, from, to - from, of};
                     y = min(stop, begin + of);
@@ -912,66 +822,6 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
         for (int i = 0; i < kStages; ++i) sm100::mbar_drain(&sm.full[warp][i], i < stage_out ? parity : parity ^ 1u);
 }
 
-// ---- joining an item that several CTAs walked -------------------------------------
-// A CTA a row: its warps take the parts in turn, a lane four channels.
-template <int D, int NT>
-__global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Args a) {
-    constexpr int ROWS = 8 * NT;
-    __shared__ float s_top[4], s_sum[4];
-    __shared__ float4 s_acc[4][D / 4];
-    follow();
-    const Shape& s = a.s;
-    const int per = a.p.tiles * s.H, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = blockIdx.x % ROWS, item_no = blockIdx.x / ROWS;
-    const int u = item_no / per, item = item_no % per, h = item / a.p.tiles, tile = item % a.p.tiles;
-    if (tile * ROWS + row >= a.p.R) return;
-    const int of = unit_tiles(a, u);
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float sum = 0.0f;
-    if (of) {
-        const int64_t run = a.w.run[0], x0 = a.w.run[1 + u] + (int64_t)item * (of + kItemCost) + kItemCost;
-        const int64_t c0 = x0 / run, c1 = (x0 + of - 1) / run;
-        if (c0 == c1) return;                         // one CTA had it all, and wrote the output
-        const int n = (int)(c1 - c0) + 1;
-        // the last CTA's part is its first segment, the others' their last
-        auto slot = [&](int i) { return 2 * (c0 + i) + (i + 1 < n ? 1 : 0); };
-        float top = kLow;
-        for (int i = threadIdx.x; i < n; i += 128) top = fmaxf(top, a.w.part_ml[(slot(i) * ROWS + row) * 2]);
-#pragma unroll
-        for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, k));
-        if (lane == 0) s_top[warp] = top;
-        __syncthreads();
-        top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-#pragma unroll 4
-        for (int i = warp; i < n; i += 4) {
-            const float2 ml = *reinterpret_cast<const float2*>(a.w.part_ml + (slot(i) * ROWS + row) * 2);
-            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (lane < D / 4) y = *reinterpret_cast<const float4*>(a.w.part + (slot(i) * ROWS + row) * D + 4 * lane);
-            const float f = exp2_fast(ml.x - top);
-            sum = fmaf(ml.y, f, sum);
-            acc = make_float4(fmaf(y.x, f, acc.x), fmaf(y.y, f, acc.y), fmaf(y.z, f, acc.z), fmaf(y.w, f, acc.w));
-        }
-        if (lane == 0) s_sum[warp] = sum;
-        if (lane < D / 4) s_acc[warp][lane] = acc;
-        __syncthreads();
-        sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-        if (lane < D / 4) {
-            acc = s_acc[0][lane];
-#pragma unroll
-            for (int w = 1; w < 4; ++w) {
-                const float4 y = s_acc[w][lane];
-                acc = make_float4(acc.x + y.x, acc.y + y.y, acc.z + y.z, acc.w + y.w);
-            }
-        }
-    }
-    if (warp || lane >= D / 4) return;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    __nv_bfloat162 y[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv), __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
-    const int b = a.list ? u / s.T : u, x = tile * ROWS + row;
-    const int tq = a.list ? u % s.T : x / s.G, g = a.list ? x : x % s.G;
-    *reinterpret_cast<uint2*>(a.O + (((int64_t)b * s.T + tq) * s.HQ + h * s.G + g) * D + 4 * lane) = *reinterpret_cast<uint2*>(y);
-}
-
 // ---- the alpha-entmax threshold ----------------------------------------------------
 // One CTA an item's eight rows, a warp a row in the end.  A row's support lies
 // within 1 of its largest x = (alpha - 1) score: of the tiles whose maxima reach that
@@ -1220,7 +1070,6 @@ __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_con
 template <int NT>
 constexpr int warps_of() { return NT == 1 ? 8 : 4; }
 constexpr int ctas_of(int nt) { return nt == 1 ? 2 : 3; }        // an SM holds
-constexpr int kSms = 148;
 
 int row_tiles(const Shape& s, bool lists) { return (lists ? s.G : s.T * s.G) > 8 ? 2 : 1; }
 
@@ -1236,6 +1085,8 @@ Plan make_plan(const Shape& s, int keep) {
     // CTA writes the output itself and nothing is joined.
     const int64_t items = (int64_t)p.U * p.tiles * s.H;
     p.split = p.cap > 32 && items < 8 * kSms * ctas_of(nt);
+    p.tile = kTile * kBlock;
+    p.item_cost = kItemCost;
     p.least = kItemCost + (nt == 1 ? 8 : 4);
     p.vec = 0;
     p.page_shift = 0;
@@ -1298,18 +1149,20 @@ cudaError_t attend_as(const Args& a, cudaStream_t st) {
         if (e == cudaSuccess) e = launch_walk<D, NT, kValues>(a, st);
     }
     if (e != cudaSuccess || !a.p.split) return e;
-    return launch(combine_kernel<D, NT>, (unsigned)(items * 8 * NT), 128, 0, st, a);
+    return launch(combine_kernel<D, 8 * NT>, (unsigned)(items * 8 * NT), 128, 0, st, a);
 }
 
 }  // namespace
 
 size_t attend_workspace(const Shape& s, int keep) {
+    if (chunk_takes(s, keep)) return chunk_workspace(s);
     return lay_out(s, make_plan(s, keep), nullptr, nullptr) + 16;
 }
 
 cudaError_t attend(const Shape& s, const void* Q, Strides qs, const uint8_t* pool, const int32_t* table,
                    const int32_t* lengths, const int32_t* list, int keep, void* O, void* ws, int* err,
                    cudaStream_t st) {
+    if (chunk_takes(s, keep)) return chunk_attend(s, Q, qs, pool, table, lengths, O, ws, err, st);
     Args a;
     a.s = s;
     a.p = make_plan(s, keep);
