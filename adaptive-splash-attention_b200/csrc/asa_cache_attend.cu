@@ -25,9 +25,10 @@
 // output to bf16 has 8); its products with the values' scales are taken as the
 // rounded product and the rest, two products of the codes, so that codes and
 // offsets are weighted by the same P and a value near zero, a difference of the
-// two, is not disturbed by more than its own size.  P is kept near 2^14, so
-// neither a small weight nor a small scale falls among fp16's subnormals; a running
-// exponent lowers it where scales above 2 would overflow.  Sums, maxima and
+// two, is not disturbed by more than its own size.  P is kept within 2^10 and
+// 2^14.5 at its largest, so that small weights and scales stay clear of fp16's
+// subnormals and a reference is seldom moved; a running exponent lowers it where
+// scales above 2 would overflow.  Sums, maxima and
 // accumulators are fp32.
 #include "asa_cache_attend.cuh"
 
@@ -441,7 +442,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                                                   : *reinterpret_cast<const float2*>(&mine_rows.factor[8 * nt + 2 * t]);
                 rf[nt][0] = f2.x;
                 rf[nt][1] = f2.y;
-                m[nt][0] = m[nt][1] = MODE == kSoftmax ? 0.0f : -kTop;
+                m[nt][0] = m[nt][1] = MODE == kSoftmax ? 0.0f : -14.0f;   // (entmax weights are at most 1)
                 room[nt][0] = room[nt][1] = -INFINITY;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) oz[nt][e] = 0.0f;
@@ -630,7 +631,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                                 }
                         }
                     }
-                    // weights near 2^14, below 2^(14.5 - lift) at most, scales below 2^(lift + 1),
+                    // weights below 2^(kMost - lift), scales below 2^(lift + 1),
                     // so that their products stay within fp16: rescale where a score or a scale
                     // has outgrown what they were fitted to
                     uint32_t sbig = hmax2(sp[0][0][0], sp[0][0][1]);
@@ -663,7 +664,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                                     const float to = top - kTop + (float)up;
                                     if (room[nt][e] > -INFINITY) by = fmaxf(by, to);
                                     else by = top > -INFINITY ? to : 0.0f;
-                                    if (room[nt][e] > -INFINITY || top > -INFINITY) room[nt][e] = kTop + 0.5f - (float)up;
+                                    if (room[nt][e] > -INFINITY || top > -INFINITY) room[nt][e] = kMost - (float)up;
 #pragma unroll
                                     for (int i = 0; i < kTile; ++i) v[i][nt][e] -= by, v[i][nt][e + 2] -= by;
                                 }

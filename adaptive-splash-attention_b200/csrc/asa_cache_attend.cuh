@@ -9,7 +9,10 @@ namespace cache {
 namespace {
 
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kTop = 14.0f;         // log2 of the weight that a row's largest score gets
+// Weights are powers of two of a score over its row's reference.  A reference is set
+// so that the row's largest weight is 2^kTop, and stays until one would pass
+// 2^kMost: fp16 holds 65504, and keeps 11 bits of weights down to 2^-14.
+constexpr float kTop = 10.0f, kMost = 14.5f;
 constexpr float kLow = -1.0e30f;      // below any score
 constexpr int kSms = 148;
 

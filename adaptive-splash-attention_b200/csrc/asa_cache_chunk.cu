@@ -14,13 +14,15 @@
 //
 // fp16 is chosen for all operands: a code times its scale plus its offset, both
 // fp16, rounds to 11 bits there (bf16 would keep 8), its subnormals hold the
-// smallest values exactly, and P, kept near 2^14, keeps 11 bits as well.  A row's
-// reference moves only when a score outgrows it by 2^14.5 over 2^14; O in tensor
-// memory is then rescaled by the rows' own warps.
+// smallest values exactly, and P keeps 11 bits as well.  A row's reference moves only
+// when a weight outgrows it (kTop, kMost); O in tensor memory is then rescaled by the
+// rows' own warps.
 //
 // Channels are not moved into their order: keys and queries share the order in
 // which masking words yields them, and the output's is undone as it is stored.
 #include "asa_cache_attend.cuh"
+
+#include <type_traits>
 
 namespace asa {
 namespace cache {
@@ -109,13 +111,11 @@ __device__ __forceinline__ void values_of(uint32_t w, uint32_t s, uint32_t z, ui
         out[i] = *reinterpret_cast<const uint32_t*>(&v);
     }
 }
-__device__ __forceinline__ bool any_infinite(uint32_t h) {
-    return (h & 0x7c00u) == 0x7c00u || (h & 0x7c000000u) == 0x7c000000u;
-}
-__device__ __forceinline__ void values_of(uint32_t w, uint32_t s, uint32_t z, uint32_t (&out)[4]) {
+// Whether some value 15 s + z passes fp16's largest (or is NaN already).
+__device__ __forceinline__ bool passes_largest(uint32_t s, uint32_t z) {
     const __half2 top = __hfma2(__float2half2_rn(15.0f), *reinterpret_cast<const __half2*>(&s), *reinterpret_cast<const __half2*>(&z));
-    if (any_infinite(*reinterpret_cast<const uint32_t*>(&top))) values_of<true>(w, s, z, out);
-    else values_of<false>(w, s, z, out);
+    const uint32_t h = *reinterpret_cast<const uint32_t*>(&top);
+    return (h & 0x7c00u) == 0x7c00u || (h & 0x7c000000u) == 0x7c000000u;
 }
 
 template <int D>
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     constexpr int NG = D / 32, NP = NG / 2, BB = block_bytes(D), RB = row_bytes(D), PB = par_bytes(D);
     constexpr uint32_t kO = 256;                      // tensor memory: scores (P over them) 2 x 128 columns, then O
     extern __shared__ uint8_t smem_raw[];
-    auto& sm = *reinterpret_cast<ChunkSmem<D>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+    auto& sm = *reinterpret_cast<ChunkSmem<D>*>(smem_raw + (-smem_u32(smem_raw) & 1023u));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const Shape& s = a.s;
     const int per = a.p.tiles * s.H;
@@ -354,7 +354,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 all_rows();                           // (also: sm.row may be written again)
                 arrive(sm.b.q_ready);
             }
-            float m = 0.0f, room = -INFINITY, l = 0.0f;   // as in asa_cache_attend.cu
+            float m = 0.0f, room = -INFINITY;         // as in asa_cache_attend.cu
+            float2 l2 = make_float2(0.0f, 0.0f);      // the weights' sum, in two parts
             uint32_t nan_groups = 0;
             for (int i = 0; i < v.n; ++i, ++j) {
                 const int b = j & 1;
@@ -367,10 +368,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 const bool whole = info.present == 0xff && info.base + kTokens - 1 <= v.pos_lo;
                 tmem_ld_wait();
                 float top = -INFINITY;
+                const float2 rf2 = make_float2(rf, rf), m2 = make_float2(-m, -m);
 #pragma unroll
                 for (int c = 0; c < 2; ++c)
 #pragma unroll
-                    for (int k = 0; k < 32; ++k) r[c][k] = __float_as_uint(fmaf(__uint_as_float(r[c][k]), rf, -m));
+                    for (int k = 0; k < 32; k += 2) {
+                        const float2 y = __ffma2_rn(make_float2(__uint_as_float(r[c][k]), __uint_as_float(r[c][k + 1])), rf2, m2);
+                        r[c][k] = __float_as_uint(y.x), r[c][k + 1] = __float_as_uint(y.y);
+                    }
                 if (!whole) {
                     const int see = pos - info.base - 64 * half;   // the last of this thread's keys that the row sees
 #pragma unroll
@@ -388,10 +393,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 top = fmaxf(top, sm.row[b][half ^ 1][row]);
                 if (__any_sync(~0u, top > room)) {    // (the same in both halves' warps)
                     float by = 0.0f;
-                    if (top > room) by = top - kTop, room = kTop + 0.5f;
+                    if (top > room) by = top - kTop, room = kMost;
                     m += by;
                     const float f = exp2_fast(-by);
-                    l *= f;
+                    l2.x *= f, l2.y *= f;
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
 #pragma unroll
@@ -419,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                         for (int k = 0; k < 8; ++k) {
                             const float y = exp2_fast(__uint_as_float(r[c][16 * e + 2 * k]));
                             const float z = exp2_fast(__uint_as_float(r[c][16 * e + 2 * k + 1]));
-                            l += y + z;
+                            l2 = __fadd2_rn(l2, make_float2(y, z));
                             const __half2 two = __floats2half2_rn(y, z);
                             p[k] = *reinterpret_cast<const uint32_t*>(&two);
                         }
@@ -442,6 +447,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             }
             wait(sm.b.o_done, segs);
             tc_fence_after();
+            float l = l2.x + l2.y;
             sm.row[0][half][row] = l;
             all_rows();
             l += sm.row[0][half ^ 1][row];
@@ -504,64 +510,93 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 const uint8_t* vb = kb + kBlocks * BB;
                 wait(sm.b.k_free[st], (j >> 1) ^ 1u);
                 // keys: a lane eight channels of every group, of tokens lane % 8 and 8 on
+                {
+                    const int tok = lane & 7, run = lane >> 3;
+                    uint32_t w[2][NG], sc[2][NP], zo[2][NP];
+                    bool clip = false;
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int tok = (lane & 7) + 8 * k, run = lane >> 3;
-                    uint8_t* to = sm.k[st] + (16 * dq + tok) * 128;
-                    uint32_t w[NG], sz[NG];           // sz: scales, then offsets, in halves
+                    for (int k = 0; k < 2; ++k) {
+                        const uint8_t *row = kb + (tok + 8 * k) * RB + run * 4 * NG, *par = kb + kBlock * RB + (tok + 8 * k) * PB;
 #pragma unroll
-                    for (int e = 0; e < NG; ++e) {
-                        w[e] = *reinterpret_cast<const uint32_t*>(kb + tok * RB + run * 4 * NG + 4 * e);
-                        sz[e] = *reinterpret_cast<const uint32_t*>(kb + kBlock * RB + tok * PB + 4 * e);
+                        for (int e = 0; e < NG; ++e) w[k][e] = reinterpret_cast<const uint32_t*>(row)[e];
+#pragma unroll
+                        for (int e = 0; e < NP; ++e) {
+                            sc[k][e] = reinterpret_cast<const uint32_t*>(par)[e];
+                            zo[k][e] = reinterpret_cast<const uint32_t*>(par)[NP + e];
+                            if (!there) sc[k][e] = zo[k][e] = 0u;
+                            clip |= passes_largest(sc[k][e], zo[k][e]);
+                        }
                     }
+                    auto store = [&](auto clip_c) {
 #pragma unroll
-                    for (int e = 0; e < NG; ++e) {
-                        const uint32_t pick = e & 1 ? 0x3232u : 0x1010u;
-                        uint32_t y[4] = {0u, 0u, 0u, 0u};
-                        if (there) values_of(w[e], __byte_perm(sz[e >> 1], 0u, pick), __byte_perm(sz[NP + (e >> 1)], 0u, pick), y);
-                        const int c = NG * run + e;
-                        *reinterpret_cast<uint4*>(to + (c >> 3) * kBox + (((c & 7) ^ (tok & 7)) << 4)) = make_uint4(y[0], y[1], y[2], y[3]);
-                    }
+                        for (int k = 0; k < 2; ++k)
+#pragma unroll
+                            for (int e = 0; e < NG; ++e) {
+                                const uint32_t pick = e & 1 ? 0x3232u : 0x1010u;
+                                uint32_t y[4];
+                                values_of<decltype(clip_c)::value>(w[k][e], __byte_perm(sc[k][e >> 1], 0u, pick), __byte_perm(zo[k][e >> 1], 0u, pick), y);
+                                const int c = NG * run + e;
+                                *reinterpret_cast<uint4*>(sm.k[st] + (c >> 3) * kBox + (16 * dq + tok + 8 * k) * 128 + (((c & 7) ^ tok) << 4)) =
+                                    make_uint4(y[0], y[1], y[2], y[3]);
+                            }
+                    };
+                    if (__any_sync(~0u, clip)) store(std::true_type{}); else store(std::false_type{});
                 }
                 fence_async_smem();
                 arrive(sm.b.k_ready[st]);
                 wait(sm.b.v_free[st], (j >> 1) ^ 1u);
                 // values: a lane four channels of every group, of two tokens and two runs
                 const bool whole = info.present == 0xff && info.base + kTokens - 1 <= v.pos_lo;
+                {
+                    const int tok = lane & 7;
+                    uint32_t w[2][2][NP], sc[2][NP], zo[2][NP];
+                    bool clip = false;
 #pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const int tok = (lane & 7) + 8 * k;
-                    const bool seen = there && info.base + 16 * dq + tok <= v.pos_hi;
-                    uint32_t sc[NP], zo[NP];
+                    for (int k = 0; k < 2; ++k) {
+                        const uint8_t *row = vb + (tok + 8 * k) * RB, *par = vb + kBlock * RB + (tok + 8 * k) * PB;
 #pragma unroll
-                    for (int e = 0; e < NP; ++e) {
-                        sc[e] = *reinterpret_cast<const uint32_t*>(vb + kBlock * RB + tok * PB + 4 * e);
-                        zo[e] = *reinterpret_cast<const uint32_t*>(vb + kBlock * RB + tok * PB + 4 * (NP + e));
+                        for (int e = 0; e < NP; ++e) {
+                            w[k][0][e] = reinterpret_cast<const uint32_t*>(row + (lane >> 3) * 2 * NG)[e];
+                            w[k][1][e] = reinterpret_cast<const uint32_t*>(row + ((lane >> 3) + 4) * 2 * NG)[e];
+                            sc[k][e] = reinterpret_cast<const uint32_t*>(par)[e];
+                            zo[k][e] = reinterpret_cast<const uint32_t*>(par)[NP + e];
+                        }
                     }
                     if (!whole) {
                         // what no row sees may be anything, and becomes zero; so does a NaN that some
                         // rows see, and they are told
 #pragma unroll
-                        for (int e = 0; e < NG; ++e) {
-                            const uint32_t half = 0xffffu << (16 * (e & 1)), inf = 0x7c00u << (16 * (e & 1));
-                            const bool bad = (sc[e >> 1] & inf) == inf || (zo[e >> 1] & inf) == inf;
-                            const uint32_t votes = __ballot_sync(~0u, seen && bad) & 255u;
-                            if (lane == 0) reinterpret_cast<uint8_t*>(&sm.nan[st][e][dq])[k] = (uint8_t)votes;
-                            if (!seen || bad) sc[e >> 1] &= ~half, zo[e >> 1] &= ~half;
+                        for (int k = 0; k < 2; ++k) {
+                            const bool seen = there && info.base + 16 * dq + tok + 8 * k <= v.pos_hi;
+#pragma unroll
+                            for (int e = 0; e < NG; ++e) {
+                                const uint32_t half = 0xffffu << (16 * (e & 1)), inf = 0x7c00u << (16 * (e & 1));
+                                const bool bad = (sc[k][e >> 1] & inf) == inf || (zo[k][e >> 1] & inf) == inf;
+                                const uint32_t votes = __ballot_sync(~0u, seen && bad) & 255u;
+                                if (lane == 0) reinterpret_cast<uint8_t*>(&sm.nan[st][e][dq])[k] = (uint8_t)votes;
+                                if (!seen || bad) sc[k][e >> 1] &= ~half, zo[k][e >> 1] &= ~half;
+                            }
                         }
                     }
 #pragma unroll
-                    for (int q = 0; q < 2; ++q) {
-                        const int run = (lane >> 3) + 4 * q;
+                    for (int k = 0; k < 2; ++k)
 #pragma unroll
-                        for (int e = 0; e < NP; ++e) {
-                            uint32_t y[4];
-                            values_of(*reinterpret_cast<const uint32_t*>(vb + tok * RB + run * 2 * NG + 4 * e), sc[e], zo[e], y);
-                            const int c = NP * run + e;
-                            *reinterpret_cast<uint4*>(sm.v[st] + (c >> 3) * kBox + (16 * dq + tok) * 128 + (((c & 7) ^ (tok & 7)) << 4)) =
-                                make_uint4(y[0], y[1], y[2], y[3]);
-                        }
-                    }
+                        for (int e = 0; e < NP; ++e) clip |= passes_largest(sc[k][e], zo[k][e]);
+                    auto store = [&](auto clip_c) {
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+#pragma unroll
+                            for (int q = 0; q < 2; ++q)
+#pragma unroll
+                                for (int e = 0; e < NP; ++e) {
+                                    uint32_t y[4];
+                                    values_of<decltype(clip_c)::value>(w[k][q][e], sc[k][e], zo[k][e], y);
+                                    const int c = NP * ((lane >> 3) + 4 * q) + e;
+                                    *reinterpret_cast<uint4*>(sm.v[st] + (c >> 3) * kBox + (16 * dq + tok + 8 * k) * 128 + (((c & 7) ^ tok) << 4)) =
+                                        make_uint4(y[0], y[1], y[2], y[3]);
+                                }
+                    };
+                    if (__any_sync(~0u, clip)) store(std::true_type{}); else store(std::false_type{});
                 }
                 fence_async_smem();
                 arrive(sm.b.v_ready[st]);
