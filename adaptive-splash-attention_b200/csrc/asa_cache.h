@@ -32,7 +32,7 @@ struct Shape {
     int pages, width;                // the pool's pages; entries of a block table row
     int dtype;
     float scale, alpha;
-    long long spins;
+    int naps;                        // bound on device-side waits, in naps of 20 us at most
     int64_t rec;                     // bytes of one page's record of one key head
 };
 

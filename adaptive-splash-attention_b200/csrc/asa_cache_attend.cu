@@ -25,10 +25,10 @@
 // output to bf16 has 8); its products with the values' scales are taken as the
 // rounded product and the rest, two products of the codes, so that codes and
 // offsets are weighted by the same P and a value near zero, a difference of the
-// two, is not disturbed by more than its own size.  P is kept within 2^10 and
-// 2^14.5 at its largest, so that small weights and scales stay clear of fp16's
-// subnormals and a reference is seldom moved; a running exponent lowers it where
-// scales above 2 would overflow.  Sums, maxima and
+// two, is not disturbed by more than its own size.  A row's largest P times
+// the scales starts near 2^4 and may grow to 2^14.5 before its reference is moved: a
+// running exponent fits P to the scales, so that small ones stay clear of fp16's
+// subnormals and large ones do not overflow.  Sums, maxima and
 // accumulators are fp32.
 #include "asa_cache_attend.cuh"
 
@@ -38,6 +38,7 @@ namespace {
 
 constexpr int kTile = 2;              // blocks of a tile
 constexpr int kStages = 2;            // tiles a warp has in flight
+constexpr int kLeast = -8;            // weights are raised for small scales by 2^8 at most
 constexpr int kItemCost = 8;          // Plan::item_cost
 constexpr int kSegments = 32;         // segments a CTA lines up at a time
 
@@ -428,8 +429,10 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
             float rf[NT][2];                          // scores: the factor of rows 2t, 2t + 1; values: their thresholds
             float m[NT][2], room[NT][2];              // references, and how far above them a score may lie (-inf: unset)
             float oz[NT][4], o[NT][2 * NG][4];        // oz: by group the offsets' sums, and the weights'
-            int lift = 0;                             // log2 by which weights are lowered for large scales
-            uint32_t s_most = 0x4000u;                // the fp16 scale 2^(lift + 1) that they allow
+            // log2 by which weights are lowered for large scales (raised for small ones), and the
+            // fp16 scale 2^(lift + 1) that this allows
+            int lift = MODE == kSoftmax ? kLeast : 0;
+            uint32_t s_most = (uint32_t)(lift + 16) << 10;
             const float* tau = a.w.tau + item_no * ROWS;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
@@ -456,9 +459,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
             while (in_flight) {
                 const Info info = sm.info[warp][stage_out];
                 if (info.seg != sg) break;
-                if (!sm100::mbar_try(&sm.full[warp][stage_out], parity) &&
-                    !wait_full(&sm.full[warp][stage_out], parity, s.spins, a.err))
-                    lost = true;
+                if (!wait_full(&sm.full[warp][stage_out], parity, s.naps, a.err)) lost = true;
                 __syncwarp();
                 const uint8_t* const st = ring + stage_out * kStage;
                 // every row sees all of both blocks
@@ -631,7 +632,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                                 }
                         }
                     }
-                    // weights below 2^(kMost - lift), scales below 2^(lift + 1),
+                    // weights below 2^(kMost - max(lift, 0)), scales below 2^(lift + 1),
                     // so that their products stay within fp16: rescale where a score or a scale
                     // has outgrown what they were fitted to
                     uint32_t sbig = hmax2(sp[0][0][0], sp[0][0][1]);
@@ -664,7 +665,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                                     const float to = top - kTop + (float)up;
                                     if (room[nt][e] > -INFINITY) by = fmaxf(by, to);
                                     else by = top > -INFINITY ? to : 0.0f;
-                                    if (room[nt][e] > -INFINITY || top > -INFINITY) room[nt][e] = kMost - (float)up;
+                                    if (room[nt][e] > -INFINITY || top > -INFINITY) room[nt][e] = kMost - (float)max(up, 0);
 #pragma unroll
                                     for (int i = 0; i < kTile; ++i) v[i][nt][e] -= by, v[i][nt][e + 2] -= by;
                                 }

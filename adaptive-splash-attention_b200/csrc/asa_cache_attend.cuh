@@ -12,7 +12,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // Weights are powers of two of a score over its row's reference.  A reference is set
 // so that the row's largest weight is 2^kTop, and stays until one would pass
 // 2^kMost: fp16 holds 65504, and keeps 11 bits of weights down to 2^-14.
-constexpr float kTop = 10.0f, kMost = 14.5f;
+constexpr float kTop = 4.0f, kMost = 14.5f;
 constexpr float kLow = -1.0e30f;      // below any score
 constexpr int kSms = 148;
 
@@ -64,13 +64,22 @@ __device__ __forceinline__ void bulk_load(void* dst, const void* src, uint32_t b
     asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
                  ::"r"(sm100::smem_u32(dst)), "l"(src), "r"(bytes), "r"(sm100::smem_u32(bar)) : "memory");
 }
-// Bounded wait for a block's copy.  An error word set by something else than a
-// wait that gave up (a page outside the pool) does not cut it short.
-__device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity, long long spins, int* err) {
-    if (sm100::mbar_try(bar, parity)) return true;
-    for (long long i = 0; i < spins; ++i) {
-        if (sm100::mbar_try(bar, parity)) return true;
-        if ((i & 1023) == 1023 && err && *reinterpret_cast<volatile int*>(err) == ASA_ERR_DEVICE_TIMEOUT) return false;
+// Bounded wait for a phase, in naps of up to 20 us: a warp that waits takes few issue
+// slots from those that work.  An error word set by something else than a wait that
+// gave up (a page outside the pool) does not cut it short.
+__device__ __forceinline__ bool nap(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n\t.reg .pred p;\n\t"
+                 "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+                 "selp.u32 %0, 1, 0, p;\n\t}"
+                 : "=r"(ok) : "r"(sm100::smem_u32(bar)), "r"(parity), "r"(20000u) : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity, int naps, int* err) {
+    if (nap(bar, parity)) return true;
+    for (int i = naps; i > 0; --i) {
+        if (nap(bar, parity)) return true;
+        if (err && *reinterpret_cast<volatile int*>(err) == ASA_ERR_DEVICE_TIMEOUT) return false;
     }
     if (err) atomicExch(err, ASA_ERR_DEVICE_TIMEOUT);
     return false;

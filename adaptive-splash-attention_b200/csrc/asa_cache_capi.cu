@@ -45,7 +45,9 @@ int check(const asa_cache_params* p, Shape* s, bool queries) {
     s->dtype = p->dtype;
     s->scale = p->sm_scale;
     s->alpha = p->alpha;
-    s->spins = p->timeout_spins > 0 ? p->timeout_spins : (1LL << 22);
+    // the training kernels' spins, sixteen to a nap (five seconds by default)
+    const long long spins = p->timeout_spins > 0 ? p->timeout_spins : (1LL << 22);
+    s->naps = (int)((spins >> 4) + 1 < (1 << 30) ? (spins >> 4) + 1 : (1 << 30));
     s->rec = asa::cache::record_bytes(p->d, p->page_size);
     return ASA_OK;
 }

@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
 
-    auto wait = [&](uint64_t& bar, uint32_t parity) { wait_full(&bar, parity & 1u, s.spins, a.err); };
+    auto wait = [&](uint64_t& bar, uint32_t parity) { wait_full(&bar, parity & 1u, s.naps, a.err); };
     auto position = [&](int u, int row) -> int {      // of an item's row (its tile's first row added)
         if (row >= a.p.R) return -1;
         return (int)max(-1ll, min((long long)__ldg(a.lengths + u) - s.T + row / s.G, (long long)s.width * s.P - 1));
@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 top = fmaxf(top, sm.row[b][half ^ 1][row]);
                 if (__any_sync(~0u, top > room)) {    // (the same in both halves' warps)
                     float by = 0.0f;
-                    if (top > room) by = top - kTop, room = kMost;
+                    if (top > room) by = top, room = kMost;   // the largest weight 1: fp16 has room below too
                     m += by;
                     const float f = exp2_fast(-by);
                     l2.x *= f, l2.y *= f;
@@ -499,6 +499,21 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     } else {
         // ---- codes to fp16: 16 tokens of each tile a warp ----------------------------------
         const int dq = warp < 4 ? warp - 2 : warp - 10;
+        // where a lane's pieces of a key row and of a value row go (token lane % 8 of the warp's 16)
+        const int tok = lane & 7, run = lane >> 3;
+        uint32_t to_k[NG], to_v[2][NP];
+#pragma unroll
+        for (int e = 0; e < NG; ++e) {
+            const int c = NG * run + e;
+            to_k[e] = (c >> 3) * kBox + (16 * dq + tok) * 128 + (((c & 7) ^ tok) << 4);
+        }
+#pragma unroll
+        for (int q = 0; q < 2; ++q)
+#pragma unroll
+            for (int e = 0; e < NP; ++e) {
+                const int c = NP * (run + 4 * q) + e;
+                to_v[q][e] = (c >> 3) * kBox + (16 * dq + tok) * 128 + (((c & 7) ^ tok) << 4);
+            }
         while (next_segment(a, sm.pref, x, x1, g)) {
             const View v = view_of(g);
             for (int i = 0; i < v.n; ++i, ++j) {
@@ -511,7 +526,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 wait(sm.b.k_free[st], (j >> 1) ^ 1u);
                 // keys: a lane eight channels of every group, of tokens lane % 8 and 8 on
                 {
-                    const int tok = lane & 7, run = lane >> 3;
                     uint32_t w[2][NG], sc[2][NP], zo[2][NP];
                     bool clip = false;
 #pragma unroll
@@ -535,9 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                                 const uint32_t pick = e & 1 ? 0x3232u : 0x1010u;
                                 uint32_t y[4];
                                 values_of<decltype(clip_c)::value>(w[k][e], __byte_perm(sc[k][e >> 1], 0u, pick), __byte_perm(zo[k][e >> 1], 0u, pick), y);
-                                const int c = NG * run + e;
-                                *reinterpret_cast<uint4*>(sm.k[st] + (c >> 3) * kBox + (16 * dq + tok + 8 * k) * 128 + (((c & 7) ^ tok) << 4)) =
-                                    make_uint4(y[0], y[1], y[2], y[3]);
+                                *reinterpret_cast<uint4*>(sm.k[st] + to_k[e] + 8 * k * 128) = make_uint4(y[0], y[1], y[2], y[3]);
                             }
                     };
                     if (__any_sync(~0u, clip)) store(std::true_type{}); else store(std::false_type{});
@@ -548,7 +560,6 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 // values: a lane four channels of every group, of two tokens and two runs
                 const bool whole = info.present == 0xff && info.base + kTokens - 1 <= v.pos_lo;
                 {
-                    const int tok = lane & 7;
                     uint32_t w[2][2][NP], sc[2][NP], zo[2][NP];
                     bool clip = false;
 #pragma unroll
@@ -556,8 +567,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                         const uint8_t *row = vb + (tok + 8 * k) * RB, *par = vb + kBlock * RB + (tok + 8 * k) * PB;
 #pragma unroll
                         for (int e = 0; e < NP; ++e) {
-                            w[k][0][e] = reinterpret_cast<const uint32_t*>(row + (lane >> 3) * 2 * NG)[e];
-                            w[k][1][e] = reinterpret_cast<const uint32_t*>(row + ((lane >> 3) + 4) * 2 * NG)[e];
+                            w[k][0][e] = reinterpret_cast<const uint32_t*>(row + run * 2 * NG)[e];
+                            w[k][1][e] = reinterpret_cast<const uint32_t*>(row + (run + 4) * 2 * NG)[e];
                             sc[k][e] = reinterpret_cast<const uint32_t*>(par)[e];
                             zo[k][e] = reinterpret_cast<const uint32_t*>(par)[NP + e];
                         }
@@ -591,9 +602,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                                 for (int e = 0; e < NP; ++e) {
                                     uint32_t y[4];
                                     values_of<decltype(clip_c)::value>(w[k][q][e], sc[k][e], zo[k][e], y);
-                                    const int c = NP * ((lane >> 3) + 4 * q) + e;
-                                    *reinterpret_cast<uint4*>(sm.v[st] + (c >> 3) * kBox + (16 * dq + tok + 8 * k) * 128 + (((c & 7) ^ tok) << 4)) =
-                                        make_uint4(y[0], y[1], y[2], y[3]);
+                                    *reinterpret_cast<uint4*>(sm.v[st] + to_v[q][e] + 8 * k * 128) = make_uint4(y[0], y[1], y[2], y[3]);
                                 }
                     };
                     if (__any_sync(~0u, clip)) store(std::true_type{}); else store(std::false_type{});
