@@ -59,6 +59,17 @@ __device__ __forceinline__ void mma0(float (&c)[4], uint32_t a0, uint32_t a1, ui
                  : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
 }
+// Larger and smaller that keep a NaN.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float c;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+    return c;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float c;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(c) : "f"(a), "f"(b));
+    return c;
+}
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -412,7 +423,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                 }
                 const float hi = __half2float(__float2half_rn(own));
                 out.q[nt][4 * NG][lane] = pack(hi, own - hi);
-                if (t == 0) out.factor[8 * nt + r] = scalbnf(s.scale * (MODE == kSoftmax ? kLog2e : 1.0f), 24 - up);
+                if (t == 0) out.factor[8 * nt + r] = scalbnf(s.scale * (MODE == kSoftmax ? kLog2e : s.alpha - 1.0f), 24 - up);
             }
         };
         if (warp < NT && segs) make_rows(0, warp);
@@ -527,29 +538,27 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                     }
                 }
                 if constexpr (MODE == kScores) {
-                    const float am1 = s.alpha - 1.0f;
+                    const float most = 10.0f * (s.alpha - 1.0f);   // x = (alpha - 1) score, clamped as in training
                     const int64_t place = item_no * a.p.cap + info.tile;
                     each([&](int i, int nt, int e) {
-                        const float y = v[i][nt][e] * rf[nt][e & 1];
-                        v[i][nt][e] = y != y ? y : am1 * fminf(fmaxf(y, -10.0f), 10.0f);
+                        v[i][nt][e] = min_nan(max_nan(v[i][nt][e] * rf[nt][e & 1], -most), most);
                     });
                     if (!whole) mask();
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt) {
-                        float top[2] = {-INFINITY, -INFINITY};
+                        float top[2] = {-INFINITY, -INFINITY};     // a NaN score: its row is NaN
 #pragma unroll
                         for (int i = 0; i < kTile; ++i) {
 #pragma unroll
-                            for (int e = 0; e < 4; ++e)   // a NaN score: its row is NaN
-                                top[e & 1] = fmaxf(top[e & 1], v[i][nt][e] != v[i][nt][e] ? INFINITY : v[i][nt][e]);
+                            for (int e = 0; e < 4; ++e) top[e & 1] = max_nan(top[e & 1], v[i][nt][e]);
                             if (8 * nt + 2 * t < rows)
                                 a.w.score[((place * kTile + i) * NT + nt) * 32 + 8 * t + r] =
                                     make_float4(v[i][nt][0], v[i][nt][1], v[i][nt][2], v[i][nt][3]);
                         }
 #pragma unroll
                         for (int k = 4; k < 32; k <<= 1) {
-                            top[0] = fmaxf(top[0], __shfl_xor_sync(~0u, top[0], k));
-                            top[1] = fmaxf(top[1], __shfl_xor_sync(~0u, top[1], k));
+                            top[0] = max_nan(top[0], __shfl_xor_sync(~0u, top[0], k));
+                            top[1] = max_nan(top[1], __shfl_xor_sync(~0u, top[1], k));
                         }
                         // rows past the last take no part
                         if (8 * nt + 2 * t >= rows) top[0] = -INFINITY;
@@ -874,18 +883,18 @@ __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_con
         float y[8];
         tops_of(j, y);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top[i] = fmaxf(top[i], y[i]);
+        for (int i = 0; i < 8; ++i) top[i] = max_nan(top[i], y[i]);
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
 #pragma unroll
-        for (int k = 16; k; k >>= 1) top[i] = fmaxf(top[i], __shfl_xor_sync(~0u, top[i], k));
+        for (int k = 16; k; k >>= 1) top[i] = max_nan(top[i], __shfl_xor_sync(~0u, top[i], k));
         if (lane == 0) s_max[warp][i] = top[i];
     }
     __syncthreads();
     if (tid < 8) {
         float y = s_max[0][tid];
-        for (int w = 1; w < W; ++w) y = fmaxf(y, s_max[w][tid]);
+        for (int w = 1; w < W; ++w) y = max_nan(y, s_max[w][tid]);
         s_top[tid] = y;
     }
     __syncthreads();
@@ -1064,7 +1073,7 @@ __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_con
     __syncthreads();
     if (tid < 8) {
         const float y = s_top[tid];
-        tau_out[tid] = y == -INFINITY ? INFINITY : y == INFINITY ? NAN : y + s_tau[tid];
+        tau_out[tid] = y == -INFINITY ? INFINITY : y + s_tau[tid];   // (NaN where a score is)
     }
 }
 

@@ -20,7 +20,7 @@ namespace {
 
 constexpr int kThreads = 512, kWarps = kThreads / 32;
 constexpr int kShared = 4096;         // pages whose keys fit in shared memory
-constexpr int kChunk = 512;           // pages a CTA of score_kernel scores
+constexpr int kChunk = 256;           // pages a CTA of score_kernel scores
 
 // Larger floats as larger integers; NaN lowest, -0 as 0.
 __device__ __forceinline__ uint32_t ordered(float f) {
@@ -142,7 +142,7 @@ __device__ __forceinline__ void score_pages(const Query& a, int b, int h, int fr
     }
 }
 
-// Keys of an item's pages, kChunk a CTA, for items whose keys do not fit in shared memory.
+// Keys of an item's pages, kChunk a CTA.
 template <int D>
 __global__ void __launch_bounds__(256) score_kernel(const __grid_constant__ Query a, uint32_t* __restrict__ keys, int chunks) {
     follow();
@@ -170,9 +170,8 @@ __device__ __forceinline__ int cta_sum(int v, int* slot, int* before = nullptr) 
     return __reduce_add_sync(~0u, of);
 }
 
-// One CTA a (query, key head): its keys (scored here, where they fit in shared
-// memory), the edge between taken and left, and the taken pages in ascending order.
-template <int D, bool SHARED>
+// One CTA a (query, key head): its keys (scored here, or read back), the edge between taken and left, and the taken pages in ascending order.
+template <int D, bool SCORE>
 __global__ void __launch_bounds__(kThreads) pick_kernel(const __grid_constant__ Query a, const uint32_t* __restrict__ keys,
                                                         int32_t* __restrict__ pages) {
     extern __shared__ __align__(16) int8_t s_q[];    // the query, its units, the keys
@@ -190,14 +189,18 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const __grid_constant__ 
         return;
     }
     const int m = n - 1;                              // those that are weighed; the query's own is taken
-    if constexpr (SHARED) {
+    const uint32_t* key = keys + (int64_t)blockIdx.x * s.width;
+    if constexpr (SCORE) {
         make_query<D>(a, b, t, h, s_q, s_unit);
         __syncthreads();
         score_pages<D>(a, b, h, 0, m, kWarps, s_q, s_unit,
                        [&](int page, uint32_t k, bool more) { s_key[page] = more ? max(s_key[page], k) : k; });
-        __syncthreads();
+    } else if (m <= kShared) {
+        s_key = reinterpret_cast<uint32_t*>(s_q);
+        for (int i = tid; i < m; i += kThreads) s_key[i] = __ldg(key + i);
     }
-    const uint32_t* key = SHARED ? s_key : keys + (int64_t)blockIdx.x * s.width;
+    if (SCORE || m <= kShared) key = s_key;
+    __syncthreads();
     // the largest number that `need` keys reach
     const int need = keep - 1;
     uint32_t edge = 0;
@@ -245,11 +248,17 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const __grid_constant__ 
     if (tid == 0) out[keep - 1] = m;
 }
 
+// One launch where the tables are short, or the items fill the SMs; else the pages are
+// scored by CTAs of their own first.
+bool scores_itself(const Shape& s) {
+    return s.width <= 512 || (s.width <= kShared && (int64_t)s.B * s.T * s.H >= 296);
+}
+
 template <int D>
 cudaError_t select_as(const Query& a, int32_t* pages, void* ws, cudaStream_t st) {
     const unsigned items = (unsigned)(a.s.B * a.s.T * a.s.H);
     const size_t query = (size_t)((a.s.G + 7) & ~7) * (2 * D + 4) /* 67 KB at most */, keys = (size_t)a.s.width * 4;
-    if (a.s.width <= kShared) {
+    if (scores_itself(a.s)) {
         if (query + keys > 48 * 1024) {
             const cudaError_t e = cudaFuncSetAttribute(pick_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 116 * 1024);
             if (e != cudaSuccess) return e;
@@ -263,13 +272,14 @@ cudaError_t select_as(const Query& a, int32_t* pages, void* ws, cudaStream_t st)
         if (e != cudaSuccess) return e;
     }
     const cudaError_t e = launch(score_kernel<D>, items * chunks, 256, query, st, a, (uint32_t*)ws, chunks);
-    return e != cudaSuccess ? e : launch(pick_kernel<D, false>, items, kThreads, 0, st, a, (const uint32_t*)ws, pages);
+    return e != cudaSuccess ? e : launch(pick_kernel<D, false>, items, kThreads, keys < kShared * 4 ? keys : kShared * 4, st, a,
+                                         (const uint32_t*)ws, pages);
 }
 
 }  // namespace
 
 size_t select_workspace(const Shape& s) {
-    const size_t keys = s.width <= kShared ? 0 : (size_t)s.B * s.T * s.H * s.width * 4;
+    const size_t keys = scores_itself(s) ? 0 : (size_t)s.B * s.T * s.H * s.width * 4;
     return (keys + 16 + 15) & ~size_t(15);
 }
 
