@@ -523,3 +523,193 @@ def test_refusals(cuda):
         m.cache_read(cache, tab, dev([0]), 3, dtype=torch.float16)
     with pytest.raises(ValueError):
         m.cache_read(cache, tab, dev([0]), -1)
+
+
+# ---- the paths that sizes choose ---------------------------------------------------
+@pytest.mark.parametrize("alpha", [1.0, 1.5])
+@pytest.mark.parametrize("T", [1, 3, 40])
+@pytest.mark.parametrize("P", [16, 32, 64, 128])
+@pytest.mark.parametrize("d", [32, 64, 96, 128])
+def test_every_head_dim_and_page_size(cuda, d, P, T, alpha):
+    lengths = [T + 171, T]
+    cache, table, seqs = filled(2, lengths, 2, d, P, seed=d + P + T, k_scale=1.5)
+    q = torch.randn(2, T, 6, d, generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+    o = sa().cache_attention(q, cache, dev(table), dev(lengths), alpha=alpha)
+    check_attention(o, q, seqs, lengths, P, alpha, d ** -0.5)
+
+
+@pytest.mark.parametrize("alpha", [1.0, 1.5])
+@pytest.mark.parametrize("T,HQ", [(1, 4), (2, 8)])
+def test_many_sequences(cuda, T, HQ, alpha):
+    """More sequences than a block of threads, their work cut into equal runs."""
+    B, H, d, P = 330, 2, 32, 16
+    g = np.random.RandomState(3)
+    lengths = [int(x) for x in g.randint(0, 60, B)]
+    lengths[7], lengths[300], lengths[329] = 1500, 900, 1100
+    cache, table, seqs = filled(B, lengths, H, d, P, seed=1)
+    q = torch.randn(B, T, HQ, d, generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+    o = sa().cache_attention(q, cache, dev(table), dev(lengths), alpha=alpha)
+    check_attention(o, q, seqs, lengths, P, alpha, d ** -0.5)
+
+
+@pytest.mark.parametrize("alpha,q_scale", [(1.5, 1e-3), (1.25, 0.1), (1.05, 1.0), (3.0, 1e-3)])
+def test_wide_support(cuda, alpha, q_scale):
+    """More support than a row's list holds."""
+    lengths = [3000]
+    cache, table, seqs = filled(1, lengths, 1, 64, 64, seed=6)
+    q = (torch.randn(1, 1, 3, 64, generator=torch.Generator().manual_seed(5)) * q_scale).bfloat16().cuda()
+    o = sa().cache_attention(q, cache, dev(table), dev(lengths), alpha=alpha)
+    check_attention(o, q, seqs, lengths, 64, alpha, 64 ** -0.5)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("T,HQ,H,P,lengths", [
+    (64, 1, 1, 64, [64, 200]),
+    (40, 4, 2, 16, [1000, 25]),              # the second sequence's first queries see nothing
+    (257, 3, 1, 128, [700, 257]),
+    (130, 2, 2, 32, [130, 0]),
+    (9, 64, 2, 64, [5000, 9]),
+])
+def test_chunks(cuda, d, T, HQ, H, P, lengths):
+    cache, table, seqs = filled(2, lengths, H, d, P, seed=T, k_scale=1.2)
+    wide = torch.randn(2, HQ, T, d + 8, generator=torch.Generator().manual_seed(8)).bfloat16().cuda()
+    for q in (wide[..., :d].permute(0, 2, 1, 3).contiguous(), wide.permute(0, 2, 1, 3)[..., 4: 4 + d]):
+        o = sa().cache_attention(q, cache, dev(table), dev(lengths))
+        check_attention(o, q, seqs, lengths, P, 1.0, d ** -0.5)
+    assert torch.equal(sa().cache_attention(q, cache, dev(table), dev(lengths)), o)
+    assert sa().device_error() == 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_chunk_nan_in_places_nobody_sees(cuda, d):
+    T, HQ, H, P = 96, 2, 1, 64
+    lengths = [300]
+    cache, table, seqs = filled(1, lengths, H, d, P, seed=4, fill=255)
+    bad = torch.zeros(1, 1, H, d, device="cuda").bfloat16()
+    bad[..., 5] = float("nan")
+    zeros = torch.zeros_like(bad)
+    sa().cache_write(zeros, bad, cache, dev(table), dev([290]))        # query 86 stands there
+    q = torch.randn(1, T, HQ, d, generator=torch.Generator().manual_seed(6)).bfloat16().cuda()
+    q[0, 3, 1, 7] = float("nan")
+    o = sa().cache_attention(q, cache, dev(table), dev(lengths))
+    assert torch.isnan(o[0, 3, 1]).all()
+    o, clean = o.clone(), q.clone()
+    o[0, 3, 1], clean[0, 3, 1] = o[0, 3, 0], q[0, 3, 0]
+    check_attention(o[:, :86], clean[:, :86], seqs, [290], P, 1.0, d ** -0.5)
+    assert torch.isnan(o[0, 86:, :, :32]).all() and torch.isfinite(o[0, 86:, :, 32:]).all()
+    sa().cache_write(bad, zeros, cache, dev(table), dev([290]))        # a NaN key: its rows' scores
+    o = sa().cache_attention(clean, cache, dev(table), dev(lengths))
+    check_attention(o[:, :86], clean[:, :86], seqs, [290], P, 1.0, d ** -0.5)
+    assert torch.isnan(o[0, 86:]).all()
+
+
+@pytest.mark.parametrize("v_scale,v_shift,k_scale,q_scale,sm_scale", [
+    (1e-6, 0.0, 1.0, 1.0, None), (3000.0, 0.0, 1.0, 1.0, None), (1.0, 500.0, 1.0, 1.0, None),
+    (1.0, 0.0, 3.0, 40.0, None), (1.0, 0.0, 1.0, 1e-20, 1e20), (1.0, 0.0, 1.0, 1.0, -0.1), (1.0, 0.0, 1.0, 1.0, 0.0),
+])
+def test_chunk_magnitudes(cuda, v_scale, v_shift, k_scale, q_scale, sm_scale):
+    lengths = [401]
+    cache, table, seqs = filled(1, lengths, 1, 128, 64, seed=3, k_scale=k_scale, v_scale=v_scale, v_shift=v_shift)
+    q = (torch.randn(1, 70, 1, 128, generator=torch.Generator().manual_seed(5)) * q_scale).bfloat16().cuda()
+    o = sa().cache_attention(q, cache, dev(table), dev(lengths), sm_scale=sm_scale)
+    check_attention(o, q, seqs, lengths, 64, 1.0, 128 ** -0.5 if sm_scale is None else sm_scale)
+
+
+def test_values_at_the_top_of_the_range(cuda):
+    """A group over all of fp16's range: its largest value rounds past fp16."""
+    P, d, n = 64, 64, 128
+    V = torch.linspace(-65504, 65504, d).repeat(1, n, 1, 1).cuda()
+    K = torch.randn(1, n, 1, d, generator=torch.Generator().manual_seed(1)).cuda()
+    cache, table = fresh(1, [n], 1, d, P)
+    sa().cache_write(K, V, cache, dev(table), dev([0]))
+    _, v = F.decode(cache.pool.cpu().numpy(), d, P)
+    v = v[table[0, 0], 0, 0]
+    for T in (1, 80):
+        q = torch.randn(1, T, 1, d, generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+        o = num(sa().cache_attention(q, cache, dev(table), dev([n])))
+        # every value is the same token's: the output is it, within fp16's and bf16's roundings
+        assert np.isfinite(o).all() and (np.abs(o - v) <= 2.0 ** -7 * np.abs(v) + 1e-3).all()
+
+
+def test_chunk_unreadable_pages(cuda):
+    lengths = [200]
+    cache, table, seqs = filled(1, lengths, 1, 64, 16, seed=2)
+    bad = table.copy()
+    bad[0, 1], bad[0, 4], bad[0, 12] = cache.pool.shape[0] + 5, -3, 1 << 30
+    q = torch.randn(1, 64, 1, 64, generator=torch.Generator().manual_seed(8)).bfloat16().cuda()
+    sa().device_error()
+    o = sa().cache_attention(q, cache, dev(bad), dev(lengths))
+    assert sa().device_error() == INVALID
+    keepers = np.array([i for i in range(13) if i not in (1, 4, 12)], np.int32)
+    check_attention(o, q, seqs, lengths, 16, 1.0, 64 ** -0.5, np.broadcast_to(keepers, (1, 64, 1, len(keepers))))
+    short = table[:, :7].copy()
+    o = sa().cache_attention(q, cache, dev(short), dev(lengths))
+    assert sa().device_error() == 0                       # a length past the table's end is no error
+    check_attention(o, q, [tuple(x[:, :112] for x in seqs[0])], lengths, 16, 1.0, 64 ** -0.5)
+
+
+def test_more_pages_than_a_block_keeps(cuda):
+    H, d, P, n = 1, 32, 16, 70000
+    cache, table, _ = filled(1, [n], H, d, P, seed=13)
+    q = torch.randn(1, 1, 2, d, generator=torch.Generator().manual_seed(8)).bfloat16().cuda()
+    got = sa().select_pages(q, cache, dev(table), dev([n]), 40)
+    want = F.select(num(q)[0], cache.bounds.cpu().numpy(), table[0], n, 0, 1, P, 40, 2)
+    assert np.array_equal(got[0, 0].cpu().numpy(), want)
+
+
+def test_pools_past_32_bits(cuda):
+    """Records beyond 4 GiB of a pool."""
+    H, d, P, n = 8, 128, 128, 300
+    pages = 30000                                             # 20 KiB a record: 4.9 GB
+    cache = sa().new_cache(pages, H, d, P)
+    table = np.array([[pages - 1, 5, pages - 7, -1]], np.int32)
+    g = torch.Generator().manual_seed(3)
+    K, V = (torch.randn(1, n, H, d, generator=g).bfloat16().cuda() for _ in range(2))
+    sa().cache_write(K, V, cache, dev(table), dev([0]))
+    k, v = (num(x) for x in sa().cache_read(cache, dev(table), dev([0]), n, dtype=torch.float32))
+    small = sa().KVCache(cache.pool[[pages - 1, 5, pages - 7]].contiguous(), cache.bounds[[pages - 1, 5, pages - 7]].contiguous())
+    other = dev([[0, 1, 2, -1]])
+    for a, b in zip(sa().cache_read(small, other, dev([0]), n, dtype=torch.float32), (k, v)):
+        assert np.array_equal(num(a), b)
+    for T in (1, 20):
+        q = torch.randn(1, T, 32, d, generator=g).bfloat16().cuda()
+        for alpha in (1.0, 1.5):
+            assert torch.equal(sa().cache_attention(q, cache, dev(table), dev([n]), alpha=alpha),
+                               sa().cache_attention(q, small, other, dev([n]), alpha=alpha))
+        assert torch.equal(sa().select_pages(q, cache, dev(table), dev([n]), 2),
+                           sa().select_pages(q, small, other, dev([n]), 2))
+    assert k.any() and v.any() and sa().device_error() == 0
+
+
+def test_select_refuses_too_many_heads(cuda):
+    cache = sa().new_cache(2, 1, 32, 16)
+    q = torch.zeros(1, 1, 257, 32, device="cuda").bfloat16()
+    with pytest.raises(RuntimeError):
+        sa().select_pages(q, cache, dev(np.zeros((1, 2))), dev([5]), 1)
+
+
+def test_launches_are_counted_and_timed(cuda):
+    from splash_attention import ops
+    lengths = [300]
+    cache, table, _ = filled(1, lengths, 2, 64, 16)
+    q = torch.randn(1, 1, 4, 64).bfloat16().cuda()
+    with ops.profile() as prof:
+        sa().cache_attention(q, cache, dev(table), dev(lengths))
+        sa().cache_attention(q, cache, dev(table), dev(lengths), alpha=1.5)
+        sa().select_pages(q, cache, dev(table), dev(lengths), 2)
+    assert {"cache_attention", "cache_entmax", "cache_select"} <= set(prof.result)
+    assert all(ms > 0 and n > 0 for ms, n in prof.result.values())
+
+
+def test_example(cuda):
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "serve_cache.py")
+    spec = importlib.util.spec_from_file_location("serve_cache", path)
+    m = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(m)
+    err = m.main(prompt=400, steps=2)
+    # a quantisation step is about range/15 of a group's 32 values: a uniform error of 1/sqrt(12)
+    # of 4 sigma / 15, 0.08 of a value; attention averages values and sharpens scores
+    assert err["keys read back"] < 0.1 and err["values read back"] < 0.1
+    assert all(e < 0.6 for e in err.values()), err
