@@ -39,7 +39,10 @@ namespace {
 constexpr int kTile = 2;              // blocks of a tile
 constexpr int kStages = 2;            // tiles a warp has in flight
 constexpr int kLeast = -8;            // weights are raised for small scales by 2^8 at most
-constexpr int kItemCost = 12;         // Plan::item_cost (8, 16, 24 measured: 48 ragged sequences 57.6, 48.5, 48.7 us, this 50; three guesses of 5 short ones 32.9, 33.7, 37.1, this 32.2)
+// Plan::item_cost.  Measured: 48 ragged sequences 57.6 us with 8, 50.4 with 12, 48.5 with 16;
+// three guesses of five short ones 32.9, 32.2, 33.7; listed pages (items of one size) 41.8 with
+// 8, 44.8 with 12, 46.2 with 4.
+constexpr int kItemCost = 12, kListedCost = 8;
 constexpr int kSegments = 32;         // segments a CTA lines up at a time
 
 
@@ -1097,7 +1100,7 @@ Plan make_plan(const Shape& s, int keep) {
     const int64_t items = (int64_t)p.U * p.tiles * s.H;
     p.split = p.cap > 32 && items < 8 * kSms * ctas_of(nt);
     p.tile = kTile * kBlock;
-    p.item_cost = kItemCost;
+    p.item_cost = keep ? kListedCost : kItemCost;
     p.least = nt == 1 ? 16 : 12;
     p.vec = 0;
     p.page_shift = 0;

@@ -43,9 +43,13 @@ def full(q, k, v, length, alpha):
 def main(B=2, prompt=1000, steps=8, heads=16, kv_heads=4, d=128, page=64, keep=8, alpha=1.5, seed=0):
     g = torch.Generator("cuda").manual_seed(seed)
     total = prompt + steps + 96
-    make = lambda h: torch.randn(B, total, h, d, generator=g, device="cuda").bfloat16()  # noqa: E731
-    q, k, v = make(heads), make(kv_heads), make(kv_heads)
-    k = k + 1.5 * torch.randn(B, total // 50 + 1, kv_heads, d, generator=g, device="cuda").repeat_interleave(50, 1)[:, :total].bfloat16()
+    make = lambda *shape: torch.randn(*shape, generator=g, device="cuda")  # noqa: E731
+    # keys in runs of 50 about a topic each; a query looks for the topic of a run before it
+    topic = make(B, total // 50 + 1, kv_heads, d)
+    run = torch.arange(total, device="cuda") // 50
+    look = (torch.rand(B, total, generator=g, device="cuda") * (run + 1)).long()
+    q = make(B, total, kv_heads, heads // kv_heads, d) + 0.8 * topic[torch.arange(B, device="cuda")[:, None], look].unsqueeze(3)
+    q, k, v = q.flatten(2, 3).bfloat16(), (make(B, total, kv_heads, d) + 1.5 * topic[:, run]).bfloat16(), make(B, total, kv_heads, d).bfloat16()
 
     # a page of the pool to every `page` tokens, handed out in any order
     per = -(-total // page)
