@@ -7,6 +7,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
+
 #include "../../include/asa.h"
 
 namespace asa {
@@ -51,6 +53,19 @@ struct Strides { int64_t b, t, h; };
 __device__ __forceinline__ void follow() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+// Allows a kernel `bytes` of dynamic shared memory, once a device (`done`: the kernel's own).
+struct Allowed { std::atomic<unsigned long long> devices{0}; };
+template <typename K>
+cudaError_t allow_shared(K kernel, int bytes, Allowed& done) {
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (dev < 64 && (done.devices.load(std::memory_order_relaxed) & bit)) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev < 64) done.devices.fetch_or(bit, std::memory_order_relaxed);
+    return e;
 }
 template <typename... P, typename... A>
 cudaError_t launch(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, A&&... args) {

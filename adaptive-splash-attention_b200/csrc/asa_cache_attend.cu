@@ -1121,8 +1121,8 @@ size_t lay_out(const Shape& s, const Plan& p, void* base, Space* w) {
         return q;
     };
     Space x{};
-    x.run = (int64_t*)take(((size_t)p.U + 1) * 8);
     if (p.split) {
+        x.run = (int64_t*)take(((size_t)p.U + 1) * 8);
         x.part = (float*)take((size_t)slots * rows * s.d * 4);
         x.part_ml = (float*)take((size_t)slots * 2 * rows * 4);
     }
@@ -1140,7 +1140,8 @@ cudaError_t launch_walk(const Args& a, cudaStream_t st) {
     constexpr int W = warps_of<NT>();
     const int smem = (int)sizeof(Smem<D, NT, W>);
     auto kernel = walk_kernel<D, NT, W, MODE>;
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static Allowed allowed;
+    cudaError_t e = allow_shared(kernel, smem, allowed);
     if (e != cudaSuccess) return e;
     const int64_t items = (int64_t)a.p.U * a.p.tiles * a.s.H;
     const unsigned grid = a.p.split ? kSms * ctas_of(NT) : (unsigned)items;
@@ -1157,7 +1158,8 @@ cudaError_t attend_as(const Args& a, cudaStream_t st) {
     } else {
         e = launch_walk<D, NT, kScores>(a, st);
         if (e != cudaSuccess) return e;
-        e = cudaFuncSetAttribute(threshold_kernel<NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kTauSmem);
+        static Allowed allowed;
+        e = allow_shared(threshold_kernel<NT>, kTauSmem, allowed);
         if (e != cudaSuccess) return e;
         e = launch(threshold_kernel<NT>, (unsigned)(items * NT), kTauThreads, kTauSmem, st, a);
         if (e == cudaSuccess) e = launch_walk<D, NT, kValues>(a, st);
@@ -1170,7 +1172,7 @@ cudaError_t attend_as(const Args& a, cudaStream_t st) {
 
 size_t attend_workspace(const Shape& s, int keep) {
     if (chunk_takes(s, keep)) return chunk_workspace(s);
-    return lay_out(s, make_plan(s, keep), nullptr, nullptr) + 16;
+    return lay_out(s, make_plan(s, keep), nullptr, nullptr);
 }
 
 cudaError_t attend(const Shape& s, const void* Q, Strides qs, const uint8_t* pool, const int32_t* table,

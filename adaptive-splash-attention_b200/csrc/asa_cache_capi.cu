@@ -52,6 +52,8 @@ int check(const asa_cache_params* p, Shape* s, bool queries) {
     return ASA_OK;
 }
 
+bool lacks(const void* ws, size_t bytes, size_t need) { return need && (bytes < need || !ws || !aligned(ws, 16)); }
+
 Strides strides(const int64_t v[3]) { return Strides{v[0], v[1], v[2]}; }
 
 // Times what is launched while it lives, when profiling is on.
@@ -141,7 +143,7 @@ int asa_cache_select(const asa_cache_params* p, const void* Q, const int64_t q_s
     if (!Q || !q_strides || !lengths || !pages || (s.width && !block_table) || (s.pages && !bounds))
         return ASA_ERR_INVALID;
     if (!aligned(bounds, 16)) return ASA_ERR_INVALID;
-    if (ws_bytes < asa::cache::select_workspace(s) || !ws || !aligned(ws, 16)) return ASA_ERR_WORKSPACE;
+    if (lacks(ws, ws_bytes, asa::cache::select_workspace(s))) return ASA_ERR_WORKSPACE;
     cudaStream_t st = (cudaStream_t)stream;
     Scope ps("cache_select", st);
     return asa::cuda_status_of(asa::cache::select(s, Q, strides(q_strides), (const int8_t*)bounds,
@@ -162,8 +164,7 @@ int asa_cache_attention(const asa_cache_params* p, const void* Q, const int64_t 
     if (!Q || !q_strides || !lengths || !O || (s.width && !block_table) || (s.pages && !pool))
         return ASA_ERR_INVALID;
     if (!aligned(pool, 16) || !aligned(O, 16)) return ASA_ERR_INVALID;
-    if (ws_bytes < asa::cache::attend_workspace(s, keep) || !ws || !aligned(ws, 16))
-        return ASA_ERR_WORKSPACE;
+    if (lacks(ws, ws_bytes, asa::cache::attend_workspace(s, keep))) return ASA_ERR_WORKSPACE;
     cudaStream_t st = (cudaStream_t)stream;
     Scope ps(s.alpha == 1.0f ? "cache_attention" : "cache_entmax", st);
     return asa::cuda_status_of(asa::cache::attend(s, Q, strides(q_strides), (const uint8_t*)pool,

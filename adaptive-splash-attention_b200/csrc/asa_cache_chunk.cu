@@ -641,8 +641,8 @@ size_t chunk_lay_out(const Shape& s, const Plan& p, void* base, Space* w) {
         return q;
     };
     Space x{};
-    x.run = (int64_t*)take(((size_t)p.U + 1) * 8);
     if (p.split) {
+        x.run = (int64_t*)take(((size_t)p.U + 1) * 8);
         x.part = (float*)take((size_t)2 * kSms * kRows * s.d * 4);
         x.part_ml = (float*)take((size_t)2 * kSms * 2 * kRows * 4);
     }
@@ -656,7 +656,8 @@ cudaError_t chunk_as(const Args& a, cudaStream_t st) {
     static_assert(smem <= 227 * 1024, "shared memory");
     const int64_t items = (int64_t)a.p.U * a.p.tiles * a.s.H;
     if (items * kRows > 0x7fffffff) return cudaErrorInvalidConfiguration;
-    cudaError_t e = cudaFuncSetAttribute(chunk_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static Allowed allowed;
+    cudaError_t e = allow_shared(chunk_kernel<D>, smem, allowed);
     if (e == cudaSuccess) e = launch(chunk_kernel<D>, a.p.split ? kSms : (unsigned)items, kThreads, smem, st, a);
     if (e != cudaSuccess || !a.p.split) return e;
     return launch(combine_kernel<D, kRows>, (unsigned)(items * kRows), 128, 0, st, a);
@@ -669,7 +670,7 @@ bool chunk_takes(const Shape& s, int keep) {
     return keep == 0 && s.alpha == 1.0f && (s.d == 64 || s.d == 128) && (int64_t)s.T * s.G >= 64;
 }
 
-size_t chunk_workspace(const Shape& s) { return chunk_lay_out(s, chunk_plan(s), nullptr, nullptr) + 16; }
+size_t chunk_workspace(const Shape& s) { return chunk_lay_out(s, chunk_plan(s), nullptr, nullptr); }
 
 cudaError_t chunk_attend(const Shape& s, const void* Q, Strides qs, const uint8_t* pool, const int32_t* table,
                          const int32_t* lengths, void* O, void* ws, int* err, cudaStream_t st) {

@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const __grid_constant__ 
 // One launch where the tables are short, or the items fill the SMs; else the pages are
 // scored by CTAs of their own first.
 bool scores_itself(const Shape& s) {
-    return s.width <= 512 || (s.width <= kShared && (int64_t)s.B * s.T * s.H >= 296);
+    return s.width <= 256 || (s.width <= kShared && (int64_t)s.B * s.T * s.H >= 296);
 }
 
 template <int D>
@@ -260,7 +260,8 @@ cudaError_t select_as(const Query& a, int32_t* pages, void* ws, cudaStream_t st)
     const size_t query = (size_t)((a.s.G + 7) & ~7) * (2 * D + 4) /* 67 KB at most */, keys = (size_t)a.s.width * 4;
     if (scores_itself(a.s)) {
         if (query + keys > 48 * 1024) {
-            const cudaError_t e = cudaFuncSetAttribute(pick_kernel<D, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, 116 * 1024);
+            static Allowed allowed;
+            const cudaError_t e = allow_shared(pick_kernel<D, true>, 116 * 1024, allowed);
             if (e != cudaSuccess) return e;
         }
         return launch(pick_kernel<D, true>, items, kThreads, query + keys, st, a, (const uint32_t*)nullptr, pages);
@@ -268,7 +269,8 @@ cudaError_t select_as(const Query& a, int32_t* pages, void* ws, cudaStream_t st)
     const int chunks = (a.s.width + kChunk - 1) / kChunk;
     if ((int64_t)items * chunks > 0x7fffffff) return cudaErrorInvalidConfiguration;
     if (query > 48 * 1024) {
-        const cudaError_t e = cudaFuncSetAttribute(score_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, 100 * 1024);
+        static Allowed allowed;
+        const cudaError_t e = allow_shared(score_kernel<D>, 100 * 1024, allowed);
         if (e != cudaSuccess) return e;
     }
     const cudaError_t e = launch(score_kernel<D>, items * chunks, 256, query, st, a, (uint32_t*)ws, chunks);
@@ -279,8 +281,7 @@ cudaError_t select_as(const Query& a, int32_t* pages, void* ws, cudaStream_t st)
 }  // namespace
 
 size_t select_workspace(const Shape& s) {
-    const size_t keys = scores_itself(s) ? 0 : (size_t)s.B * s.T * s.H * s.width * 4;
-    return (keys + 16 + 15) & ~size_t(15);
+    return scores_itself(s) ? 0 : ((size_t)s.B * s.T * s.H * s.width * 4 + 15) & ~size_t(15);
 }
 
 cudaError_t select(const Shape& s, const void* Q, Strides qs, const int8_t* bounds, const int32_t* table,

@@ -2,10 +2,10 @@
 // PyTorch's dispatcher, a thin layer over the C ABI of libasa.so.
 //
 //   splash_attention::cache_write(K, V, pool!, bounds!, block_table, start, count?)
-//   splash_attention::cache_read(pool, block_table, start, T, d, count?, out_f32) -> (K, V)
+//   splash_attention::cache_read(pool, bounds, block_table, start, T, count?, out_f32) -> (K, V)
 //   splash_attention::cache_bounds(bounds, pages) -> (upper, lower)
-//   splash_attention::cache_select(Q, bounds, block_table, lengths, keep, page_size) -> pages
-//   splash_attention::cache_attention(Q, pool, block_table, lengths, pages?, page_size, sm_scale, alpha) -> O
+//   splash_attention::cache_select(Q, pool, bounds, block_table, lengths, keep) -> pages
+//   splash_attention::cache_attention(Q, pool, bounds, block_table, lengths, pages?, sm_scale, alpha) -> O
 //
 // Outputs and workspaces come from PyTorch's caching allocator; launches go on
 // the current stream of the tensors' device.  Bad shapes raise ValueError, bad
@@ -66,10 +66,10 @@ Tensor index(const Tensor& t, const Tensor& like, c10::IntArrayRef shape, const 
     TORCH_CHECK_VALUE(t.dim() == (int64_t)shape.size(), "splash_attention: ", name, " must have ", shape.size(), " dimensions");
     for (size_t i = 0; i < shape.size(); ++i)
         TORCH_CHECK_VALUE(shape[i] < 0 || t.size(i) == shape[i], "splash_attention: ", name, " has shape ", t.sizes());
-    return t.to(at::kInt).contiguous();
+    return t.scalar_type() == at::kInt && t.is_contiguous() ? t : t.to(at::kInt).contiguous();
 }
 
-const int32_t* ints(const Tensor& t) { return t.defined() ? t.data_ptr<int32_t>() : nullptr; }
+const int32_t* ints(const Tensor& t) { return t.defined() ? t.const_data_ptr<int32_t>() : nullptr; }
 
 asa_stream_t stream_of(const Tensor& t) {
     return (asa_stream_t)c10::cuda::getCurrentCUDAStream(t.get_device()).stream();
@@ -132,8 +132,15 @@ void write_cuda(const Tensor& K, const Tensor& V, const Tensor& pool, const Tens
           "asa_cache_write");
 }
 
-std::tuple<Tensor, Tensor> read_cuda(const Tensor& pool, const Tensor& block_table, const Tensor& start, int64_t T,
-                                     int64_t d, const OptTensor& count, bool out_f32) {
+int64_t head_dim_of(const Tensor& bounds) {
+    TORCH_CHECK_VALUE(bounds.dim() == 3 && bounds.size(2) > ASA_CACHE_BOUNDS_PAD,
+                      "splash_attention: the bounds must be [pages, kv_heads, 2 * head_dim + 16]");
+    return (bounds.size(2) - ASA_CACHE_BOUNDS_PAD) / 2;
+}
+
+std::tuple<Tensor, Tensor> read_cuda(const Tensor& pool, const Tensor& bounds, const Tensor& block_table,
+                                     const Tensor& start, int64_t T, const OptTensor& count, bool out_f32) {
+    const int64_t d = head_dim_of(bounds);
     const int64_t P = page_size_of(pool, d), H = pool.size(1);
     TORCH_CHECK_VALUE(start.dim() == 1, "splash_attention: start must be [B]");
     const int64_t B = start.size(0);
@@ -152,9 +159,7 @@ std::tuple<Tensor, Tensor> read_cuda(const Tensor& pool, const Tensor& block_tab
 }
 
 std::tuple<Tensor, Tensor> bounds_cuda(const Tensor& bounds, const Tensor& pages) {
-    TORCH_CHECK_VALUE(bounds.dim() == 3 && bounds.size(2) > ASA_CACHE_BOUNDS_PAD, "splash_attention: the bounds must be "
-                      "[pages, kv_heads, 2 * head_dim + 16]");
-    const int64_t d = (bounds.size(2) - ASA_CACHE_BOUNDS_PAD) / 2, H = bounds.size(1);
+    const int64_t d = head_dim_of(bounds), H = bounds.size(1);
     check_bounds(bounds, d);
     const Tensor ids = index(pages, bounds, {-1}, "pages");
     c10::cuda::CUDAGuard guard(bounds.device());
@@ -174,12 +179,13 @@ void check_queries(const Tensor& Q, int64_t kv_heads) {
                       " heads are not a multiple of the cache's ", kv_heads);
 }
 
-Tensor select_cuda(const Tensor& Q, const Tensor& bounds, const Tensor& block_table, const Tensor& lengths, int64_t keep,
-                   int64_t page_size) {
+Tensor select_cuda(const Tensor& Q, const Tensor& pool, const Tensor& bounds, const Tensor& block_table,
+                   const Tensor& lengths, int64_t keep) {
     TORCH_CHECK_VALUE(bounds.dim() == 3 && Q.dim() == 4, "splash_attention: q must be [B, T, heads, head_dim]");
     const int64_t B = Q.size(0), T = Q.size(1), d = Q.size(3), H = bounds.size(1);
     check_queries(Q, H);
     check_bounds(bounds, d);
+    const int64_t page_size = page_size_of(pool, d);
     same_device(Q, bounds, "the bounds");
     TORCH_CHECK_VALUE(keep >= 1 && keep <= INT_MAX, "splash_attention: keep must be at least 1");
     const Tensor tab = index(block_table, Q, {B, -1}, "block_table"), len = index(lengths, Q, {B}, "lengths");
@@ -189,20 +195,21 @@ Tensor select_cuda(const Tensor& Q, const Tensor& bounds, const Tensor& block_ta
     Tensor out = at::empty({B, T, H, keep}, Q.options().dtype(at::kInt));
     size_t bytes = 0;
     check(asa_cache_workspace_bytes(&p, 0, nullptr, &bytes), "asa_cache_workspace_bytes");
-    Tensor ws = at::empty({(int64_t)bytes}, Q.options().dtype(at::kByte));
+    Tensor ws;
+    if (bytes) ws = at::empty({(int64_t)bytes}, Q.options().dtype(at::kByte));
     check(asa_cache_select(&p, q.t.data_ptr(), q.s, bounds.data_ptr(), ints(tab), ints(len), (int)keep,
-                           out.data_ptr<int32_t>(), ws.data_ptr(), bytes, stream_of(Q)),
+                           out.data_ptr<int32_t>(), bytes ? ws.data_ptr() : nullptr, bytes, stream_of(Q)),
           "asa_cache_select");
     return out;
 }
 
-Tensor attention_cuda(const Tensor& Q, const Tensor& pool, const Tensor& block_table, const Tensor& lengths,
-                      const OptTensor& pages, int64_t page_size, double sm_scale, double alpha) {
+Tensor attention_cuda(const Tensor& Q, const Tensor& pool, const Tensor& bounds, const Tensor& block_table,
+                      const Tensor& lengths, const OptTensor& pages, double sm_scale, double alpha) {
     TORCH_CHECK_VALUE(pool.dim() == 3, "splash_attention: the pool must be [pages, kv_heads, record]");
     check_queries(Q, pool.size(1));
     const int64_t B = Q.size(0), T = Q.size(1), HQ = Q.size(2), d = Q.size(3), H = pool.size(1);
+    TORCH_CHECK_VALUE(head_dim_of(bounds) == d, "splash_attention: q's head_dim ", d, " is not the cache's");
     const int64_t P = page_size_of(pool, d);
-    TORCH_CHECK_VALUE(P == page_size, "splash_attention: q's head_dim ", d, " is not the cache's");
     same_device(Q, pool, "the pool");
     TORCH_CHECK_VALUE(alpha == 1.0 || (alpha >= 1.05 && alpha <= 3.0), "splash_attention: alpha must be 1 (softmax) or in [1.05, 3]");
     const Tensor tab = index(block_table, Q, {B, -1}, "block_table"), len = index(lengths, Q, {B}, "lengths");
@@ -221,9 +228,10 @@ Tensor attention_cuda(const Tensor& Q, const Tensor& pool, const Tensor& block_t
     Tensor O = at::empty({B, T, HQ, d}, Q.options());
     size_t bytes = 0;
     check(asa_cache_workspace_bytes(&p, keep, &bytes, nullptr), "asa_cache_workspace_bytes");
-    Tensor ws = at::empty({(int64_t)bytes}, Q.options().dtype(at::kByte));
+    Tensor ws;
+    if (bytes) ws = at::empty({(int64_t)bytes}, Q.options().dtype(at::kByte));
     check(asa_cache_attention(&p, q.t.data_ptr(), q.s, pool.data_ptr(), ints(tab), ints(len), ints(list), keep,
-                              O.data_ptr(), ws.data_ptr(), bytes, stream_of(Q)),
+                              O.data_ptr(), bytes ? ws.data_ptr() : nullptr, bytes, stream_of(Q)),
           "asa_cache_attention");
     return O;
 }
@@ -231,8 +239,9 @@ Tensor attention_cuda(const Tensor& Q, const Tensor& pool, const Tensor& block_t
 void write_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
                 const OptTensor&) {}
 
-std::tuple<Tensor, Tensor> read_meta(const Tensor& pool, const Tensor&, const Tensor& start, int64_t T, int64_t d,
-                                     const OptTensor&, bool out_f32) {
+std::tuple<Tensor, Tensor> read_meta(const Tensor& pool, const Tensor& bounds, const Tensor&, const Tensor& start,
+                                     int64_t T, const OptTensor&, bool out_f32) {
+    const int64_t d = head_dim_of(bounds);
     const auto opt = pool.options().dtype(out_f32 ? at::kFloat : at::kBFloat16);
     return {at::empty({start.size(0), T, pool.size(1), d}, opt), at::empty({start.size(0), T, pool.size(1), d}, opt)};
 }
@@ -243,12 +252,12 @@ std::tuple<Tensor, Tensor> bounds_meta(const Tensor& bounds, const Tensor& pages
     return {at::empty({pages.size(0), bounds.size(1), d}, opt), at::empty({pages.size(0), bounds.size(1), d}, opt)};
 }
 
-Tensor select_meta(const Tensor& Q, const Tensor& bounds, const Tensor&, const Tensor&, int64_t keep, int64_t) {
+Tensor select_meta(const Tensor& Q, const Tensor&, const Tensor& bounds, const Tensor&, const Tensor&, int64_t keep) {
     return at::empty({Q.size(0), Q.size(1), bounds.size(1), keep}, Q.options().dtype(at::kInt));
 }
 
-Tensor attention_meta(const Tensor& Q, const Tensor&, const Tensor&, const Tensor&, const OptTensor&, int64_t, double,
-                      double) {
+Tensor attention_meta(const Tensor& Q, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&,
+                      double, double) {
     return at::empty(Q.sizes(), Q.options());
 }
 
@@ -257,11 +266,11 @@ Tensor attention_meta(const Tensor& Q, const Tensor&, const Tensor&, const Tenso
 TORCH_LIBRARY_FRAGMENT(splash_attention, m) {
     m.def("cache_write(Tensor K, Tensor V, Tensor(a!) pool, Tensor(b!) bounds, Tensor block_table, Tensor start, "
           "Tensor? count) -> ()");
-    m.def("cache_read(Tensor pool, Tensor block_table, Tensor start, int T, int d, Tensor? count, bool out_f32) "
+    m.def("cache_read(Tensor pool, Tensor bounds, Tensor block_table, Tensor start, int T, Tensor? count, bool out_f32) "
           "-> (Tensor, Tensor)");
     m.def("cache_bounds(Tensor bounds, Tensor pages) -> (Tensor, Tensor)");
-    m.def("cache_select(Tensor Q, Tensor bounds, Tensor block_table, Tensor lengths, int keep, int page_size) -> Tensor");
-    m.def("cache_attention(Tensor Q, Tensor pool, Tensor block_table, Tensor lengths, Tensor? pages, int page_size, "
+    m.def("cache_select(Tensor Q, Tensor pool, Tensor bounds, Tensor block_table, Tensor lengths, int keep) -> Tensor");
+    m.def("cache_attention(Tensor Q, Tensor pool, Tensor bounds, Tensor block_table, Tensor lengths, Tensor? pages, "
           "float sm_scale, float alpha) -> Tensor");
 }
 
@@ -279,4 +288,15 @@ TORCH_LIBRARY_IMPL(splash_attention, Meta, m) {
     m.impl("cache_bounds", &bounds_meta);
     m.impl("cache_select", &select_meta);
     m.impl("cache_attention", &attention_meta);
+}
+
+// A cache is read by inference: its operators pass autograd by (outputs carry no
+// gradient), which also spares a call the boxed fallback for operators without one.
+TORCH_LIBRARY_IMPL(splash_attention, Autograd, m) {
+    for (const char* name : {"cache_write", "cache_read", "cache_bounds", "cache_select", "cache_attention"})
+        m.impl(name, torch::CppFunction::makeFallthrough());
+}
+TORCH_LIBRARY_IMPL(splash_attention, ADInplaceOrView, m) {
+    for (const char* name : {"cache_write", "cache_read", "cache_bounds", "cache_select", "cache_attention"})
+        m.impl(name, torch::CppFunction::makeFallthrough());
 }

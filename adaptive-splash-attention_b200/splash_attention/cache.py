@@ -7,8 +7,8 @@ or the α-entmax weights of training, ``select_pages`` chooses the pages a query
 reads by a cheap score of the pages' bounds, and ``cache_read`` and
 ``cache_bounds`` read it back.  The formats are described in include/asa.h.
 Every computation runs in hand-written CUDA kernels behind the C ABI; the calls
-go on the current stream, synchronise nothing and can be captured in CUDA
-graphs.  The reference has no counterpart.
+go on the current stream, synchronise nothing, can be captured in CUDA graphs and
+carry no gradients.  The reference has no counterpart.
 
 Index tensors (block tables, lengths, starts, counts, page lists) are int32 on
 the cache's device; other integer types are converted.  Positions past the
@@ -19,7 +19,10 @@ from typing import NamedTuple
 
 import torch
 
+# (the overloads themselves: a step makes these calls once a layer)
 _ops = torch.ops.splash_attention
+_cache_write, _cache_read, _cache_bounds = (getattr(_ops, n).default for n in ("cache_write", "cache_read", "cache_bounds"))
+_cache_select, _cache_attention = _ops.cache_select.default, _ops.cache_attention.default
 
 BOUNDS_PAD = 16
 HEAD_DIMS = (32, 64, 96, 128)
@@ -63,7 +66,7 @@ def cache_write(K, V, cache, block_table, start, count=None):
     ``count``) at positions start[b], start[b] + 1, ... of its ``block_table`` row.
     A page belongs to one sequence; its bounds start over when its first slot is
     written, and otherwise grow."""
-    _ops.cache_write(K, V, cache.pool, cache.bounds, block_table, start, count)
+    _cache_write(K, V, cache.pool, cache.bounds, block_table, start, count)
 
 
 def cache_read(cache, block_table, start, T, count=None, *, dtype=torch.bfloat16):
@@ -71,13 +74,13 @@ def cache_read(cache, block_table, start, T, count=None, *, dtype=torch.bfloat16
     [B, T, kv_heads, head_dim] bfloat16 or float32, zero from ``count[b]`` on."""
     if dtype not in (torch.float32, torch.bfloat16):
         raise TypeError(f"splash_attention: unsupported dtype {dtype} (float32 or bfloat16)")
-    return _ops.cache_read(cache.pool, block_table, start, T, cache.head_dim, count, dtype == torch.float32)
+    return _cache_read(cache.pool, cache.bounds, block_table, start, T, count, dtype == torch.float32)
 
 
 def cache_bounds(cache, pages):
     """The bounds of the pool's pages ``pages`` [n] as values: (upper, lower)
     float32 [n, kv_heads, head_dim], no channel's keys above or below them."""
-    return _ops.cache_bounds(cache.bounds, pages)
+    return _cache_bounds(cache.bounds, pages)
 
 
 def select_pages(q, cache, block_table, lengths, keep):
@@ -87,7 +90,7 @@ def select_pages(q, cache, block_table, lengths, keep):
     at position lengths[b] - T + t.  Its own page is always among them; the others
     score highest by an upper bound of q.k from their bounds, the largest over the
     heads that share the key head, ties to the earlier page."""
-    return _ops.cache_select(q, cache.bounds, block_table, lengths, keep, cache.page_size)
+    return _cache_select(q, cache.pool, cache.bounds, block_table, lengths, keep)
 
 
 def cache_attention(q, cache, block_table, lengths, *, sm_scale=None, alpha=1.0, pages=None):
@@ -104,4 +107,4 @@ def cache_attention(q, cache, block_table, lengths, *, sm_scale=None, alpha=1.0,
     NaN or an infinity NaN."""
     if sm_scale is None:
         sm_scale = q.shape[-1] ** -0.5
-    return _ops.cache_attention(q, cache.pool, block_table, lengths, pages, cache.page_size, sm_scale, alpha)
+    return _cache_attention(q, cache.pool, cache.bounds, block_table, lengths, pages, sm_scale, alpha)

@@ -253,7 +253,7 @@ typedef struct asa_cache_params {
 long long asa_cache_record_bytes(int d, int page_size);
 
 /* Workspace of asa_cache_attention (keep > 0: over that many selected pages)
- * and of asa_cache_select, in bytes. */
+ * and of asa_cache_select, in bytes (0: none is needed, NULL may be passed). */
 int asa_cache_workspace_bytes(const asa_cache_params* p, int keep, size_t* attend_bytes,
                               size_t* select_bytes);
 

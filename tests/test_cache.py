@@ -41,7 +41,8 @@ def test_rejects_bad_params(field, value, code):
 
 def test_workspaces():
     rc, a, s = workspace(params())
-    assert rc == 0 and a > 0 and s > 0
+    assert rc == 0 and a % 16 == 0 and s % 16 == 0
+    assert workspace(params(table_width=4096))[1] > 0 and workspace(params(table_width=4096))[2] > 0
     assert workspace(params(alpha=1.5), 3)[0] == 0
     assert workspace(params(), -1)[0] == L.ASA_ERR_INVALID
 
@@ -120,9 +121,9 @@ def test_operator_shapes():
     meta = lambda *s, dtype=torch.bfloat16: torch.empty(*s, dtype=dtype, device="meta")  # noqa: E731
     i = lambda *s: meta(*s, dtype=torch.int32)  # noqa: E731
     q, pool, bounds = meta(2, 3, 8, 64), meta(5, 4, 16 * 80, dtype=torch.uint8), meta(5, 4, 144, dtype=torch.int8)
-    assert ops.cache_attention(q, pool, i(2, 3), i(2), None, 16, 0.1, 1.0).shape == q.shape
-    assert ops.cache_select(q, bounds, i(2, 3), i(2), 6, 16).shape == (2, 3, 4, 6)
-    k, v = ops.cache_read(pool, i(2, 3), i(2), 7, 64, None, True)
+    assert ops.cache_attention(q, pool, bounds, i(2, 3), i(2), None, 0.1, 1.0).shape == q.shape
+    assert ops.cache_select(q, pool, bounds, i(2, 3), i(2), 6).shape == (2, 3, 4, 6)
+    k, v = ops.cache_read(pool, bounds, i(2, 3), i(2), 7, None, True)
     assert k.shape == v.shape == (2, 7, 4, 64) and k.dtype == torch.float32
     assert ops.cache_bounds(bounds, i(9))[0].shape == (9, 4, 64)
     assert "Tensor(a!) pool" in str(ops.cache_write.default._schema)
