@@ -15,7 +15,7 @@ namespace {
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 
 // Eight neighbouring channels: words as they lie in memory, values as fp32, and the
-// lane-wise larger and smaller of two (NaN aside).
+// lane-wise larger (NaN aside) and smaller (which keeps a NaN) of two.
 template <typename X>
 struct Eight;
 template <>
@@ -46,9 +46,9 @@ struct Eight<float> {
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = fmaxf(x[i], o.x[i]);
     }
-    __device__ __forceinline__ void lower(const Eight& o) {
+    __device__ __forceinline__ void lower(const Eight& o) {      // keeps a NaN
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = fminf(x[i], o.x[i]);
+        for (int i = 0; i < 8; ++i) asm("min.NaN.f32 %0, %0, %1;" : "+f"(x[i]) : "f"(o.x[i]));
     }
     __device__ __forceinline__ void nan_to_zero() {
 #pragma unroll
@@ -89,10 +89,10 @@ struct Eight<__nv_bfloat16> {
             w[i] = reinterpret_cast<const uint32_t&>(c);
         }
     }
-    __device__ __forceinline__ void lower(const Eight& o) {
+    __device__ __forceinline__ void lower(const Eight& o) {      // keeps a NaN
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const __nv_bfloat162 c = __hmin2(reinterpret_cast<const __nv_bfloat162&>(w[i]), reinterpret_cast<const __nv_bfloat162&>(o.w[i]));
+            const __nv_bfloat162 c = __hmin2_nan(reinterpret_cast<const __nv_bfloat162&>(w[i]), reinterpret_cast<const __nv_bfloat162&>(o.w[i]));
             w[i] = reinterpret_cast<const uint32_t&>(c);
         }
     }
@@ -117,13 +117,12 @@ template <typename X>
 __device__ __forceinline__ void quantise(const Eight<X> (&x)[4], uint32_t (&codes)[4], uint32_t& grid) {
     constexpr float kMagic = 12582912.0f;
     Eight<X> least = x[0], most = x[0];
-    bool nan = x[0].nan();
 #pragma unroll
     for (int i = 1; i < 4; ++i) {
         least.lower(x[i]);
         most.raise(x[i]);
-        nan |= x[i].nan();
     }
+    const bool nan = least.nan();
     float lo = least.at(0), hi = most.at(0);
 #pragma unroll
     for (int i = 1; i < 8; ++i) lo = fminf(lo, least.at(i)), hi = fmaxf(hi, most.at(i));
@@ -142,9 +141,12 @@ __device__ __forceinline__ void quantise(const Eight<X> (&x)[4], uint32_t (&code
     for (int i = 0; i < 4; ++i) {
         float r[8];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const float y = x[i].at(j) - z, q = y * inv;
-            r[j] = (fmaf(fmaf(-q, s, y), inv, q) + kMagic) - kMagic;
+        for (int j = 0; j < 8; j += 2) {              // two at a time
+            const float2 y = __fadd2_rn(make_float2(x[i].at(j), x[i].at(j + 1)), make_float2(-z, -z));
+            const float2 inv2 = make_float2(inv, inv), q = __fmul2_rn(y, inv2);
+            const float2 rest = __ffma2_rn(q, make_float2(-s, -s), y);
+            const float2 n = __fadd2_rn(__fadd2_rn(__ffma2_rn(rest, inv2, q), make_float2(kMagic, kMagic)), make_float2(-kMagic, -kMagic));
+            r[j] = n.x, r[j + 1] = n.y;
         }
         if (!plain)
 #pragma unroll
@@ -200,28 +202,33 @@ __global__ void __launch_bounds__(NTHR) write_kernel(Shape s, const X* __restric
     uint8_t* const s_par = s_rec + 2 * s.P * RB;
     auto body = [&](auto vec_c) {
         constexpr bool VEC = decltype(vec_c)::value;
-        for (int i = tid; i < 2 * rows * NG; i += NTHR) {
-            const int g = i % NG, row = i / NG, part = row >= rows, r = part ? row - rows : row;
-            const X* src = (part ? vp + r * vs.t : kp + r * ks.t) + 32 * g;
-            Eight<X> x[4];
-            uint32_t codes[4], grid;
+        auto quantise_part = [&](auto part_c, const X* base, int64_t stride) {
+            constexpr int part = decltype(part_c)::value;   // keys, values
+            for (int i = tid; i < rows * NG; i += NTHR) {
+                const int r = i / NG, g = i % NG;
+                const X* src = base + r * stride + 32 * g;
+                Eight<X> x[4];
+                uint32_t codes[4], grid;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) x[k].template load<VEC>(src + 8 * k);
-            quantise<X>(x, codes, grid);
-            uint8_t* to = s_rec + (part * s.P + r) * RB;
+                for (int k = 0; k < 4; ++k) x[k].template load<VEC>(src + 8 * k);
+                quantise<X>(x, codes, grid);
+                uint8_t* to = s_rec + (part * s.P + r) * RB;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                if (part) {
-                    *reinterpret_cast<uint16_t*>(to + 2 * k * 2 * NG + 2 * g) = (uint16_t)codes[k];
-                    *reinterpret_cast<uint16_t*>(to + (2 * k + 1) * 2 * NG + 2 * g) = (uint16_t)(codes[k] >> 16);
-                } else {
-                    *reinterpret_cast<uint32_t*>(to + k * 4 * NG + 4 * g) = codes[k];
+                for (int k = 0; k < 4; ++k) {
+                    if constexpr (part == 1) {
+                        *reinterpret_cast<uint16_t*>(to + 2 * k * 2 * NG + 2 * g) = (uint16_t)codes[k];
+                        *reinterpret_cast<uint16_t*>(to + (2 * k + 1) * 2 * NG + 2 * g) = (uint16_t)(codes[k] >> 16);
+                    } else {
+                        *reinterpret_cast<uint32_t*>(to + k * 4 * NG + 4 * g) = codes[k];
+                    }
                 }
+                uint16_t* par = reinterpret_cast<uint16_t*>(s_par + (part * s.P + r) * PB) + g;
+                par[0] = (uint16_t)grid;
+                par[NG] = (uint16_t)(grid >> 16);
             }
-            uint16_t* par = reinterpret_cast<uint16_t*>(s_par + (part * s.P + r) * PB) + g;
-            par[0] = (uint16_t)grid;
-            par[NG] = (uint16_t)(grid >> 16);
-        }
+        };
+        quantise_part(std::integral_constant<int, 0>{}, kp, ks.t);
+        quantise_part(std::integral_constant<int, 1>{}, vp, vs.t);
         // bounds of this thread's eight channels over its set of tokens
         const int set = tid / LR, c8 = tid % LR;
         if (set < SETS) {
@@ -232,9 +239,19 @@ __global__ void __launch_bounds__(NTHR) write_kernel(Shape s, const X* __restric
             for (int r = set; r < rows; r += SETS) {
                 Eight<X> x;
                 x.template load<VEC>(kp + r * ks.t + 8 * c8);
-                if (x.nan()) x.nan_to_zero();
                 hi.raise(x);
                 lo.lower(x);
+            }
+            if (lo.nan()) {                           // again, with NaN as 0
+                hi.fill(-INFINITY);
+                lo.fill(INFINITY);
+                for (int r = set; r < rows; r += SETS) {
+                    Eight<X> x;
+                    x.template load<VEC>(kp + r * ks.t + 8 * c8);
+                    x.nan_to_zero();
+                    hi.raise(x);
+                    lo.lower(x);
+                }
             }
 #pragma unroll
             for (int i = 0; i < 8; i += 4) {
