@@ -68,19 +68,27 @@ cudaError_t allow_shared(K kernel, int bytes, Allowed& done) {
     return e;
 }
 template <typename... P, typename... A>
-cudaError_t launch(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, A&&... args) {
+cudaError_t launch_clusters(int cluster, void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t st,
+                            A&&... args) {
     cudaLaunchConfig_t c{};
     c.gridDim = dim3(grid);
     c.blockDim = dim3(block);
     c.dynamicSmemBytes = smem;
     c.stream = st;
-    cudaLaunchAttribute at{};
-    at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    at.val.programmaticStreamSerializationAllowed = 1;
-    c.attrs = &at;
-    c.numAttrs = 1;
+    cudaLaunchAttribute at[2]{};
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = cluster;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    c.attrs = at;
+    c.numAttrs = cluster > 1 ? 2 : 1;
     note_launch();
     return cudaLaunchKernelEx(&c, kernel, P(args)...);
+}
+template <typename... P, typename... A>
+cudaError_t launch(void (*kernel)(P...), unsigned grid, unsigned block, size_t smem, cudaStream_t st, A&&... args) {
+    return launch_clusters(1, kernel, grid, block, smem, st, args...);
 }
 #endif
 

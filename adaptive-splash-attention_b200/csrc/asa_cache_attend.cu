@@ -99,6 +99,22 @@ __device__ __forceinline__ uint32_t hmax2(uint32_t a, uint32_t b) {
     const __half2 h = __hmax2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
     return *reinterpret_cast<const uint32_t*>(&h);
 }
+__device__ __forceinline__ void cluster_sync() {
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+// What lies at a place of this CTA's shared memory, in the cluster's CTA `rank`.
+template <typename V>
+__device__ __forceinline__ V remote(const V* p, int rank) {
+    uint32_t at;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(sm100::smem_u32(p)), "r"(rank));
+    V v;
+    if constexpr (sizeof(V) == 16)
+        asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    else
+        asm volatile("ld.shared::cluster.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(at) : "memory");
+    return v;
+}
+
 // The token (0..7) that stands at index m of an 8-token half block in the
 // fragments: neighbours 2, 3 and 6, 7 trade places, which spreads the values' rows
 // over the shared-memory banks.
@@ -154,6 +170,7 @@ struct Smem {
     alignas(128) uint8_t ring[W][kStages][2 * kTile * block_bytes(D)];
     float4 o[W / 2][8 * NT][kStride / 4];
     float m[W][8 * NT], l[W][8 * NT];
+    float2 ml[8 * NT];                                // this CTA's references and sums, for its cluster
     Rows<D / 32, NT> rows[2];
     Info info[W][kStages];
     uint64_t full[W][kStages];
@@ -259,8 +276,10 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                 sm.next = y;
             }
         } else if (tid == 0) {
-            const int u = blockIdx.x / per, of = unit_tiles(a, u);
-            sm.seg[0] = Segment{u, (int)(blockIdx.x % per), 0, of, of};
+            const unsigned no = blockIdx.x / (unsigned)a.p.cluster, rank = blockIdx.x % (unsigned)a.p.cluster;
+            const int u = no / (unsigned)per, of = unit_tiles(a, u);
+            const int from = (int)((int64_t)of * rank / a.p.cluster), to = (int)((int64_t)of * (rank + 1) / a.p.cluster);
+            sm.seg[0] = Segment{u, (int)(no % (unsigned)per), from, to - from, of};
             sm.segs = 1;
             sm.next = 1;
         }
@@ -799,8 +818,14 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                     }
                     __syncthreads();
                 }
-                const bool all = g.n == g.of;
+                const bool all = g.n == g.of && a.p.cluster == 1;
                 const int64_t slot = 2 * (int64_t)blockIdx.x + (g.from + g.n < g.of ? 1 : 0);
+                auto put = [&](int row, int c4, float4 acc, float sum) {
+                    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+                    __nv_bfloat162 y[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv),
+                                           __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
+                    *reinterpret_cast<uint2*>(a.O + (int64_t)mine_rows.out[row] * D + 4 * c4) = *reinterpret_cast<uint2*>(y);
+                };
                 for (int i = tid; i < rows * (D / 4); i += NTHR) {
                     const int row = i / (D / 4), c4 = i % (D / 4);
                     float top = sm.m[0][row];
@@ -816,14 +841,35 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                         acc = make_float4(acc.x + y.x, acc.y + y.y, acc.z + y.z, acc.w + y.w);
                     }
                     if (all) {
-                        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-                        __nv_bfloat162 y[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv),
-                                               __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
-                        *reinterpret_cast<uint2*>(a.O + (int64_t)mine_rows.out[row] * D + 4 * c4) = *reinterpret_cast<uint2*>(y);
+                        put(row, c4, acc, sum);
+                    } else if (a.p.cluster > 1) {
+                        sm.o[0][row][c4] = acc;       // (no other thread reads or writes this place)
+                        if (c4 == 0) sm.ml[row] = make_float2(top, sum);
                     } else {
                         *reinterpret_cast<float4*>(a.w.part + (slot * ROWS + row) * D + 4 * c4) = acc;
                         if (c4 == 0) *reinterpret_cast<float2*>(a.w.part_ml + (slot * ROWS + row) * 2) = make_float2(top, sum);
                     }
+                }
+                if (a.p.cluster > 1) {                // the cluster's CTAs each join a part of the item's outputs
+                    cluster_sync();
+                    const int total = rows * (D / 4), share = (total + a.p.cluster - 1) / a.p.cluster;
+                    const int first = (int)(blockIdx.x % (unsigned)a.p.cluster) * share;
+                    for (int i = first + tid; i < min(first + share, total); i += NTHR) {
+                        const int row = i / (D / 4), c4 = i % (D / 4);
+                        float top = kLow, sum = 0.0f;
+                        for (int k = 0; k < a.p.cluster; ++k) top = fmaxf(top, remote<float2>(&sm.ml[row], k).x);
+                        float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+                        for (int k = 0; k < a.p.cluster; ++k) {
+                            const float2 ml = remote<float2>(&sm.ml[row], k);
+                            const float4 y = remote<float4>(&sm.o[0][row][c4], k);
+                            const float f = exp2_fast(ml.x - top);
+                            sum = fmaf(ml.y, f, sum);
+                            acc = make_float4(fmaf(y.x, f, acc.x), fmaf(y.y, f, acc.y), fmaf(y.z, f, acc.z), fmaf(y.w, f, acc.w));
+                        }
+                        put(row, c4, acc, sum);
+                    }
+                    cluster_sync();                   // no CTA leaves while its sums are read
                 }
                 __syncthreads();                      // sm.m, sm.o and the rows are free again
             }
@@ -1085,20 +1131,45 @@ template <int NT>
 constexpr int warps_of() { return NT == 1 ? 8 : 4; }
 constexpr int ctas_of(int nt) { return nt == 1 ? 2 : 3; }        // an SM holds
 
-int row_tiles(const Shape& s, bool lists) { return (lists ? s.G : s.T * s.G) > 8 ? 2 : 1; }
+// Row tiles (of 8) that a CTA takes at once.  Two share the reading and unpacking of the
+// codes, which pays where the tiles keep all warps busy: nine or more a warp, by
+// the rows that fill them.  Us with one and with two: 64 sequences of 1024 tokens, 8
+// key heads of 16 rows, head size 64, 53.1 and 37.6; 8 of 8192, 32 rows, 57.1 and 45.6; 32
+// of 4096, 16 rows, head size 128, 94.0 and 88.5.  With fewer the smaller grain wins:
+// 8 of 4096, 12 rows, 28.9 and 38.1; 1 of 4096, 13.7 and 19.2.
+int row_tiles(const Shape& s, int keep) {
+    const int64_t rows = keep ? s.G : (int64_t)s.T * s.G, blocks = (int64_t)(keep ? keep : s.width) * (s.P / kBlock);
+    const int64_t tiles = (int64_t)(keep ? s.B * s.T : s.B) * s.H * ((blocks + kTile - 1) / kTile);
+    return rows > 8 && tiles * rows >= 16ll * 9 * kSms * 3 * 4 ? 2 : 1;
+}
 
 Plan make_plan(const Shape& s, int keep) {
     Plan p;
-    const int nt = row_tiles(s, keep > 0);
+    const int nt = row_tiles(s, keep);
     p.U = keep ? s.B * s.T : s.B;
     p.R = keep ? s.G : s.T * s.G;
     p.tiles = (p.R + 8 * nt - 1) / (8 * nt);
     p.keep = keep;
     p.cap = ((keep ? keep : s.width) * (s.P / kBlock) + kTile - 1) / kTile;
-    // Short caches, and calls with many items a CTA, are left whole: an item's only
-    // CTA writes the output itself and nothing is joined.
-    const int64_t items = (int64_t)p.U * p.tiles * s.H;
-    p.split = p.cap > 32 && items < 8 * kSms * ctas_of(nt);
+    const int64_t items = (int64_t)p.U * p.tiles * s.H, slots = (int64_t)kSms * ctas_of(nt);
+    const int warps = nt == 1 ? 8 : 4;
+    // An item is taken by one CTA, or by a cluster whose CTAs join their sums over
+    // its shared memory: as many CTAs as have a tile a warp, and as the SMs hold for all
+    // items at once.  Or else all items are cut into equal runs, one a CTA, at the price
+    // of a second kernel: about five rounds, a round being a tile to each warp.  So they
+    // are cut where that takes fewer rounds, lengths taken to be three quarters of
+    // what the table holds.  Head size 128, 8 key heads of 4 query heads, us by CTA, by
+    // cluster of the size taken, and by runs:
+    //    1 sequence   of   512 tokens  9.2,  9.2, 13.5;  4096  30.3, 11.4, 14.4;  16384  101.6, 20.8, 18.1
+    //    8 sequences  of  1024 tokens 12.8, 11.2, 16.5;  4096  31.8, 20.5, 25.1;  32768  202.0, 85.1, 82.5
+    //   64 sequences  of  1024 tokens 34.9, -, 41.4;     4096  89.7, -, 92.2;      8192  162.2, -, 154.9
+    const auto ceil_div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
+    p.cluster = 1;
+    while (p.cluster < 8 && items * 2 * p.cluster <= slots && p.cap > p.cluster * warps) p.cluster *= 2;
+    const int64_t whole = ceil_div(items * p.cluster, slots) * ceil_div(p.cap, p.cluster * warps);
+    const int64_t runs = items * p.cap * (keep ? 4 : 3) / (4 * slots * warps) + 5;
+    p.split = items < 8 * slots && whole > runs;      // (many items even out, and runs count them all)
+    if (p.split) p.cluster = 1;
     p.tile = kTile * kBlock;
     p.item_cost = keep ? kListedCost : kItemCost;
     p.least = nt == 1 ? 16 : 12;
@@ -1112,7 +1183,7 @@ size_t up256(size_t x) { return (x + 255) & ~size_t(255); }
 
 // Offsets of the workspace's parts; its size.
 size_t lay_out(const Shape& s, const Plan& p, void* base, Space* w) {
-    const int nt = row_tiles(s, p.keep > 0), rows = 8 * nt;
+    const int nt = row_tiles(s, p.keep), rows = 8 * nt;
     const int64_t items = (int64_t)p.U * p.tiles * s.H, slots = 2ll * kSms * ctas_of(nt);
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -1144,8 +1215,8 @@ cudaError_t launch_walk(const Args& a, cudaStream_t st) {
     cudaError_t e = allow_shared(kernel, smem, allowed);
     if (e != cudaSuccess) return e;
     const int64_t items = (int64_t)a.p.U * a.p.tiles * a.s.H;
-    const unsigned grid = a.p.split ? kSms * ctas_of(NT) : (unsigned)items;
-    return launch(kernel, grid, W * 32, smem, st, a);
+    const unsigned grid = a.p.split ? kSms * ctas_of(NT) : (unsigned)(items * a.p.cluster);
+    return launch_clusters(a.p.cluster, kernel, grid, W * 32, smem, st, a);
 }
 
 template <int D, int NT>
@@ -1165,7 +1236,7 @@ cudaError_t attend_as(const Args& a, cudaStream_t st) {
         if (e == cudaSuccess) e = launch_walk<D, NT, kValues>(a, st);
     }
     if (e != cudaSuccess || !a.p.split) return e;
-    return launch(combine_kernel<D, 8 * NT>, (unsigned)(items * 8 * NT), 128, 0, st, a);
+    return launch(combine_kernel<D, 8 * NT, NT>, (unsigned)(items * 8), 128, 0, st, a);
 }
 
 }  // namespace
@@ -1192,7 +1263,7 @@ cudaError_t attend(const Shape& s, const void* Q, Strides qs, const uint8_t* poo
     a.O = (__nv_bfloat16*)O;
     a.err = err;
     a.p.vec = (reinterpret_cast<uintptr_t>(Q) & 15) == 0 && qs.b % 8 == 0 && qs.t % 8 == 0 && qs.h % 8 == 0;
-    const bool two = row_tiles(s, keep > 0) == 2;
+    const bool two = row_tiles(s, keep) == 2;
     switch (s.d) {
         case 32: return two ? attend_as<32, 2>(a, st) : attend_as<32, 1>(a, st);
         case 64: return two ? attend_as<64, 2>(a, st) : attend_as<64, 1>(a, st);

@@ -21,7 +21,8 @@ struct Plan {
     int U, R, tiles;                  // units of rows (sequences; with lists, query tokens), rows each, tiles each
     int keep;                         // pages listed a query and key head (0: all of the table)
     int cap;                          // tiles an item can have at most
-    int split;                        // items are cut into equal runs (else one CTA an item)
+    int split;                        // items are cut into equal runs (else one cluster an item)
+    int cluster;                      // CTAs of an item's cluster
     int vec;                          // q rows may be read 16 bytes at a time
     int page_shift;                   // log2 of the blocks of a page
     int tile;                         // tokens of a tile
@@ -115,62 +116,76 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* s_warp, int64_
 }
 
 // ---- joining an item that several CTAs walked -------------------------------------
-// A CTA a row: its warps take the parts in turn, a lane four channels.
-template <int D, int ROWS>
+// A CTA K rows: its warps take the parts in turn, a lane four channels of each row,
+// and keep a running reference a row, as the walk does.
+template <int D, int ROWS, int K>
 __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Args a) {
-    __shared__ float s_top[4], s_sum[4];
-    __shared__ float4 s_acc[4][D / 4];
+    __shared__ float2 s_ml[4][K];
+    __shared__ float4 s_acc[4][K][D / 4];
     follow();
     const Shape& s = a.s;
     const int per = a.p.tiles * s.H, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int row = blockIdx.x % ROWS, item_no = blockIdx.x / ROWS;
+    const int row0 = (int)(blockIdx.x % (ROWS / K)) * K, item_no = blockIdx.x / (ROWS / K);
     const int u = item_no / per, item = item_no % per, h = item / a.p.tiles, tile = item % a.p.tiles;
-    if (tile * ROWS + row >= a.p.R) return;
+    if (tile * ROWS + row0 >= a.p.R) return;
     const int of = unit_tiles(a, u);
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-    float sum = 0.0f;
+    float m[K], l[K];
+    float4 acc[K];
+#pragma unroll
+    for (int k = 0; k < K; ++k) m[k] = kLow, l[k] = 0.0f, acc[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     if (of) {
         const int64_t run = a.w.run[0], x0 = a.w.run[1 + u] + (int64_t)item * (of + a.p.item_cost) + a.p.item_cost;
         const int64_t c0 = x0 / run, c1 = (x0 + of - 1) / run;
         if (c0 == c1) return;                         // one CTA had it all, and wrote the output
         const int n = (int)(c1 - c0) + 1;
-        // the last CTA's part is its first segment, the others' their last
-        auto slot = [&](int i) { return 2 * (c0 + i) + (i + 1 < n ? 1 : 0); };
-        float top = kLow;
-        for (int i = threadIdx.x; i < n; i += 128) top = fmaxf(top, a.w.part_ml[(slot(i) * ROWS + row) * 2]);
-#pragma unroll
-        for (int k = 16; k; k >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, k));
-        if (lane == 0) s_top[warp] = top;
-        __syncthreads();
-        top = fmaxf(fmaxf(s_top[0], s_top[1]), fmaxf(s_top[2], s_top[3]));
-#pragma unroll 4
+#pragma unroll(K >= 4 ? 1 : 4)
         for (int i = warp; i < n; i += 4) {
-            const float2 ml = *reinterpret_cast<const float2*>(a.w.part_ml + (slot(i) * ROWS + row) * 2);
-            float4 y = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-            if (lane < D / 4) y = *reinterpret_cast<const float4*>(a.w.part + (slot(i) * ROWS + row) * D + 4 * lane);
-            const float f = exp2_fast(ml.x - top);
-            sum = fmaf(ml.y, f, sum);
-            acc = make_float4(fmaf(y.x, f, acc.x), fmaf(y.y, f, acc.y), fmaf(y.z, f, acc.z), fmaf(y.w, f, acc.w));
-        }
-        if (lane == 0) s_sum[warp] = sum;
-        if (lane < D / 4) s_acc[warp][lane] = acc;
-        __syncthreads();
-        sum = s_sum[0] + s_sum[1] + s_sum[2] + s_sum[3];
-        if (lane < D / 4) {
-            acc = s_acc[0][lane];
+            // the last CTA's part is its first segment, the others' their last
+            const int64_t at = (2 * (c0 + i) + (i + 1 < n ? 1 : 0)) * ROWS + row0;
+            float2 ml[K];
+            float4 y[K];
 #pragma unroll
-            for (int w = 1; w < 4; ++w) {
-                const float4 y = s_acc[w][lane];
-                acc = make_float4(acc.x + y.x, acc.y + y.y, acc.z + y.z, acc.w + y.w);
+            for (int k = 0; k < K; ++k) {
+                ml[k] = *reinterpret_cast<const float2*>(a.w.part_ml + (at + k) * 2);
+                y[k] = lane < D / 4 ? *reinterpret_cast<const float4*>(a.w.part + (at + k) * D + 4 * lane)
+                                    : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+#pragma unroll
+            for (int k = 0; k < K; ++k) {
+                const float top = fmaxf(m[k], ml[k].x), f = exp2_fast(m[k] - top), g = exp2_fast(ml[k].x - top);
+                m[k] = top;
+                l[k] = fmaf(l[k], f, ml[k].y * g);
+                acc[k] = make_float4(fmaf(acc[k].x, f, y[k].x * g), fmaf(acc[k].y, f, y[k].y * g),
+                                     fmaf(acc[k].z, f, y[k].z * g), fmaf(acc[k].w, f, y[k].w * g));
             }
         }
     }
-    if (warp || lane >= D / 4) return;
-    const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
-    __nv_bfloat162 y[2] = {__floats2bfloat162_rn(acc.x * inv, acc.y * inv), __floats2bfloat162_rn(acc.z * inv, acc.w * inv)};
-    const int b = a.list ? u / s.T : u, x = tile * ROWS + row;
-    const int tq = a.list ? u % s.T : x / s.G, g = a.list ? x : x % s.G;
-    *reinterpret_cast<uint2*>(a.O + (((int64_t)b * s.T + tq) * s.HQ + h * s.G + g) * D + 4 * lane) = *reinterpret_cast<uint2*>(y);
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+        if (lane == 0) s_ml[warp][k] = make_float2(m[k], l[k]);
+        if (lane < D / 4) s_acc[warp][k][lane] = acc[k];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < K * (D / 4); i += 128) {
+        const int k = i / (D / 4), c4 = i % (D / 4), x = tile * ROWS + row0 + k;
+        if (x >= a.p.R) break;
+        float top = s_ml[0][k].x, sum = 0.0f;
+#pragma unroll
+        for (int w = 1; w < 4; ++w) top = fmaxf(top, s_ml[w][k].x);
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+            const float f = exp2_fast(s_ml[w][k].x - top);
+            const float4 y = s_acc[w][k][c4];
+            sum = fmaf(s_ml[w][k].y, f, sum);
+            o = make_float4(fmaf(y.x, f, o.x), fmaf(y.y, f, o.y), fmaf(y.z, f, o.z), fmaf(y.w, f, o.w));
+        }
+        const float inv = sum == 0.0f ? 0.0f : 1.0f / sum;
+        __nv_bfloat162 y[2] = {__floats2bfloat162_rn(o.x * inv, o.y * inv), __floats2bfloat162_rn(o.z * inv, o.w * inv)};
+        const int b = a.list ? u / s.T : u;
+        const int tq = a.list ? u % s.T : x / s.G, g = a.list ? x : x % s.G;
+        *reinterpret_cast<uint2*>(a.O + (((int64_t)b * s.T + tq) * s.HQ + h * s.G + g) * D + 4 * c4) = *reinterpret_cast<uint2*>(y);
+    }
 }
 
 }  // namespace

@@ -626,9 +626,15 @@ Plan chunk_plan(const Shape& s) {
     p.tile = kTokens;
     p.item_cost = kChunkCost;
     const int64_t items = (int64_t)p.U * p.tiles * s.H;
-    // many items, or short ones, are left whole
-    p.split = p.cap > 4 && items < 8 * kSms;
+    // Items are left whole, or cut into equal runs, whose parts' way through memory
+    // costs as much as about nine tiles and one to each twenty items.  Head size 128, 8 key
+    // heads of 4 query heads, us whole and cut: 128 tokens behind 384 17.9, 24.1, behind
+    // 3968 66.0, 34.4; 512 tokens behind 3584 67.0, 85.9, behind 32256 456, 421; 640
+    // tokens (160 items to 148 SMs) behind 7552 238.5, 160.8.
+    const int64_t whole = (items + kSms - 1) / kSms * p.cap, runs = items * p.cap / kSms + 9 + items / 20;
+    p.split = items < 8 * kSms && whole > runs;
     p.least = kChunkCost + 2;
+    p.cluster = 1;
     while (kBlock << p.page_shift < s.P) ++p.page_shift;
     return p;
 }
@@ -660,7 +666,7 @@ cudaError_t chunk_as(const Args& a, cudaStream_t st) {
     cudaError_t e = allow_shared(chunk_kernel<D>, smem, allowed);
     if (e == cudaSuccess) e = launch(chunk_kernel<D>, a.p.split ? kSms : (unsigned)items, kThreads, smem, st, a);
     if (e != cudaSuccess || !a.p.split) return e;
-    return launch(combine_kernel<D, kRows>, (unsigned)(items * kRows), 128, 0, st, a);
+    return launch(combine_kernel<D, kRows, 8>, (unsigned)(items * (kRows / 8)), 128, 0, st, a);
 }
 
 }  // namespace

@@ -251,7 +251,7 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const __grid_constant__ 
 // One launch where the tables are short, or the items fill the SMs; else the pages are
 // scored by CTAs of their own first.
 bool scores_itself(const Shape& s) {
-    return s.width <= 256 || (s.width <= kShared && (int64_t)s.B * s.T * s.H >= 296);
+    return s.width <= 512 || (s.width <= kShared && (int64_t)s.B * s.T * s.H >= 296);
 }
 
 template <int D>
