@@ -436,9 +436,13 @@ cudaError_t write_as(const Shape& s, const void* K, const void* V, Strides ks, S
     };
     const int vec = fits(K, ks) && fits(V, vs);
     const size_t smem = (size_t)2 * s.P * (row_bytes(D) + par_bytes(D));   // 20 KB at most
-    // A step writes a token or a few of each sequence: two warps a page then start sooner than eight.
-    const auto kernel = s.T <= 4 ? write_kernel<X, D, 64> : write_kernel<X, D, 256>;
-    return launch(kernel, (unsigned)grid, s.T <= 4 ? 64 : 256, smem, st, s, (const X*)K, (const X*)V, ks, vs, vec, pool,
+    // Two warps a page where the page is small and pages are many, else four (which
+    // shorten the way of one).  Us with 64 threads and with 128, 8 key heads, bfloat16: head
+    // size 128, 65536 tokens in pages of 16 105.7 and 155.7, of 32 91.5 and 103.3, of 64 91.0
+    // and 89.0; 2048 tokens in pages of 32 6.4 and 5.5, 512 in pages of 64 8.7 and 5.4.
+    const bool two = s.P * D <= 4096 && grid >= 2048;
+    const auto kernel = two ? write_kernel<X, D, 64> : write_kernel<X, D, 128>;
+    return launch(kernel, (unsigned)grid, two ? 64 : 128, smem, st, s, (const X*)K, (const X*)V, ks, vs, vec, pool,
                   bounds, table, start, count, touched, page_shift, err);
 }
 
