@@ -1236,7 +1236,11 @@ cudaError_t attend_as(const Args& a, cudaStream_t st) {
         if (e == cudaSuccess) e = launch_walk<D, NT, kValues>(a, st);
     }
     if (e != cudaSuccess || !a.p.split) return e;
-    return launch(combine_kernel<D, 8 * NT, NT>, (unsigned)(items * 8), 128, 0, st, a);
+    // eight warps share a row's parts where items are few (2 sequences of 131072 tokens, 4
+    // key heads, with the walk: 51.1 us, 53.5 by four), else four (48 of up to 8192, 8 key
+    // heads: 52.3 by eight, 50.0)
+    if (items * 8 <= 4 * kSms) return launch(combine_kernel<D, 8 * NT, NT, 8>, (unsigned)(items * 8), 256, 0, st, a);
+    return launch(combine_kernel<D, 8 * NT, NT, 4>, (unsigned)(items * 8), 128, 0, st, a);
 }
 
 }  // namespace

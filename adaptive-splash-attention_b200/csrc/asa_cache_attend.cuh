@@ -116,12 +116,14 @@ __device__ __forceinline__ int64_t block_scan(int64_t v, int64_t* s_warp, int64_
 }
 
 // ---- joining an item that several CTAs walked -------------------------------------
-// A CTA K rows: its warps take the parts in turn, a lane four channels of each row,
-// and keep a running reference a row, as the walk does.
-template <int D, int ROWS, int K>
-__global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Args a) {
-    __shared__ float2 s_ml[4][K];
-    __shared__ float4 s_acc[4][K][D / 4];
+// A CTA K rows: its W warps take the parts in turn, a lane four channels of each row,
+// and keep a running reference a row, as the walk does.  Few rows have many parts
+// (the few items of long contexts), many rows few (the 128 of a prompt's chunk).
+template <int D, int ROWS, int K, int W>
+__global__ void __launch_bounds__(32 * W) combine_kernel(const __grid_constant__ Args a) {
+    constexpr int U = K >= 4 ? 1 : 4;                 // parts of a warp whose loads are under way at once
+    __shared__ float2 s_ml[W][K];
+    __shared__ float4 s_acc[W][K][D / 4];
     follow();
     const Shape& s = a.s;
     const int per = a.p.tiles * s.H, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -138,25 +140,36 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Ar
         const int64_t c0 = x0 / run, c1 = (x0 + of - 1) / run;
         if (c0 == c1) return;                         // one CTA had it all, and wrote the output
         const int n = (int)(c1 - c0) + 1;
-#pragma unroll(K >= 4 ? 1 : 4)
-        for (int i = warp; i < n; i += 4) {
-            // the last CTA's part is its first segment, the others' their last
-            const int64_t at = (2 * (c0 + i) + (i + 1 < n ? 1 : 0)) * ROWS + row0;
-            float2 ml[K];
-            float4 y[K];
+#pragma unroll 1
+        for (int i0 = warp; i0 < n; i0 += U * W) {
+            float2 ml[U][K];
+            float4 y[U][K];
 #pragma unroll
-            for (int k = 0; k < K; ++k) {
-                ml[k] = *reinterpret_cast<const float2*>(a.w.part_ml + (at + k) * 2);
-                y[k] = lane < D / 4 ? *reinterpret_cast<const float4*>(a.w.part + (at + k) * D + 4 * lane)
-                                    : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            for (int e = 0; e < U; ++e) {
+                // the last CTA's part is its first segment, the others' their last
+                const int i = i0 + e * W, j = U == 1 ? i : min(i, n - 1);
+                const int64_t at = (2 * (c0 + j) + (j + 1 < n ? 1 : 0)) * ROWS + row0;
+#pragma unroll
+                for (int k = 0; k < K; ++k) {
+                    ml[e][k] = *reinterpret_cast<const float2*>(a.w.part_ml + (at + k) * 2);
+                    y[e][k] = *reinterpret_cast<const float4*>(a.w.part + (at + k) * D + 4 * min(lane, D / 4 - 1));
+                    if (U > 1 && i >= n) ml[e][k] = make_float2(kLow, 0.0f), y[e][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                }
             }
 #pragma unroll
             for (int k = 0; k < K; ++k) {
-                const float top = fmaxf(m[k], ml[k].x), f = exp2_fast(m[k] - top), g = exp2_fast(ml[k].x - top);
+                float top = m[k];
+#pragma unroll
+                for (int e = 0; e < U; ++e) top = fmaxf(top, ml[e][k].x);
+                const float f = exp2_fast(m[k] - top);
                 m[k] = top;
-                l[k] = fmaf(l[k], f, ml[k].y * g);
-                acc[k] = make_float4(fmaf(acc[k].x, f, y[k].x * g), fmaf(acc[k].y, f, y[k].y * g),
-                                     fmaf(acc[k].z, f, y[k].z * g), fmaf(acc[k].w, f, y[k].w * g));
+#pragma unroll
+                for (int e = 0; e < U; ++e) {
+                    const float g = exp2_fast(ml[e][k].x - top), by = e ? 1.0f : f;
+                    l[k] = fmaf(l[k], by, ml[e][k].y * g);
+                    acc[k] = make_float4(fmaf(acc[k].x, by, y[e][k].x * g), fmaf(acc[k].y, by, y[e][k].y * g),
+                                         fmaf(acc[k].z, by, y[e][k].z * g), fmaf(acc[k].w, by, y[e][k].w * g));
+                }
             }
         }
     }
@@ -166,15 +179,15 @@ __global__ void __launch_bounds__(128) combine_kernel(const __grid_constant__ Ar
         if (lane < D / 4) s_acc[warp][k][lane] = acc[k];
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < K * (D / 4); i += 128) {
+    for (int i = threadIdx.x; i < K * (D / 4); i += 32 * W) {
         const int k = i / (D / 4), c4 = i % (D / 4), x = tile * ROWS + row0 + k;
         if (x >= a.p.R) break;
         float top = s_ml[0][k].x, sum = 0.0f;
 #pragma unroll
-        for (int w = 1; w < 4; ++w) top = fmaxf(top, s_ml[w][k].x);
+        for (int w = 1; w < W; ++w) top = fmaxf(top, s_ml[w][k].x);
         float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < W; ++w) {
             const float f = exp2_fast(s_ml[w][k].x - top);
             const float4 y = s_acc[w][k][c4];
             sum = fmaf(s_ml[w][k].y, f, sum);

@@ -666,7 +666,7 @@ cudaError_t chunk_as(const Args& a, cudaStream_t st) {
     cudaError_t e = allow_shared(chunk_kernel<D>, smem, allowed);
     if (e == cudaSuccess) e = launch(chunk_kernel<D>, a.p.split ? kSms : (unsigned)items, kThreads, smem, st, a);
     if (e != cudaSuccess || !a.p.split) return e;
-    return launch(combine_kernel<D, kRows, 8>, (unsigned)(items * (kRows / 8)), 128, 0, st, a);
+    return launch(combine_kernel<D, kRows, 8, 4>, (unsigned)(items * (kRows / 8)), 128, 0, st, a);
 }
 
 }  // namespace

@@ -81,11 +81,21 @@ __device__ __forceinline__ void make_query(const Query& a, int b, int t, int h, 
     }
 }
 
+// The ids of the pages of the table that a lane scores: p0 + r and p0 + r + 8.
+__device__ __forceinline__ void look_up(const Query& a, int b, int p0, int to, int (&next)[2]) {
+    const int r = (threadIdx.x & 31) >> 2;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+        const int page = p0 + r + 8 * e;
+        next[e] = page < to ? __ldg(a.table + (int64_t)b * a.s.width + page) : -1;
+    }
+}
+
 // Keys of pages from .. to - 1 (ordered scores; put(page, key, whether earlier heads had a say)) by
-// the warps of a CTA, 16 pages each.
+// the warps of a CTA, 16 pages each; `first`: the ids of a lane's first two.
 template <int D, typename Put>
 __device__ __forceinline__ void score_pages(const Query& a, int b, int h, int from, int to, int warps, const int8_t* s_q,
-                                            const float* s_unit, Put put) {
+                                            const float* s_unit, const int (&first)[2], Put put) {
     constexpr int SEG = 2 * D / 64;                   // 64-byte stretches of a page's bounds
     const Shape& s = a.s;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, q4 = lane & 3;
@@ -96,22 +106,15 @@ __device__ __forceinline__ void score_pages(const Query& a, int b, int h, int fr
             w[k] = *reinterpret_cast<const uint4*>(s_q + (8 * tile + r) * 2 * D + 64 * k + 16 * q4);
         const float u0 = s_unit[8 * tile + 2 * q4], u1 = s_unit[8 * tile + 2 * q4 + 1];
         const bool in0 = 8 * tile + 2 * q4 < s.G, in1 = 8 * tile + 2 * q4 + 1 < s.G;
-        int next[2];                                  // the pages' ids, looked up an iteration ahead
-        auto look_up = [&](int p0) {
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const int page = p0 + r + 8 * e;
-                next[e] = page < to ? __ldg(a.table + (int64_t)b * s.width + page) : -1;
-            }
-        };
-        look_up(from + 16 * warp);
+        int next[2] = {first[0], first[1]};           // the pages' ids, looked up an iteration ahead
+        if (tile) look_up(a, b, from + 16 * warp, to, next);
         for (int p0 = from + 16 * warp; p0 < to; p0 += 16 * warps) {
             const int8_t* rec[2];
             float scale[2];
             uint4 x[2][SEG];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
-                const int id = next[e];
+                const int id = p0 + r + 8 * e < to ? next[e] : -1;
                 rec[e] = nullptr;
                 scale[e] = 0.0f;
                 if (id >= 0 && id < s.pages) rec[e] = a.bounds + ((int64_t)id * s.H + h) * bounds_bytes(D);
@@ -121,7 +124,7 @@ __device__ __forceinline__ void score_pages(const Query& a, int b, int h, int fr
                     x[e][k] = rec[e] ? __ldg(reinterpret_cast<const uint4*>(rec[e] + 64 * k + 16 * q4)) : make_uint4(0u, 0u, 0u, 0u);
                 if (rec[e]) scale[e] = __int_as_float((min(max(__ldg(reinterpret_cast<const int*>(rec[e] + 2 * D)), -126), 127) + 127) << 23);
             }
-            look_up(p0 + 16 * warps);
+            look_up(a, b, p0 + 16 * warps, to, next);
             int acc[4] = {0, 0, 0, 0};
 #pragma unroll
             for (int k = 0; k < SEG; ++k) {
@@ -148,15 +151,28 @@ __global__ void __launch_bounds__(256) score_kernel(const __grid_constant__ Quer
     follow();
     const int item = blockIdx.x / chunks, chunk = blockIdx.x % chunks;
     const int h = item % a.s.H, bt = item / a.s.H, t = bt % a.s.T, b = bt / a.s.T;
-    const int n = pages_seen(a, b, t);
-    if (n <= a.keep) return;
     uint32_t* key = keys + (int64_t)item * a.s.width;
     extern __shared__ __align__(16) int8_t s_q[];
     float* s_unit = reinterpret_cast<float*>(s_q + ((a.s.G + 7) & ~7) * 2 * D);
+    int first[2];                                     // (its load and the query's do not wait for the length)
+    look_up(a, b, chunk * kChunk + 16 * (threadIdx.x >> 5), a.s.width, first);
+    const int n = pages_seen(a, b, t);
     make_query<D>(a, b, t, h, s_q, s_unit);
     __syncthreads();
-    score_pages<D>(a, b, h, chunk * kChunk, min((chunk + 1) * kChunk, n - 1), 8, s_q, s_unit,
+    if (n <= a.keep) return;
+    score_pages<D>(a, b, h, chunk * kChunk, min((chunk + 1) * kChunk, n - 1), 8, s_q, s_unit, first,
                    [&](int page, uint32_t k, bool more) { key[page] = more ? max(key[page], k) : k; });
+}
+
+// The bits in which a CTA's keys differ (0: none do), and a key: from each warp's.
+__device__ __forceinline__ uint32_t cta_differ(uint32_t any, uint32_t all, uint32_t* slot, uint32_t* common) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (lane == 0) slot[warp] = any, slot[kWarps + warp] = all;
+    __syncthreads();
+    any = __reduce_or_sync(~0u, lane < kWarps ? slot[lane] : 0u);
+    all = __reduce_and_sync(~0u, lane < kWarps ? slot[kWarps + lane] : ~0u);
+    *common = all;
+    return any & ~all;
 }
 
 // Sum of a number a warp over the CTA, and over the warps before this one.  One
@@ -176,6 +192,8 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const __grid_constant__ 
                                                         int32_t* __restrict__ pages) {
     extern __shared__ __align__(16) int8_t s_q[];    // the query, its units, the keys
     __shared__ int s_count[2][kWarps];
+    __shared__ uint32_t s_bits[2 * kWarps];
+    __shared__ int4 s_three[2][kWarps];
     float* s_unit = reinterpret_cast<float*>(s_q + ((a.s.G + 7) & ~7) * 2 * D);
     uint32_t* s_key = reinterpret_cast<uint32_t*>(s_unit + ((a.s.G + 7) & ~7));
     const Shape& s = a.s;
@@ -183,7 +201,10 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const __grid_constant__ 
     follow();
     const int h = blockIdx.x % s.H, bt = blockIdx.x / s.H, t = bt % s.T, b = bt / s.T;
     int32_t* out = pages + (int64_t)blockIdx.x * keep;
+    int first[2];                                     // (its load and the query's do not wait for the length)
+    if constexpr (SCORE) look_up(a, b, 16 * warp, s.width, first);
     const int n = pages_seen(a, b, t);
+    if constexpr (SCORE) make_query<D>(a, b, t, h, s_q, s_unit);
     if (n <= keep) {
         for (int i = tid; i < keep; i += kThreads) out[i] = i < n ? i : -1;
         return;
@@ -191,9 +212,8 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const __grid_constant__ 
     const int m = n - 1;                              // those that are weighed; the query's own is taken
     const uint32_t* key = keys + (int64_t)blockIdx.x * s.width;
     if constexpr (SCORE) {
-        make_query<D>(a, b, t, h, s_q, s_unit);
         __syncthreads();
-        score_pages<D>(a, b, h, 0, m, kWarps, s_q, s_unit,
+        score_pages<D>(a, b, h, 0, m, kWarps, s_q, s_unit, first,
                        [&](int page, uint32_t k, bool more) { s_key[page] = more ? max(s_key[page], k) : k; });
     } else if (m <= kShared) {
         s_key = reinterpret_cast<uint32_t*>(s_q);
@@ -201,18 +221,36 @@ __global__ void __launch_bounds__(kThreads) pick_kernel(const __grid_constant__ 
     }
     if (SCORE || m <= kShared) key = s_key;
     __syncthreads();
-    // the largest number that `need` keys reach
+    // The largest number that `need` keys reach: the bits that all keys share, then two
+    // bits a step, by the counts of keys that reach each of the three numbers.
     const int need = keep - 1;
     uint32_t edge = 0;
     int above = m;                                    // keys that reach it
-    if (need == 0) edge = ~0u, above = -1;            // (none is taken)
     int turn = 0;
-    for (int bit = 31; bit >= 0 && above != need && need; --bit, turn ^= 1) {
-        const uint32_t next = edge | 1u << bit;
-        int count = 0;
-        for (int i = tid; i < m; i += kThreads) count += key[i] >= next;
-        count = cta_sum(__reduce_add_sync(~0u, count), s_count[turn]);
-        if (count >= need) edge = next, above = count;
+    if (need == 0) {
+        edge = ~0u, above = -1;                       // (none is taken)
+    } else {
+        uint32_t any = 0u, every = ~0u;
+        for (int i = tid; i < m; i += kThreads) any |= key[i], every &= key[i];
+        const uint32_t differ = cta_differ(__reduce_or_sync(~0u, any), __reduce_and_sync(~0u, every), s_bits, &edge);
+        int bit = differ ? (31 - __clz(differ)) & ~1 : -1;
+        if (bit >= 0) edge &= bit == 30 ? 0u : ~0u << (bit + 2);
+        for (; bit >= 0 && above != need; bit -= 2, turn ^= 1) {
+            const uint32_t t1 = edge | 1u << bit, t2 = edge | 2u << bit, t3 = edge | 3u << bit;
+            int n1 = 0, n2 = 0, n3 = 0;
+            for (int i = tid; i < m; i += kThreads) {
+                const uint32_t k = key[i];
+                n1 += k >= t1, n2 += k >= t2, n3 += k >= t3;
+            }
+            n1 = __reduce_add_sync(~0u, n1), n2 = __reduce_add_sync(~0u, n2), n3 = __reduce_add_sync(~0u, n3);
+            if (lane == 0) s_three[turn][warp] = make_int4(n1, n2, n3, 0);
+            __syncthreads();
+            const int4 of = lane < kWarps ? s_three[turn][lane] : make_int4(0, 0, 0, 0);
+            n1 = __reduce_add_sync(~0u, of.x), n2 = __reduce_add_sync(~0u, of.y), n3 = __reduce_add_sync(~0u, of.z);
+            if (n3 >= need) edge = t3, above = n3;
+            else if (n2 >= need) edge = t2, above = n2;
+            else if (n1 >= need) edge = t1, above = n1;
+        }
     }
     // Keys beyond the edge are taken, and of those on it the first; where exactly
     // `need` reach it, all are.
