@@ -6,13 +6,26 @@
 //
 // Work.  An item is a tile of 8 or 16 query rows of one key head (rows of one
 // sequence, or of one query token where each has its own pages); its keys are
-// walked in tiles of 32 tokens.  The items' tiles, laid end to end with a few
-// tiles' worth of time between items for what starting one costs, are cut into
+// walked in tiles of 32 tokens.  Short items are taken whole, by a CTA or a cluster
+// that joins its sums over shared memory.  Else the items' tiles, laid end to end with
+// a few tiles' worth of time between items for what starting one costs, are cut into
 // equal runs, one a CTA, so that a batch of very unequal sequences keeps every SM
 // busy; an item that a cut divides is joined by combine_kernel from its runs'
 // partial sums (largest score, sum of weights, weighted values), in a fixed order.
 // A CTA's warps take an item's tiles in turn, each with its own ring of bulk
 // copies that runs ahead into the CTA's next item.
+//
+// What it reads bounds it: 1.25 d bytes a token and key head, against 4 d operations
+// a query head.  Two sequences of 131072 tokens, 4 key heads of 8 query heads, d 128
+// (168 MB) take 51 us with the join, 3.3 TB/s: 33 us of that go by the tokens, 5.0 TB/s
+// or 0.78 of a copy's rate, the rest is starting, the warps' and the runs' joins.  A tile
+// is some 1.6 us of a warp, most of it waiting on its own chain (codes, products,
+// maxima, weights, products); 16 warps an SM at 128 registers each cover that, and
+// keeping the next tile's products in registers as well was slower (it spilled).
+// Below a few thousand tokens the chain itself is what is left: 8 us for 100 tokens.
+// Entmax, 8 sequences of 32768, 8 key heads: scores 42 us (168 MB of keys in, 67 MB of
+// scores out), thresholds 18, values 18 of which most is finding the few tiles
+// that have weight.
 //
 // Arithmetic.  A code 0..15 in an fp16 half is the subnormal n * 2^-24, and in
 // the next nibble n * 2^-20: masking a word gives tensor-core operands without
@@ -44,7 +57,6 @@ constexpr int kLeast = -8;            // weights are raised for small scales by 
 // 8, 44.8 with 12, 46.2 with 4.
 constexpr int kItemCost = 12, kListedCost = 8;
 constexpr int kSegments = 32;         // segments a CTA lines up at a time
-
 
 enum Mode { kSoftmax = 0, kScores = 1, kValues = 2 };
 
@@ -886,9 +898,11 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
 // One CTA an item's eight rows, a warp a row in the end.  A row's support lies
 // within 1 of its largest x = (alpha - 1) score: of the tiles whose maxima reach that
 // (listed first) each such x is put on its row's list, every lane in a stretch of its
-// own, so that no sum depends on timing; the stretches are closed up, and the root of sum (x - tau)_+^(1/(alpha-1)) = 1 is found among them by Newton's steps
-// from the left, kept inside a bracket.  Rows with more than a list holds (a flat
-// row, a small alpha) have every step read the tiles again.
+// own, so that no sum depends on timing; the stretches are closed up, and the root of
+// sum (x - tau)_+^(1/(alpha-1)) = 1 is found among them by Newton's steps from the left,
+// kept inside a bracket.  Rows with more than a list holds (a flat row, a small
+// alpha) have every step read the tiles again.  One dependent step after another is
+// what it costs: 9 us over 2000 tokens, 18 over 32768 (64 items, 2 MB of maxima).
 constexpr int kTauThreads = 512, kTauWarps = kTauThreads / 32;
 constexpr int kTileList = 2048;       // tiles listed
 constexpr int kListCap = 1024;        // of a row, closed up
