@@ -896,16 +896,21 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
 
 // ---- the alpha-entmax threshold ----------------------------------------------------
 // One CTA an item's eight rows, a warp a row in the end.  A row's support lies
-// within 1 of its largest x = (alpha - 1) score: of the tiles whose maxima reach that
-// (listed first) each such x is put on its row's list, every lane in a stretch of its
+// within 1 of its largest x = (alpha - 1) score, and above the threshold of any part of
+// its x: a few of Newton's steps over the tiles' maxima give such a bound (to the left
+// of the root the steps stay there, the sum being convex for alpha <= 2).  Of the tiles whose
+// maxima reach it (listed first) each such x is put on its row's list, every lane in a stretch of its
 // own, so that no sum depends on timing; the stretches are closed up, and the root of
 // sum (x - tau)_+^(1/(alpha-1)) = 1 is found among them by Newton's steps from the left,
 // kept inside a bracket.  Rows with more than a list holds (a flat row, a small
 // alpha) have every step read the tiles again.  One dependent step after another is
-// what it costs: 9 us over 2000 tokens, 18 over 32768 (64 items, 2 MB of maxima).
+// what it costs: 9 us over 2000 tokens, 14 over 32768 (64 items, 2 MB of maxima).
 constexpr int kTauThreads = 512, kTauWarps = kTauThreads / 32;
 constexpr int kTileList = 2048;       // tiles listed
 constexpr int kListCap = 1024;        // of a row, closed up
+// Without the bound, 8 sequences of 32768 tokens took 84 to 131 us by their numbers (a list
+// overflowed now and then), with it 80; three guesses of 2000 tokens 24.0 without, 25.4 with.
+constexpr int kBoundSteps = 4;
 constexpr int kPart = 13;             // of a row and lane (odd: no bank twice)
 constexpr int kTauSmem = (kTileList + 8 * kListCap + 8 * kTauWarps * 8 * kPart) * 4;
 
@@ -915,7 +920,7 @@ __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_con
     extern __shared__ int s_tiles[];
     float* const s_list = reinterpret_cast<float*>(s_tiles + kTileList);     // [8][kListCap]
     float* const s_part = s_list + 8 * kListCap;                             // [8][W * 8][kPart]
-    __shared__ float s_max[W][8], s_top[8], s_sum[W][8][2], s_tau[8];
+    __shared__ float s_max[W][8], s_top[8], s_low[8], s_sum[W][8][2], s_tau[8];
     __shared__ int s_count[W], s_rows[8][W * 8], s_mine[8];
     follow();
     const Shape& s = a.s;
@@ -945,8 +950,13 @@ __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_con
     for (int j = tid; j < nb; j += kTauThreads) {
         float y[8];
         tops_of(j, y);
+        // on the rows' lists for now, from kListCap tiles on the larger of what shares a place
+        float* const place = s_list + j % kListCap;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) top[i] = max_nan(top[i], y[i]);
+        for (int i = 0; i < 8; ++i) {
+            top[i] = max_nan(top[i], y[i]);
+            place[i * kListCap] = j < kListCap ? y[i] : max_nan(place[i * kListCap], y[i]);
+        }
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -960,9 +970,43 @@ __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_con
         for (int w = 1; w < W; ++w) y = max_nan(y, s_max[w][tid]);
         s_top[tid] = y;
     }
+    const float ex = 1.0f / (s.alpha - 1.0f);
+    auto gain = [&](float y, float tau, float& f, float& df) {   // y, tau relative to the row's maximum
+        const float d = y - tau;
+        if (!(d > 0.0f)) return;
+        if (s.alpha == 1.5f) {
+            f = fmaf(d, d, f);
+            df = fmaf(2.0f, d, df);
+        } else {
+            const float p = exp2f(log2f(d) * ex);
+            f += p;
+            df += ex * p / d;
+        }
+    };
     __syncthreads();
+    if (warp < 8) {                                   // row `warp`: a bound of its threshold
+        const float* list = s_list + warp * kListCap;
+        const float y0 = s_top[warp];
+        float tau = -1.0f;
+        for (int it = 0; it < (s.alpha <= 2.0f ? kBoundSteps : 0); ++it) {
+            float f = 0.0f, df = 0.0f;
+#pragma unroll 4
+            for (int i = lane; i < min(nb, kListCap); i += 32) gain(list[i] - y0, tau, f, df);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top[i] = s_top[i];
+            for (int k = 16; k; k >>= 1) {
+                f += __shfl_xor_sync(~0u, f, k);
+                df += __shfl_xor_sync(~0u, df, k);
+            }
+            if (!(f > 1.0f)) break;                   // (also: no key, or a NaN)
+            tau += (f - 1.0f) / df;
+        }
+        if (lane == 0) s_low[warp] = fmaxf(tau - 1e-4f, -1.0f);   // sums of fp32 are not that far off
+    }
+    __syncthreads();
+    float low[8];                                     // x that may have weight lie above
+#pragma unroll
+    for (int i = 0; i < 8; ++i) low[i] = s_top[i] + s_low[i];
+    const float low0 = s_low[2 * t], low1 = s_low[2 * t + 1];
     const float top0 = 2 * t < rows ? s_top[2 * t] : INFINITY, top1 = 2 * t + 1 < rows ? s_top[2 * t + 1] : INFINITY;
     // the tiles that may hold support, in order
     int listed = 0;
@@ -972,7 +1016,7 @@ __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_con
             float y[8];
             tops_of(base + tid, y);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) want |= y[i] > top[i] - 1.0f;
+            for (int i = 0; i < 8; ++i) want |= y[i] > low[i];
         }
         const uint32_t votes = __ballot_sync(~0u, want);
         if (lane == 0) s_count[warp] = __popc(votes);
@@ -1005,7 +1049,7 @@ __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_con
                         tops_of((int)j, z);
                         read = false;
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) read |= z[e] > top[e] - 1.0f;
+                        for (int e = 0; e < 8; ++e) read |= z[e] > low[e];
                     }
                     if (read) {
                         y[2 * k] = __ldg(tiles + j * kTile * NT * 32 + lane);
@@ -1021,17 +1065,17 @@ __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_con
     const int stretch = warp * 8 + (lane & 7);
     float* const l0 = s_part + (2 * t * W * 8 + stretch) * kPart;
     float* const l1 = l0 + W * 8 * kPart;
-    auto put = [&](float y, float* list, int& n) {
-        if (y > -1.0f) {
+    auto put = [&](float y, float least, float* list, int& n) {
+        if (y > least) {
             if (n < kPart) list[n] = y;
             ++n;
         }
     };
     each([&](float4 y) {
-        put(y.x - top0, l0, n0);
-        put(y.z - top0, l0, n0);
-        put(y.y - top1, l1, n1);
-        put(y.w - top1, l1, n1);
+        put(y.x - top0, low0, l0, n0);
+        put(y.z - top0, low0, l0, n0);
+        put(y.y - top1, low1, l1, n1);
+        put(y.w - top1, low1, l1, n1);
     });
     s_rows[2 * t][stretch] = n0;
     s_rows[2 * t + 1][stretch] = n1;
@@ -1062,19 +1106,6 @@ __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_con
         for (int k = 0; k < n1; ++k) s_list[(2 * t + 1) * kListCap + s_rows[2 * t + 1][stretch] + k] = l1[k];
     }
     __syncthreads();
-    const float ex = 1.0f / (s.alpha - 1.0f);
-    auto gain = [&](float y, float tau, float& f, float& df) {   // y, tau relative to the row's maximum
-        const float d = y - tau;
-        if (!(d > 0.0f)) return;
-        if (s.alpha == 1.5f) {
-            f = fmaf(d, d, f);
-            df = fmaf(2.0f, d, df);
-        } else {
-            const float p = exp2f(log2f(d) * ex);
-            f += p;
-            df += ex * p / d;
-        }
-    };
     // one step: the bracket [lo, hi] around the root, the next point within it
     auto step = [](float f, float df, float& lo, float& hi, float& tau) {
         if (f >= 1.0f) lo = tau; else hi = tau;
@@ -1088,7 +1119,7 @@ __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_con
     if (fits) {
         if (warp < 8) {
             const float* list = s_list + warp * kListCap;
-            float tau = -1.0f, lo = -1.0f, hi = 0.0f;
+            float tau = s_low[warp], lo = tau, hi = 0.0f;
             for (int it = 0; it < 60; ++it) {
                 float f = 0.0f, df = 0.0f;
                 for (int i = lane; i < mine; i += 32) gain(list[i], tau, f, df);
@@ -1102,7 +1133,7 @@ __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_con
             if (lane == 0) s_tau[warp] = tau;
         }
     } else {
-        float tau[2] = {-1.0f, -1.0f}, lo[2] = {-1.0f, -1.0f}, hi[2] = {0.0f, 0.0f};
+        float tau[2] = {low0, low1}, lo[2] = {low0, low1}, hi[2] = {0.0f, 0.0f};
         for (int it = 0; it < 60; ++it) {
             float f[2] = {0.0f, 0.0f}, df[2] = {0.0f, 0.0f};
             each([&](float4 y) {
