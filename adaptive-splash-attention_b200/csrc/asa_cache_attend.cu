@@ -23,8 +23,8 @@
 // maxima, weights, products); 16 warps an SM at 128 registers each cover that, and
 // keeping the next tile's products in registers as well was slower (it spilled).
 // Below a few thousand tokens the chain itself is what is left: 8 us for 100 tokens.
-// Entmax, 8 sequences of 32768, 8 key heads: scores 42 us (168 MB of keys in, 67 MB of
-// scores out), thresholds 18, values 18 of which most is finding the few tiles
+// Entmax, 8 sequences of 32768, 8 key heads: scores 44 us (168 MB of keys in, 34 MB of
+// scores out), thresholds 14, values 18 of which most is finding the few tiles
 // that have weight.
 //
 // Arithmetic.  A code 0..15 in an fp16 half is the subnormal n * 2^-24, and in

@@ -20,7 +20,7 @@
 //
 // Measured, 32 heads over 8 key heads, 8192 tokens, d 128: 512 query tokens (66.6 GFLOP)
 // 122 us, 545 TFLOP/s; of 4 sequences 461 us, 578 (0.35 of cuBLAS); d 64, 2048 tokens
-// (120 GFLOP) 361 us, 333.  A tile takes 1.7 us, of which the products are 0.8: the
+// (120 GFLOP) 361 us, 333.  A tile takes 1.7 us, of which the products are 0.75: the
 // exponentials and the conversion of codes, which do not depend on d and on the rows
 // respectively, take the SM's other issue slots.  Starting and ending an item is some 10 us.
 //
