@@ -17,7 +17,7 @@
 //
 // What it reads bounds it: 1.25 d bytes a token and key head, against 4 d operations
 // a query head.  Two sequences of 131072 tokens, 4 key heads of 8 query heads, d 128
-// (168 MB) take 51 us with the join, 3.3 TB/s: 33 us of that go by the tokens, 5.0 TB/s
+// (168 MB) take 52 us with the join, 3.2 TB/s: 33 us of that go by the tokens, 5.0 TB/s
 // or 0.78 of a copy's rate, the rest is starting, the warps' and the runs' joins.  A tile
 // is some 1.6 us of a warp, most of it waiting on its own chain (codes, products,
 // maxima, weights, products); 16 warps an SM at 128 registers each cover that, and
@@ -38,7 +38,10 @@
 // output to bf16 has 8); its products with the values' scales are taken as the
 // rounded product and the rest, two products of the codes, so that codes and
 // offsets are weighted by the same P and a value near zero, a difference of the
-// two, is not disturbed by more than its own size.  A row's largest P times
+// two, is not disturbed by more than its own size.  There the codes are brought to
+// n * 2^-9 first: the tensor cores align a product of a subnormal by the least normal
+// exponent, and cut what lies ten bits further up than need be (a value near zero
+// under a weight near one was off by 2^-16 of its offset).  Scores have room for that.  A row's largest P times
 // the scales starts near 2^4 and may grow to 2^14.5 before its reference is moved: a
 // running exponent fits P to the scales, so that small ones stay clear of fp16's
 // subnormals and large ones do not overflow.  Sums, maxima and
@@ -51,6 +54,7 @@ namespace {
 
 constexpr int kTile = 2;              // blocks of a tile
 constexpr int kStages = 2;            // tiles a warp has in flight
+constexpr uint32_t kUp15 = 0x78007800u, kUp11 = 0x68006800u;   // fp16 pairs: 2^15, 2^11
 constexpr int kLeast = -8;            // weights are raised for small scales by 2^8 at most
 // Plan::item_cost.  Measured: 48 ragged sequences 57.6 us with 8, 50.4 with 12, 48.5 with 16;
 // three guesses of five short ones 32.9, 32.2, 33.7; listed pages (items of one size) 41.8 with
@@ -761,14 +765,22 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                             const uint32_t pick = k & 1 ? 0x7632u : 0x5410u;
                             const uint32_t x0 = __byte_perm(ca[k >> 1], cb[k >> 1], pick), x8 = x0 >> 8;
                             const uint32_t y0 = __byte_perm(cc[k >> 1], cd[k >> 1], pick), y8 = y0 >> 8;
+                            uint32_t c[2][4];         // the codes times 2^-9
+#pragma unroll
+                            for (int e = 0; e < 2; ++e) {
+                                const uint32_t x = e ? x8 : x0, y = e ? y8 : y0;
+                                c[e][0] = hmul2(x & 0x000f000fu, kUp15), c[e][1] = hmul2(x & 0x00f000f0u, kUp11);
+                                c[e][2] = hmul2(y & 0x000f000fu, kUp15), c[e][3] = hmul2(y & 0x00f000f0u, kUp11);
+                            }
 #pragma unroll
                             for (int nt = 0; nt < NT; ++nt) {
                                 const uint32_t b0 = hmul2(pb[i][nt][0], sp[i][k][0]), b1 = hmul2(pb[i][nt][1], sp[i][k][1]);
                                 const uint32_t e0 = hrest2(pb[i][nt][0], sp[i][k][0], b0), e1 = hrest2(pb[i][nt][1], sp[i][k][1], b1);
-                                mma(o[nt][2 * k], x0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x000f000fu, y0 & 0x00f000f0u, b0, b1);
-                                mma(o[nt][2 * k + 1], x8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x000f000fu, y8 & 0x00f000f0u, b0, b1);
-                                mma(o[nt][2 * k], x0 & 0x000f000fu, x0 & 0x00f000f0u, y0 & 0x000f000fu, y0 & 0x00f000f0u, e0, e1);
-                                mma(o[nt][2 * k + 1], x8 & 0x000f000fu, x8 & 0x00f000f0u, y8 & 0x000f000fu, y8 & 0x00f000f0u, e0, e1);
+#pragma unroll
+                                for (int e = 0; e < 2; ++e) {
+                                    mma(o[nt][2 * k + e], c[e][0], c[e][1], c[e][2], c[e][3], b0, b1);
+                                    mma(o[nt][2 * k + e], c[e][0], c[e][1], c[e][2], c[e][3], e0, e1);
+                                }
                             }
                         }
                     }
@@ -813,12 +825,12 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                                 float top = sm.m[0][row];
 #pragma unroll
                                 for (int w = 1; w < W; ++w) top = fmaxf(top, sm.m[w][row]);
-                                const float f = exp2_fast(m[nt][e] - top), k0 = 16777216.0f * f, k1 = 1048576.0f * f;   // codes count 2^-24 and 2^-20
+                                const float f = exp2_fast(m[nt][e] - top), k0 = 512.0f * f;   // codes count 2^-9
 #pragma unroll
                                 for (int k = 0; k < NG; ++k) {
                                     const float z = __shfl_sync(~0u, oz[nt][e], 4 * k + t) * f;
-                                    float4 y = make_float4(fmaf(o[nt][2 * k][e], k0, z), fmaf(o[nt][2 * k][e + 2], k1, z),
-                                                           fmaf(o[nt][2 * k + 1][e], k0, z), fmaf(o[nt][2 * k + 1][e + 2], k1, z));
+                                    float4 y = make_float4(fmaf(o[nt][2 * k][e], k0, z), fmaf(o[nt][2 * k][e + 2], k0, z),
+                                                           fmaf(o[nt][2 * k + 1][e], k0, z), fmaf(o[nt][2 * k + 1][e + 2], k0, z));
                                     float4* dst = &sm.o[warp % H][row][8 * k + r];
                                     if (half == 0) {
                                         const float4 u = *dst;
