@@ -56,10 +56,10 @@ constexpr int kTile = 2;              // blocks of a tile
 constexpr int kStages = 2;            // tiles a warp has in flight
 constexpr uint32_t kUp15 = 0x78007800u, kUp11 = 0x68006800u;   // fp16 pairs: 2^15, 2^11
 constexpr int kLeast = -8;            // weights are raised for small scales by 2^8 at most
-// Plan::item_cost.  Measured: 48 ragged sequences 57.6 us with 8, 50.4 with 12, 48.5 with 16;
-// three guesses of five short ones 32.9, 32.2, 33.7; listed pages (items of one size) 41.8 with
-// 8, 44.8 with 12, 46.2 with 4.
-constexpr int kItemCost = 12, kListedCost = 8;
+// Plan::item_cost.  Measured: 48 ragged sequences of up to 8192 tokens 57.7 us with 8, 50.8 with
+// 12, 48.8 with 16, 49.1 with 20, 52.1 with 28; 12 of up to 16384 42.8, 36.8, 35.6, 35.6, 36.3;
+// listed pages (items of one size) 41.8 with 8, 44.8 with 12, 46.2 with 4.
+constexpr int kItemCost = 16, kListedCost = 8;
 constexpr int kSegments = 32;         // segments a CTA lines up at a time
 
 enum Mode { kSoftmax = 0, kScores = 1, kValues = 2 };
@@ -1226,6 +1226,12 @@ Plan make_plan(const Shape& s, int keep) {
     const int64_t whole = ceil_div(items * p.cluster, slots) * ceil_div(p.cap, p.cluster * warps);
     const int64_t runs = items * p.cap * (keep ? 4 : 3) / (4 * slots * warps) + 5;
     p.split = items < 8 * slots && whole > runs;      // (many items even out, and runs count them all)
+    // The values of an entmax row are those of few tiles: taken to be a quarter at most,
+    // items that fill the SMs at once are left whole more often, and need no join (with
+    // all three kernels, 8 sequences of 32768 tokens, 8 key heads, 74.2 us, 77.5 with the
+    // values cut as the scores; 32 of 4096 73.5, 76.4; but 1 of 32768, 64 CTAs, 77.2, 75.8).
+    const bool fill = items * p.cluster <= slots && 2 * items * p.cluster > slots;
+    p.values = p.split && s.alpha != 1.0f && fill && whole <= 4 * runs ? p.cluster : 0;
     if (p.split) p.cluster = 1;
     p.tile = kTile * kBlock;
     p.item_cost = keep ? kListedCost : kItemCost;
@@ -1290,7 +1296,14 @@ cudaError_t attend_as(const Args& a, cudaStream_t st) {
         e = allow_shared(threshold_kernel<NT>, kTauSmem, allowed);
         if (e != cudaSuccess) return e;
         e = launch(threshold_kernel<NT>, (unsigned)(items * NT), kTauThreads, kTauSmem, st, a);
-        if (e == cudaSuccess) e = launch_walk<D, NT, kValues>(a, st);
+        if (e != cudaSuccess) return e;
+        if (a.p.values) {
+            Args v = a;
+            v.p.split = 0;
+            v.p.cluster = a.p.values;
+            return launch_walk<D, NT, kValues>(v, st);
+        }
+        e = launch_walk<D, NT, kValues>(a, st);
     }
     if (e != cudaSuccess || !a.p.split) return e;
     // eight warps share a row's parts where items are few (2 sequences of 131072 tokens, 4

@@ -23,6 +23,7 @@ struct Plan {
     int cap;                          // tiles an item can have at most
     int split;                        // items are cut into equal runs (else one cluster an item)
     int cluster;                      // CTAs of an item's cluster
+    int values;                       // entmax: such CTAs for the values, where only the scores are cut (else 0)
     int vec;                          // q rows may be read 16 bytes at a time
     int page_shift;                   // log2 of the blocks of a page
     int tile;                         // tokens of a tile
