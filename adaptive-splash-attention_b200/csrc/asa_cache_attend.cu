@@ -901,7 +901,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
         if (!a.p.split) break;
     }
     // A wait gave up: nothing of this CTA may be in flight when it ends.  The last
-    // phase of a stage is this round's before stage_out, else the round's before.
+    // phase of a stage is this turn's of the ring before stage_out, else the last turn's.
     if (lost)
         for (int i = 0; i < kStages; ++i) sm100::mbar_drain(&sm.full[warp][i], i < stage_out ? parity : parity ^ 1u);
 }
