@@ -704,6 +704,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
 #pragma unroll
                             for (int e = 0; e < 2; ++e) {
                                 float by = (float)(up - lift);     // what the reference rises by
+                                const bool none = MODE == kSoftmax && room[nt][e] == -INFINITY;   // no key of it seen yet
                                 if constexpr (MODE == kSoftmax) {
                                     float top = fmaxf(fmaxf(v[0][nt][e], v[0][nt][e + 2]), fmaxf(v[1][nt][e], v[1][nt][e + 2]));
                                     top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
@@ -716,7 +717,8 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
 #pragma unroll
                                     for (int i = 0; i < kTile; ++i) v[i][nt][e] -= by, v[i][nt][e + 2] -= by;
                                 }
-                                f[e] = exp2_fast(-by);
+                                // (a first reference may lie far below 0: nothing is summed yet that it could scale)
+                                f[e] = none ? 1.0f : exp2_fast(-by);
                                 m[nt][e] += by;
                                 oz[nt][e] *= f[e];
                             }
