@@ -399,9 +399,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 top = fmaxf(top, sm.row[b][half ^ 1][row]);
                 if (__any_sync(~0u, top > room)) {    // (the same in both halves' warps)
                     float by = 0.0f;
+                    const bool none = room == -INFINITY;      // no key of the row seen yet
                     if (top > room) by = top, room = kMost;   // the largest weight 1: fp16 has room below too
                     m += by;
-                    const float f = exp2_fast(-by);
+                    // (a first reference may lie far below 0: nothing is summed yet that it could scale)
+                    const float f = none ? 1.0f : exp2_fast(-by);
                     l2.x *= f, l2.y *= f;
 #pragma unroll
                     for (int c = 0; c < 2; ++c)

@@ -122,3 +122,51 @@ def test_listed_pages_far_below(cuda, d, P, level):
     o = sa().cache_attention(q, cache, dev(table), dev(lengths), pages=dev(lists))
     check_attention(o, q, seqs, lengths, P, 1.0, d ** -0.5, lists)
     check_one_key(num(o)[1, 0, :G], seqs[1][1][0, P: P + 1].repeat(G, 0))
+
+
+# ---- chunks of prompts -------------------------------------------------------------
+@pytest.mark.parametrize("level", LEVELS)
+@pytest.mark.parametrize("d,P", [(64, 16), (64, 128), (128, 64)])
+@pytest.mark.parametrize("T,G,lengths,tokens", [
+    (64, 1, [64, 64], 0),                    # a prompt: its first token sees one key
+    (40, 2, [300, 39], 0),                   # and one that sees none before it
+    (64, 3, [2000, 65], 0),
+    (64, 1, [700, 64], 32768),               # cut into equal runs
+])
+def test_chunks_far_below(cuda, d, P, T, G, lengths, tokens, level):
+    cache, table, seqs = made(lengths, 1, d, P, level, seed=6)
+    q = asks(2, T, G, d, level)
+    o = sa().cache_attention(q, cache, dev(widened(table, tokens // P)), dev(lengths))
+    assert torch.isfinite(o).all() and not o[1, : max(0, T - lengths[1])].any()
+    for b, n in enumerate(lengths):
+        if 0 <= T - n < T:
+            check_one_key(num(o)[b, T - n], seqs[b][1][0, :1].repeat(G, 0))
+    assert sa().device_error() == 0
+
+
+@pytest.mark.parametrize("level", LEVELS)
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("tokens", [0, 32768])
+def test_chunks_whose_first_pages_cannot_be_read(cuda, d, tokens, level):
+    """A row's first keys come with a later tile, its output already under way."""
+    P, T, n = 64, 64, 900
+    cache, table, seqs = made([n], 1, d, P, level, seed=7)
+    bad = widened(table, tokens // P)
+    bad[0, :3] = -1
+    q = asks(1, T, 2, d, level)
+    o = sa().cache_attention(q, cache, dev(bad), dev([n]))
+    sa().device_error()
+    seen = np.arange(3, -(-n // P), dtype=np.int32)
+    check_attention(o, q, seqs, [n], P, 1.0, d ** -0.5, np.broadcast_to(seen, (1, T, 1, len(seen))))
+
+
+@pytest.mark.parametrize("level", LEVELS)
+@pytest.mark.parametrize("d", [64, 128])
+def test_chunk_tiles_far_below_beside_others(cuda, d, level):
+    pick = np.random.RandomState(0).rand(16) < 0.4
+    cache, table, seqs = made([1800], 1, d, 64, level, seed=8,
+                              blocks=lambda b, n: np.nonzero(pick[np.arange(n) // 128])[0])
+    q = asks(1, 70, 1, d, level)
+    for pages in (0, 512):
+        o = sa().cache_attention(q, cache, dev(widened(table, pages)), dev([1800]))
+        check_attention(o, q, seqs, [1800], 64, 1.0, d ** -0.5)
