@@ -475,14 +475,13 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
             const auto& mine_rows = sm.rows[sg & 1];
             const int pos_hi = mine_rows.pos[rows - 1], pos_lo = mine_rows.pos[0];   // rows stand in order
             uint32_t qf[NT][NG][4], qz[NT];
-            float rf[NT][2];                          // scores: the factor of rows 2t, 2t + 1; values: their thresholds
+            float rf[NT][2];                          // the factor of rows 2t, 2t + 1's scores
             float m[NT][2], room[NT][2];              // references, and how far above them a score may lie (-inf: unset)
             float oz[NT][4], o[NT][2 * NG][4];        // oz: by group the offsets' sums, and the weights'
             // log2 by which weights are lowered for large scales (raised for small ones), and the
             // fp16 scale 2^(lift + 1) that this allows
             int lift = MODE == kSoftmax ? kLeast : 0;
             uint32_t s_most = (uint32_t)(lift + 16) << 10;
-            const float* tau = a.w.tau + item_no * ROWS;
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
                 if constexpr (MODE != kValues) {
@@ -490,10 +489,10 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                     for (int i = 0; i < 4 * NG; ++i) qf[nt][i / 4][i % 4] = mine_rows.q[nt][i][lane];
                     qz[nt] = mine_rows.q[nt][4 * NG][lane];
                 }
-                const float2 f2 = MODE == kValues ? *reinterpret_cast<const float2*>(tau + 8 * nt + 2 * t)
-                                                  : *reinterpret_cast<const float2*>(&mine_rows.factor[8 * nt + 2 * t]);
-                rf[nt][0] = f2.x;
-                rf[nt][1] = f2.y;
+                if constexpr (MODE != kValues) {
+                    const float2 f2 = *reinterpret_cast<const float2*>(&mine_rows.factor[8 * nt + 2 * t]);
+                    rf[nt][0] = f2.x, rf[nt][1] = f2.y;
+                }
                 m[nt][0] = m[nt][1] = MODE == kSoftmax ? 0.0f : -14.0f;   // (entmax weights are at most 1)
                 room[nt][0] = room[nt][1] = -INFINITY;
 #pragma unroll
@@ -608,14 +607,19 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                     if constexpr (MODE == kValues) {
                         const int64_t place = item_no * a.p.cap + info.tile;
 #pragma unroll
-                        for (int i = 0; i < kTile; ++i)
+                        for (int nt = 0; nt < NT; ++nt) {
+                            // rows 2t, 2t + 1: the largest x, and the threshold relative to it
+                            const float4 edge = __ldg(reinterpret_cast<const float4*>(a.w.edge + item_no * ROWS + 8 * nt + 2 * t));
 #pragma unroll
-                            for (int nt = 0; nt < NT; ++nt) {
+                            for (int i = 0; i < kTile; ++i) {
                                 float4 y = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
                                 if (8 * nt + 2 * t < rows) y = a.w.score[((place * kTile + i) * NT + nt) * 32 + 8 * t + r];
-                                v[i][nt][0] = y.x - rf[nt][0], v[i][nt][1] = y.y - rf[nt][1];
-                                v[i][nt][2] = y.z - rf[nt][0], v[i][nt][3] = y.w - rf[nt][1];
+                                // (close to the largest the first difference is exact, and so keeps what
+                                // the threshold's distance from it, 1e-9 and less among many ties, is made of)
+                                v[i][nt][0] = (y.x - edge.x) - edge.y, v[i][nt][1] = (y.y - edge.z) - edge.w;
+                                v[i][nt][2] = (y.z - edge.x) - edge.y, v[i][nt][3] = (y.w - edge.z) - edge.w;
                             }
+                        }
                     } else {
                         each([&](int i, int nt, int e) { v[i][nt][e] = fmaf(v[i][nt][e], rf[nt][e & 1], -m[nt][e & 1]); });
                         if (!whole) mask();
@@ -926,6 +930,9 @@ constexpr int kListCap = 1024;        // of a row, closed up
 // overflowed now and then), with it 80; three guesses of 2000 tokens 24.0 without, 25.4 with.
 constexpr int kBoundSteps = 4;
 constexpr int kPart = 13;             // of a row and lane (odd: no bank twice)
+// A threshold lies n^-(alpha-1) below n equal largest x: at alpha 3 and 1500 of them 4e-7, less than
+// fp32 tells apart at x = 20.  So it is held relative to the largest x, and found to this part of itself.
+constexpr float kDone = 4e-7f;
 constexpr int kTauSmem = (kTileList + 8 * kListCap + 8 * kTauWarps * 8 * kPart) * 4;
 
 template <int NT>
@@ -944,8 +951,9 @@ __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_con
     const int u = (int)(item_no / per), tile = (int)(item_no % per) % a.p.tiles;
     const int rows = min(8, a.p.R - tile * ROWS - 8 * nt);
     float* tau_out = a.w.tau + item_no * ROWS + 8 * nt;
+    float2* edge_out = a.w.edge + item_no * ROWS + 8 * nt;
     if (rows <= 0) {
-        if (tid < 8) tau_out[tid] = INFINITY;
+        if (tid < 8) tau_out[tid] = INFINITY, edge_out[tid] = make_float2(0.0f, INFINITY);
         return;
     }
     const int nb = unit_tiles(a, u);
@@ -1126,7 +1134,7 @@ __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_con
         const float next = tau + (f - 1.0f) / df;
         const bool inside = next >= lo && next <= hi;
         const float to_ = inside ? next : 0.5f * (lo + hi);
-        const bool end = fabsf(to_ - tau) <= 1e-7f || hi - lo <= 1e-7f;
+        const bool end = fminf(fabsf(to_ - tau), hi - lo) <= kDone * fabsf(to_);
         tau = to_;
         return end;
     };
@@ -1180,8 +1188,10 @@ __global__ void __launch_bounds__(kTauThreads) threshold_kernel(const __grid_con
     }
     __syncthreads();
     if (tid < 8) {
-        const float y = s_top[tid];
-        tau_out[tid] = y == -INFINITY ? INFINITY : y + s_tau[tid];   // (NaN where a score is)
+        const float y = s_top[tid];                   // (NaN where a score is)
+        const bool none = y == -INFINITY;
+        tau_out[tid] = none ? INFINITY : __fadd_rd(y, s_tau[tid]);
+        edge_out[tid] = none ? make_float2(0.0f, INFINITY) : make_float2(y, s_tau[tid]);
     }
 }
 
@@ -1266,6 +1276,7 @@ size_t lay_out(const Shape& s, const Plan& p, void* base, Space* w) {
         x.score = (float4*)take((size_t)items * p.cap * kTile * nt * 512);
         x.top = (float*)take((size_t)items * p.cap * rows * 4);
         x.tau = (float*)take((size_t)items * rows * 4);
+        x.edge = (float2*)take((size_t)items * rows * 8);
     }
     if (w) *w = x;
     return at;

@@ -38,7 +38,8 @@ struct Space {
     float* part_ml;                   // [2 * CTAs][2][rows]
     float4* score;                    // [items][cap][2][NT][32]
     float* top;                       // [items][cap][8 NT]
-    float* tau;                       // [items][8 NT]
+    float* tau;                       // [items][8 NT] at or just below the thresholds: by these tiles are chosen
+    float2* edge;                     // [items][8 NT] a row's largest x, and its threshold relative to that
 };
 
 struct Args {
