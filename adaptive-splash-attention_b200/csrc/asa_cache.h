@@ -14,7 +14,7 @@
 namespace asa {
 
 void note_launch(int n = 1);
-int* device_error_word();              // asa_capi.cu
+int* cache_error_word();               // asa_capi.cu
 int cuda_status_of(cudaError_t e);
 void* profile_open(const char* label, cudaStream_t st);
 void profile_close(void* scope);

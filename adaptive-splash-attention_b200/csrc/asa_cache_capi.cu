@@ -98,7 +98,7 @@ int asa_cache_write(const asa_cache_params* p, const void* K, const void* V, con
     Scope ps("cache_write", st);
     return asa::cuda_status_of(asa::cache::write(s, K, V, strides(k_strides), strides(v_strides),
                                                  (uint8_t*)pool, (int8_t*)bounds, block_table, start,
-                                                 count, asa::device_error_word(), st));
+                                                 count, asa::cache_error_word(), st));
 }
 
 int asa_cache_read(const asa_cache_params* p, const void* pool, const int32_t* block_table,
@@ -112,7 +112,7 @@ int asa_cache_read(const asa_cache_params* p, const void* pool, const int32_t* b
     cudaStream_t st = (cudaStream_t)stream;
     Scope ps("cache_read", st);
     return asa::cuda_status_of(asa::cache::read(s, (const uint8_t*)pool, block_table, start, count, K, V,
-                                                asa::device_error_word(), st));
+                                                asa::cache_error_word(), st));
 }
 
 int asa_cache_bounds(const asa_cache_params* p, const void* bounds, const int32_t* pages, int n,
@@ -127,7 +127,7 @@ int asa_cache_bounds(const asa_cache_params* p, const void* bounds, const int32_
     cudaStream_t st = (cudaStream_t)stream;
     Scope ps("cache_bounds", st);
     return asa::cuda_status_of(asa::cache::read_bounds(s, (const int8_t*)bounds, pages, n, upper, lower,
-                                                       asa::device_error_word(), st));
+                                                       asa::cache_error_word(), st));
 }
 
 int asa_cache_select(const asa_cache_params* p, const void* Q, const int64_t q_strides[3],
@@ -148,7 +148,7 @@ int asa_cache_select(const asa_cache_params* p, const void* Q, const int64_t q_s
     Scope ps("cache_select", st);
     return asa::cuda_status_of(asa::cache::select(s, Q, strides(q_strides), (const int8_t*)bounds,
                                                   block_table, lengths, keep, pages, ws,
-                                                  asa::device_error_word(), st));
+                                                  asa::cache_error_word(), st));
 }
 
 int asa_cache_attention(const asa_cache_params* p, const void* Q, const int64_t q_strides[3],
@@ -169,7 +169,7 @@ int asa_cache_attention(const asa_cache_params* p, const void* Q, const int64_t 
     Scope ps(s.alpha == 1.0f ? "cache_attention" : "cache_entmax", st);
     return asa::cuda_status_of(asa::cache::attend(s, Q, strides(q_strides), (const uint8_t*)pool,
                                                   block_table, lengths, pages, keep, O, ws,
-                                                  asa::device_error_word(), st));
+                                                  asa::cache_error_word(), st));
 }
 
 }  // extern "C"

@@ -44,7 +44,9 @@ cudaError_t tc_backward(const Shape& s, const void* Q, const void* K, const void
                         cudaStream_t st, int stages);
 }  // namespace asa
 
-__device__ int g_asa_error;
+// The error words: the training operators', whose kernels take any value for a wait that
+// gave up, and the cache's, which also records what it did not read or write.
+__device__ int g_asa_error[2];
 
 namespace {
 std::atomic<long long> g_launches{0};
@@ -224,7 +226,10 @@ int cuda_status(cudaError_t e) {
 
 // The same services for the cache's entry points (asa_cache_capi.cu).
 namespace asa {
-int* device_error_word() { return error_word(); }
+int* cache_error_word() {
+    int* w = error_word();
+    return w ? w + 1 : nullptr;
+}
 int cuda_status_of(cudaError_t e) { return cuda_status(e); }
 void* profile_open(const char* label, cudaStream_t st) {
     return g_prof.on ? new (std::nothrow) ProfScope(label, st) : nullptr;
@@ -549,12 +554,13 @@ int asa_device_error(asa_stream_t stream, int* code) {
     int* w = error_word();
     if (!w) return ASA_ERR_CUDA;
     cudaStream_t st = (cudaStream_t)stream;
-    int v = 0;
-    cudaError_t e = cudaMemcpyAsync(&v, w, sizeof(int), cudaMemcpyDeviceToHost, st);
+    int v[2] = {0, 0};
+    cudaError_t e = cudaMemcpyAsync(v, w, sizeof(v), cudaMemcpyDeviceToHost, st);
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-    if (e == cudaSuccess) e = cudaMemsetAsync(w, 0, sizeof(int), st);
+    const int which = v[0] ? 0 : 1;       // the other word stays for the next call
+    if (e == cudaSuccess) e = cudaMemsetAsync(w + which, 0, sizeof(int), st);
     if (e == cudaSuccess) e = cudaStreamSynchronize(st);
-    *code = v;
+    *code = v[which];
     return cuda_status(e);
 }
 

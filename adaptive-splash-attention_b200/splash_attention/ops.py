@@ -231,8 +231,9 @@ def scrub_(x):
 
 
 def device_error(device=None):
-    """Read and clear the device error word (bounded waits that ran out).
-    Synchronises the current stream."""
+    """Read and clear the device error word (bounded waits that ran out) or, where
+    that holds nothing, the cache operators' own (also places they did not read or
+    write).  Synchronises the current stream."""
     code = ctypes.c_int()
     with torch.cuda.device(device):
         L.check(L.lib().asa_device_error(_stream(), ctypes.byref(code)), "asa_device_error")

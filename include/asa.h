@@ -230,8 +230,9 @@ int asa_stable_backward(const asa_params* p, const void* Q, const void* K, const
  * A sequence's positions at or past table_width * page_size, negative ones, and
  * pages outside the pool are neither read nor written; their keys are not seen.
  * Reading or writing such a position, or meeting such a page, records
- * ASA_ERR_INVALID in the device error word (a length past the table's end does
- * not: the keys there are just not seen).  d: 32, 64, 96 or 128.
+ * ASA_ERR_INVALID in the cache's error word, which asa_device_error reads (a
+ * length past the table's end does not: the keys there are just not seen).  No
+ * other operator is affected by it.  d: 32, 64, 96 or 128.
  * pool and bounds must be 16-byte aligned.  Strides are in elements; the
  * innermost dimension is contiguous. */
 #define ASA_CACHE_BOUNDS_PAD 16
@@ -306,12 +307,13 @@ int asa_cache_attention(const asa_cache_params* p, const void* Q, const int64_t 
 int asa_scrub(int dtype, void* x, size_t n, void* ws, asa_stream_t stream);
 
 /* Reads (and clears) the device error word the kernels set when a bounded
- * wait runs out.  Synchronises the stream.  *code is 0 when no error. */
+ * wait runs out, or, where that holds nothing, the cache operators' own.
+ * Synchronises the stream.  *code is 0 when neither holds an error. */
 int asa_device_error(asa_stream_t stream, int* code);
 
-/* Enqueues on `stream` a copy of the device error word into *host_word
- * (pinned host memory, for the copy to stay asynchronous) without clearing
- * it or synchronising: a caller checks the value after a later
+/* Enqueues on `stream` a copy of the device error word (the cache operators'
+ * own is not among it) into *host_word (pinned host memory, for the copy to
+ * stay asynchronous) without clearing it or synchronising: a caller checks the value after a later
  * synchronisation point and then reads and clears the word with
  * asa_device_error.  No counterpart in the reference, whose host launchers
  * synchronise and raise after every call (CUDA_CHECK, :24-27). */
