@@ -12,9 +12,13 @@
 // are double-buffered, so that conversion, softmax and products of three tiles
 // overlap.
 //
-// fp16 is chosen for all operands: a code times its scale plus its offset, both
-// fp16, rounds to 11 bits there (bf16 would keep 8), its subnormals hold the
-// smallest values exactly, and P keeps 11 bits as well.  A row's reference moves only
+// fp16 is chosen for all operands.  A key is (c + n s) + (z - c), c = -7.5 s: the first
+// part, of the size of its group's spread, rounds to fp16's 11 bits (bf16 would keep 8),
+// a 500th of a code's step at most; the second enters as a product of its own, z and c with
+// the group sums of q in two fp16 halves each, so that an offset far above the
+// scale takes no bits from the codes.  A value is z + n s, rounded once to 11 bits: that
+// error is weighted as the value is, and lies below the output's.  P keeps 11 bits
+// as well.  A row's reference moves only
 // when a weight outgrows it (kTop, kMost); O in tensor memory is then rescaled by the
 // rows' own warps.
 //
@@ -38,6 +42,7 @@ using namespace sm100;
 
 constexpr int kRows = 128, kTokens = 128, kBlocks = kTokens / kBlock;
 constexpr int kBox = 16384;                           // 128 rows of 128 bytes
+constexpr int kEdge = 128 * 32;                       // 128 rows of the offsets' product: two columns of 16 bytes
 constexpr int kWarps = 18, kThreads = kWarps * 32;
 constexpr int kChunkCost = 4;                         // Plan::item_cost
 constexpr int kMaxUnits = 1184;                       // units whose prefix sums a CTA keeps
@@ -56,6 +61,9 @@ struct ChunkSmem {
     alignas(1024) uint8_t q[kTileBytes];
     alignas(1024) uint8_t k[2][kTileBytes];
     alignas(1024) uint8_t v[2][kTileBytes];
+    // rows of 16 fp16: of queries the group sums hi, lo, -hi, -lo; of keys z, z, c, c
+    alignas(128) uint8_t qz[kEdge];
+    alignas(128) uint8_t kz[2][kEdge];
     alignas(128) uint8_t staged[2][2 * kBlocks * block_bytes(D)];
     float row[2][2][kRows];                           // maxima of a tile's halves; sums; queries' maxima
     uint16_t nan[2][D / 32][kBlocks];                 // of a tile some rows see in part: value groups holding a NaN
@@ -116,6 +124,11 @@ __device__ __forceinline__ void values_of(uint32_t w, uint32_t s, uint32_t z, ui
         if constexpr (CLIP) v = __hmin2_nan(v, __float2half2_rn(kF16Max));   // the largest may round past fp16
         out[i] = *reinterpret_cast<const uint32_t*>(&v);
     }
+}
+// -7.5 s, and no less than fp16's least: what a key's codes are about the middle of.
+__device__ __forceinline__ uint32_t middle_of(uint32_t s) {
+    const __half2 c = __hmax2_nan(__hmul2(*reinterpret_cast<const __half2*>(&s), __float2half2_rn(-7.5f)), __float2half2_rn(-kF16Max));
+    return *reinterpret_cast<const uint32_t*>(&c);
 }
 // Whether some value 15 s + z passes fp16's largest (or is NaN already).
 __device__ __forceinline__ bool passes_largest(uint32_t s, uint32_t z) {
@@ -252,7 +265,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     } else if (warp == 1) {
         // ---- the products -----------------------------------------------------------
         constexpr uint32_t idS = idesc_f16(kRows, kTokens, 0, 0), idV = idesc_f16(kRows, D, 0, 1);
-        const uint64_t dQ = sdesc(smem_u32(sm.q), 16, 1024);
+        const uint64_t dQ = sdesc(smem_u32(sm.q), 16, 1024), dQz = sdesc_plain(smem_u32(sm.qz), kEdge / 2, 128);
         auto k_step = [](int kk) { return (uint64_t)((((kk >> 2) * kBox) + (kk & 3) * 32) >> 4); };
         auto values = [&](uint32_t i, bool first) {   // O += P V of tile i
             const int b = i & 1;
@@ -282,6 +295,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
 #pragma unroll
                     for (int kk = 0; kk < D / 16; ++kk)
                         mma_bf16_ss(tmem + b * 128, dQ + k_step(kk), dK + k_step(kk), idS, kk > 0);
+                    mma_bf16_ss(tmem + b * 128, dQz, sdesc_plain(smem_u32(sm.kz[b]), kEdge / 2, 128), idS, 1);
                     mma_commit(&sm.b.s_full[b]);
                     mma_commit(&sm.b.k_free[b]);
                 }
@@ -306,7 +320,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
         while (next_segment(a, sm.pref, x, x1, g)) {
             const View v = view_of(g);
             const int at = v.row0 + row, pos = position(g.u, at), tq = at / s.G, hq = v.h * s.G + at % s.G;
-            // the queries, a power of two a row (fp16 holds bf16 exactly then), in the keys' order
+            // the queries, a power of two a row (fp16 holds bf16 exactly then, and the group sums,
+            // below 2^15), in the keys' order
             float rf;
             {
                 uint32_t w[NG][2][4];
@@ -337,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 all_rows();
                 big = fmaxf(big, sm.row[0][half ^ 1][row]);
                 const bool bad = sum != sum || !(big < INFINITY);
-                const int up = big == 0.0f || bad ? 0 : 13 - max((int)(__float_as_uint(big) >> 23) - 127, -113);
+                const int up = big == 0.0f || bad ? 0 : 9 - max((int)(__float_as_uint(big) >> 23) - 127, -117);
                 const float f = bad ? NAN : pow2i(up);
                 rf = scalbnf(s.scale * kLog2e, -up);
 #pragma unroll
@@ -356,6 +371,41 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                         *reinterpret_cast<uint4*>(sm.q + (c >> 3) * kBox + row * 128 + (((c & 7) ^ (row & 7)) << 4)) =
                             make_uint4(y[0], y[1], y[2], y[3]);
                     }
+                all_rows();
+                // the sums of half the groups, of the operands as they are
+                uint32_t hi[NP], lo[NP];              // a group a half word
+#pragma unroll
+                for (int p = 0; p < NP; ++p) hi[p] = lo[p] = 0u;
+#pragma unroll
+                for (int j2 = 0; j2 < NP; ++j2) {
+                    const int i = half * NP + j2;
+                    float2 v2 = make_float2(0.0f, 0.0f);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const int c = NG * k + i;
+                        const uint4 y = *reinterpret_cast<const uint4*>(sm.q + (c >> 3) * kBox + row * 128 + (((c & 7) ^ (row & 7)) << 4));
+                        const uint32_t words[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            v2 = __fadd2_rn(v2, __half22float2(*reinterpret_cast<const __half2*>(&words[e])));
+                    }
+                    const float own = v2.x + v2.y;
+                    const __half h = __float2half_rn(own), l = __float2half_rn(own - __half2float(h));
+                    hi[j2 >> 1] |= (uint32_t)__half_as_ushort(h) << (16 * (j2 & 1));
+                    lo[j2 >> 1] |= (uint32_t)__half_as_ushort(l) << (16 * (j2 & 1));
+                }
+                uint8_t* edge = sm.qz + row * 16;
+                if constexpr (NG == 4) {
+                    *reinterpret_cast<uint32_t*>(edge + 4 * half) = hi[0];
+                    *reinterpret_cast<uint32_t*>(edge + 8 + 4 * half) = lo[0];
+                    *reinterpret_cast<uint32_t*>(edge + kEdge / 2 + 4 * half) = hi[0] ^ 0x80008000u;
+                    *reinterpret_cast<uint32_t*>(edge + kEdge / 2 + 8 + 4 * half) = lo[0] ^ 0x80008000u;
+                } else {
+                    uint16_t* at2 = reinterpret_cast<uint16_t*>(edge) + half;
+                    at2[0] = (uint16_t)hi[0], at2[2] = (uint16_t)lo[0];
+                    at2[4] = (uint16_t)(hi[0] ^ 0x8000u), at2[6] = (uint16_t)(lo[0] ^ 0x8000u);
+                    if (half) *reinterpret_cast<uint4*>(edge + kEdge / 2) = make_uint4(0u, 0u, 0u, 0u);
+                }
                 fence_async_smem();
                 all_rows();                           // (also: sm.row may be written again)
                 arrive(sm.b.q_ready);
@@ -534,7 +584,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 wait(sm.b.k_free[st], (j >> 1) ^ 1u);
                 // keys: a lane eight channels of every group, of tokens lane % 8 and 8 on
                 {
-                    uint32_t w[2][NG], sc[2][NP], zo[2][NP];
+                    uint32_t w[2][NG], sc[2][NP], zo[2][NP], mid[2][NP];
                     bool clip = false;
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
@@ -546,7 +596,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                             sc[k][e] = reinterpret_cast<const uint32_t*>(par)[e];
                             zo[k][e] = reinterpret_cast<const uint32_t*>(par)[NP + e];
                             if (!there) sc[k][e] = zo[k][e] = 0u;
-                            clip |= passes_largest(sc[k][e], zo[k][e]);
+                            mid[k][e] = middle_of(sc[k][e]);
+                            clip |= passes_largest(sc[k][e], mid[k][e]);
                         }
                     }
                     auto store = [&](auto clip_c) {
@@ -556,11 +607,20 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                             for (int e = 0; e < NG; ++e) {
                                 const uint32_t pick = e & 1 ? 0x3232u : 0x1010u;
                                 uint32_t y[4];
-                                values_of<decltype(clip_c)::value>(w[k][e], __byte_perm(sc[k][e >> 1], 0u, pick), __byte_perm(zo[k][e >> 1], 0u, pick), y);
+                                values_of<decltype(clip_c)::value>(w[k][e], __byte_perm(sc[k][e >> 1], 0u, pick), __byte_perm(mid[k][e >> 1], 0u, pick), y);
                                 *reinterpret_cast<uint4*>(sm.k[st] + to_k[e] + 8 * k * 128) = make_uint4(y[0], y[1], y[2], y[3]);
                             }
                     };
                     if (__any_sync(~0u, clip)) store(std::true_type{}); else store(std::false_type{});
+                    if (run < 2)                      // the columns z, z and c, c (64: all in the first 16 bytes)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            uint4 y;
+                            if constexpr (NG == 4) y = run ? make_uint4(mid[k][0], mid[k][1], mid[k][0], mid[k][1])
+                                                           : make_uint4(zo[k][0], zo[k][1], zo[k][0], zo[k][1]);
+                            else y = run ? make_uint4(0u, 0u, 0u, 0u) : make_uint4(zo[k][0], zo[k][0], mid[k][0], mid[k][0]);
+                            *reinterpret_cast<uint4*>(sm.kz[st] + run * (kEdge / 2) + (16 * dq + tok + 8 * k) * 16) = y;
+                        }
                 }
                 fence_async_smem();
                 arrive(sm.b.k_ready[st]);

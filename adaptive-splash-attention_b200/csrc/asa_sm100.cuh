@@ -235,6 +235,13 @@ __device__ __forceinline__ uint64_t sdesc(uint32_t saddr, uint32_t lbo_bytes, ui
     return d;
 }
 
+// The same without swizzle, K-major: blocks of 8 rows of 16 bytes; lbo = byte
+// distance between the blocks of neighbouring 16-byte columns, sbo = between
+// those of neighbouring rows.
+__device__ __forceinline__ uint64_t sdesc_plain(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
+    return sdesc(saddr, lbo_bytes, sbo_bytes) & ~((uint64_t)7 << 61);
+}
+
 // Instruction descriptor for kind::f16 with bf16 A/B and fp32 D.
 //   a_mn / b_mn: 1 when that operand is MN-major in shared memory.
 __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N, int a_mn, int b_mn) {

@@ -295,7 +295,10 @@ int asa_cache_select(const asa_cache_params* p, const void* Q, const int64_t q_s
  * see no key are zero, rows of a query holding a NaN or an infinity NaN.  A NaN
  * among the keys a query sees makes its row NaN, one among the values their
  * group's 32 channels (under alpha-entmax surely so only where it has weight);
- * what a query does not see does not reach it. */
+ * what a query does not see does not reach it.  Weights are rounded to 11 bits;
+ * codes enter as they are, but softmax over 64 and more rows (T * heads /
+ * kv_heads, d 64 or 128, no pages) rounds a key's distance from the middle of
+ * its group's codes, and a value, to 11 bits. */
 int asa_cache_attention(const asa_cache_params* p, const void* Q, const int64_t q_strides[3],
                         const void* pool, const int32_t* block_table, const int32_t* lengths,
                         const int32_t* pages, int keep, void* O, void* ws, size_t ws_bytes,
