@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                 }
                 const float hi = __half2float(__float2half_rn(own));
                 out.q[nt][4 * NG][lane] = pack(hi, own - hi);
-                if (t == 0) out.factor[8 * nt + r] = scalbnf(s.scale * (MODE == kSoftmax ? kLog2e : s.alpha - 1.0f), 24 - up);
+                if (t == 0) out.factor[8 * nt + r] = factor_of(s.scale * (MODE == kSoftmax ? kLog2e : s.alpha - 1.0f), 24 - up, kMostFactor);
             }
         };
         if (warp < NT && segs) make_rows(0, warp);

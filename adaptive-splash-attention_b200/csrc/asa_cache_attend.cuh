@@ -14,6 +14,14 @@ constexpr float kLog2e = 1.4426950408889634f;
 // 2^kMost: fp16 holds 65504, and keeps 11 bits of weights down to 2^-14.
 constexpr float kTop = 4.0f, kMost = 14.5f;
 constexpr float kLow = -1.0e30f;      // below any score
+// The most that the factor of a row's products may be (they count 2^-24, at most 2^13; in asa_cache_chunk.cu
+// 1, at most 2^34, and 2^-24 of this factor): scores stay within 2^93, less than -kLow.  Queries of some 1e22
+// and more, by the scale, would have a larger one, which fp32 need not hold (it made NaN of them); with either
+// the largest score takes all, a code's step in such a query's largest channel being 2^40 and more.
+constexpr float kMostFactor = 1.2089258e24f;          // 2^80
+__device__ __forceinline__ float factor_of(float scale, int e, float most) {
+    return fminf(fmaxf(scalbnf(scale, e), -most), most);
+}
 constexpr int kSms = 148;
 
 // How a call's rows are tiled and its work cut.

@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 const bool bad = sum != sum || !(big < INFINITY);
                 const int up = big == 0.0f || bad ? 0 : 9 - max((int)(__float_as_uint(big) >> 23) - 127, -117);
                 const float f = bad ? NAN : pow2i(up);
-                rf = scalbnf(s.scale * kLog2e, -up);
+                rf = factor_of(s.scale * kLog2e, -up, kMostFactor * 5.9604645e-8f);   // 2^56
 #pragma unroll
                 for (int i = 0; i < NG; ++i)
 #pragma unroll

@@ -1,0 +1,35 @@
+"""The 4-bit cache at the ends of what its arguments can hold."""
+import numpy as np
+import pytest
+import torch
+
+from test_cache_gpu import check_attention, dev, filled, num, sa
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("d,T", [(32, 1), (64, 1), (96, 5), (128, 1), (64, 64), (128, 64)])
+@pytest.mark.parametrize("q_scale", [1e33, 1e37])
+def test_queries_near_the_largest_number(cuda, d, T, q_scale):
+    """Softmax is the largest score's alone, whose value is the output (its rounding to bf16, and 2^-11 for
+    values held in 11 bits); alpha-entmax clamps."""
+    H, n, P = 2, 40 + T, 32
+    cache, table, seqs = filled(1, [n], H, d, P, seed=d + T, k_scale=30.0)
+    q = (torch.randn(1, T, 2 * H, d, generator=torch.Generator().manual_seed(5)) * q_scale).bfloat16().cuda()
+    o = num(sa().cache_attention(q, cache, dev(table), dev([n])))
+    assert np.isfinite(o).all()
+    checked = 0
+    for t in range(T):
+        for h in range(2 * H):
+            k, v = (x[h // 2][: n - T + t + 1] for x in seqs[0])
+            s = k @ num(q).astype(np.float64)[0, t, h]
+            best, second = np.sort(s)[-1], np.sort(s)[-2]
+            if best - second < 2.0 ** -8 * np.abs(s).max():   # too near for 32 bits of sums to be certain of
+                continue
+            checked += 1
+            ref = v[s.argmax()]
+            assert (np.abs(o[0, t, h] - ref) <= (2.0 ** -8 + 2.0 ** -11) * np.abs(ref) + 2.0 ** -20 * np.abs(v).max()).all()
+    assert checked > T
+    if T <= 5:
+        e = sa().cache_attention(q, cache, dev(table), dev([n]), alpha=1.5)
+        check_attention(e, q, seqs, [n], P, 1.5, d ** -0.5)
