@@ -59,14 +59,18 @@ void same_device(const Tensor& a, const Tensor& b, const char* name) {
     TORCH_CHECK(a.device() == b.device(), "splash_attention: ", name, " must be on ", a.device());
 }
 
-// Positions, lengths and tables as contiguous int32 on the cache's device.
+// Positions, lengths and tables as contiguous int32 on the cache's device.  Numbers that
+// int32 does not hold become its ends, which lie outside every table and pool, not others.
 Tensor index(const Tensor& t, const Tensor& like, c10::IntArrayRef shape, const char* name) {
     TORCH_CHECK_TYPE(at::isIntegralType(t.scalar_type(), false), "splash_attention: ", name, " must hold integers");
     same_device(like, t, name);
     TORCH_CHECK_VALUE(t.dim() == (int64_t)shape.size(), "splash_attention: ", name, " must have ", shape.size(), " dimensions");
     for (size_t i = 0; i < shape.size(); ++i)
         TORCH_CHECK_VALUE(shape[i] < 0 || t.size(i) == shape[i], "splash_attention: ", name, " has shape ", t.sizes());
-    return t.scalar_type() == at::kInt && t.is_contiguous() ? t : t.to(at::kInt).contiguous();
+    const auto type = t.scalar_type();
+    if (type == at::kInt) return t.contiguous();
+    const bool wide = type == at::kLong || type == at::kUInt32 || type == at::kUInt64;
+    return (wide ? t.to(at::kLong).clamp(INT_MIN, INT_MAX) : t).to(at::kInt).contiguous();
 }
 
 const int32_t* ints(const Tensor& t) { return t.defined() ? t.const_data_ptr<int32_t>() : nullptr; }

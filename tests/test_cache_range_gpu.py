@@ -6,6 +6,7 @@ import torch
 from test_cache_gpu import check_attention, dev, filled, num, sa
 
 pytestmark = pytest.mark.gpu
+INVALID = 1
 
 
 @pytest.mark.parametrize("d,T", [(32, 1), (64, 1), (96, 5), (128, 1), (64, 64), (128, 64)])
@@ -33,3 +34,31 @@ def test_queries_near_the_largest_number(cuda, d, T, q_scale):
     if T <= 5:
         e = sa().cache_attention(q, cache, dev(table), dev([n]), alpha=1.5)
         check_attention(e, q, seqs, [n], P, 1.5, d ** -0.5)
+
+
+def test_indices_past_32_bits(cuda):
+    """Whole numbers that int32 does not hold are not other ones: a page is outside the pool, a length past the table."""
+    H, d, P, n = 2, 64, 16, 100
+    cache, table, seqs = filled(1, [n], H, d, P, seed=2)
+    q = torch.randn(1, 1, 4, d, generator=torch.Generator().manual_seed(8)).bfloat16().cuda()
+    tab = dev(table)
+    sa().device_error()
+    for far in (1 << 32, -(1 << 32), 1 << 40):
+        away = tab.long()
+        away[0, 1] += far
+        o = sa().cache_attention(q, cache, away, dev([n]))
+        assert sa().device_error() == INVALID
+        check_attention(o, q, seqs, [n], P, 1.0, d ** -0.5, np.array([0, 2, 3, 4, 5, 6]).reshape(1, 1, 1, 6).repeat(H, 2))
+    short = tab[:, :3].contiguous()
+    o = sa().cache_attention(q, cache, short, torch.tensor([(1 << 32) + 5], device="cuda"))
+    want = sa().cache_attention(q, cache, short, dev([48]))
+    assert torch.equal(o, want)
+    assert not sa().cache_attention(q, cache, short, torch.tensor([5 - (1 << 32)], device="cuda")).any()
+    before = cache.pool.clone()
+    x = torch.randn(1, 1, H, d).bfloat16().cuda()
+    sa().device_error()
+    sa().cache_write(x, x, cache, tab, torch.tensor([(1 << 32) + 3], device="cuda"))
+    assert torch.equal(cache.pool, before) and sa().device_error() == INVALID
+    lists = torch.tensor([0, 1 << 32], device="cuda").repeat(1, 1, H, 1)
+    o = sa().cache_attention(q, cache, tab, dev([n]), pages=lists)
+    check_attention(o, q, seqs, [n], P, 1.0, d ** -0.5, np.zeros((1, 1, H, 1), np.int32))
