@@ -240,6 +240,22 @@ Tensor attention_cuda(const Tensor& Q, const Tensor& pool, const Tensor& bounds,
     return O;
 }
 
+// Writing, above the kernels: the cache's version counters count it, as autograd and
+// compilers expect of an operator that changes its arguments.
+void write_counted(c10::DispatchKeySet keys, const Tensor& K, const Tensor& V, const Tensor& pool, const Tensor& bounds,
+                   const Tensor& block_table, const Tensor& start, const OptTensor& count) {
+    static const auto op = c10::Dispatcher::singleton()
+                               .findSchemaOrThrow("splash_attention::cache_write", "")
+                               .typed<void(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                           const Tensor&, const OptTensor&)>();
+    {
+        at::AutoDispatchBelowADInplaceOrView guard;
+        op.redispatch(keys & c10::after_ADInplaceOrView_keyset, K, V, pool, bounds, block_table, start, count);
+    }
+    for (const Tensor* t : {&pool, &bounds})
+        if (!t->is_inference()) t->unsafeGetTensorImpl()->bump_version();
+}
+
 void write_meta(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
                 const OptTensor&) {}
 
@@ -301,6 +317,7 @@ TORCH_LIBRARY_IMPL(splash_attention, Autograd, m) {
         m.impl(name, torch::CppFunction::makeFallthrough());
 }
 TORCH_LIBRARY_IMPL(splash_attention, ADInplaceOrView, m) {
-    for (const char* name : {"cache_write", "cache_read", "cache_bounds", "cache_select", "cache_attention"})
+    m.impl("cache_write", TORCH_FN(write_counted));
+    for (const char* name : {"cache_read", "cache_bounds", "cache_select", "cache_attention"})
         m.impl(name, torch::CppFunction::makeFallthrough());
 }
