@@ -104,6 +104,8 @@ size_t select_workspace(const Shape& s);
 cudaError_t select(const Shape& s, const void* Q, Strides qs, const int8_t* bounds, const int32_t* table,
                    const int32_t* lengths, int keep, int32_t* pages, void* ws, int* err, cudaStream_t st);
 
+cudaError_t wait_probe(int naps, int* err, cudaStream_t st);
+
 size_t attend_workspace(const Shape& s, int keep);
 cudaError_t attend(const Shape& s, const void* Q, Strides qs, const uint8_t* pool, const int32_t* table,
                    const int32_t* lengths, const int32_t* list, int keep, void* O, void* ws, int* err,

@@ -374,8 +374,11 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
             }
             const int k = __ffs(there) - 1;
             there &= there - 1;
-            if (lane == k) {                          // the lane that looked it up issues its copies
+            if (lane == k)                            // the lane that looked it up issues its copies
                 sm.info[warp][stage_in] = Info{pos0, pos1, sm.seg[ahead].from + warp + (32 * (c - 1) + k) * W, ahead};
+            // (a lane none of whose waits gave up has seen all that the stage held before; another must not
+            // arm it again, since its last copy may still be awaited)
+            if (lane == k && !lost) {
                 uint8_t* dst = sm.ring[warp][stage_in];
                 uint64_t* bar = &sm.full[warp][stage_in];
                 constexpr int kParts = MODE == kSoftmax ? 2 : 1;
@@ -906,10 +909,9 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
         }
         if (!a.p.split) break;
     }
-    // A wait gave up: nothing of this CTA may be in flight when it ends.  The last
-    // phase of a stage is this turn's of the ring before stage_out, else the last turn's.
+    // A wait gave up: nothing of this CTA may be in flight when it ends
     if (lost)
-        for (int i = 0; i < kStages; ++i) sm100::mbar_drain(&sm.full[warp][i], i < stage_out ? parity : parity ^ 1u);
+        for (int i = 0; i < kStages; ++i) drain(&sm.full[warp][i]);
 }
 
 // ---- the alpha-entmax threshold ----------------------------------------------------
@@ -1327,6 +1329,25 @@ cudaError_t attend_as(const Args& a, cudaStream_t st) {
 }
 
 }  // namespace
+
+// Lane 0 waits, with the kernels' bounded wait, for an arrival that nobody makes; then it
+// completes the barrier itself, so that nothing is pending when the block ends.
+__global__ void wait_probe_kernel(int naps, int* err) {
+    __shared__ uint64_t bar;
+    if (threadIdx.x == 0) {
+        sm100::mbar_init(&bar, 1);
+        sm100::fence_barrier_init();
+        wait_full(&bar, 0, naps, err);
+        sm100::mbar_arrive(&bar);
+    }
+    __syncwarp();
+}
+
+cudaError_t wait_probe(int naps, int* err, cudaStream_t st) {
+    wait_probe_kernel<<<1, 32, 0, st>>>(naps, err);
+    note_launch();
+    return cudaGetLastError();
+}
 
 size_t attend_workspace(const Shape& s, int keep) {
     if (chunk_takes(s, keep)) return chunk_workspace(s);

@@ -96,6 +96,18 @@ __device__ __forceinline__ bool wait_full(uint64_t* bar, uint32_t parity, int na
     return false;
 }
 
+// After a wait gave up: waits for the phase that a barrier is in, a third of a second at most (it may not
+// have been armed).
+__device__ __forceinline__ void drain(uint64_t* bar) {
+    const uint32_t parity = sm100::mbar_test(bar, 0) ? 1u : 0u;
+    for (int i = 0; i < (1 << 14); ++i)
+        if (nap(bar, parity)) return;
+}
+// Whether a wait of the cache's kernels has given up.
+__device__ __forceinline__ bool timed_out(const int* err) {
+    return err && *reinterpret_cast<const volatile int*>(err) == ASA_ERR_DEVICE_TIMEOUT;
+}
+
 __device__ __forceinline__ int unit_tiles(const Args& a, int u) {
     if (a.list) return a.p.cap;
     const long long n = min((long long)max(__ldg(a.lengths + u), 0), (long long)a.s.width * a.s.P);

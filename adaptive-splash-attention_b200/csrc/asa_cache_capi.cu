@@ -13,6 +13,9 @@ using asa::cache::Strides;
 
 bool aligned(const void* p, size_t to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
+// The training kernels' spins, sixteen to a nap (five seconds by default).
+int naps_of(long long spins) { return (int)((spins >> 4) + 1 < (1 << 30) ? (spins >> 4) + 1 : (1 << 30)); }
+
 int check(const asa_cache_params* p, Shape* s, bool queries) {
     if (!p) return ASA_ERR_INVALID;
     if (p->B < 0 || p->T < 0 || p->kv_heads < 1 || p->num_pages < 0 || p->table_width < 0)
@@ -45,9 +48,7 @@ int check(const asa_cache_params* p, Shape* s, bool queries) {
     s->dtype = p->dtype;
     s->scale = p->sm_scale;
     s->alpha = p->alpha;
-    // the training kernels' spins, sixteen to a nap (five seconds by default)
-    const long long spins = p->timeout_spins > 0 ? p->timeout_spins : (1LL << 22);
-    s->naps = (int)((spins >> 4) + 1 < (1 << 30) ? (spins >> 4) + 1 : (1 << 30));
+    s->naps = naps_of(p->timeout_spins > 0 ? p->timeout_spins : (1LL << 22));
     s->rec = asa::cache::record_bytes(p->d, p->page_size);
     return ASA_OK;
 }
@@ -81,6 +82,13 @@ int asa_cache_workspace_bytes(const asa_cache_params* p, int keep, size_t* atten
     if (attend_bytes) *attend_bytes = asa::cache::attend_workspace(s, keep);
     if (select_bytes) *select_bytes = asa::cache::select_workspace(s);
     return ASA_OK;
+}
+
+int asa_cache_wait_probe(long long spins, asa_stream_t stream) {
+    if (spins < 1) return ASA_ERR_INVALID;
+    int* w = asa::cache_error_word();
+    if (!w) return ASA_ERR_CUDA;
+    return asa::cuda_status_of(asa::cache::wait_probe(naps_of(spins), w, (cudaStream_t)stream));
 }
 
 int asa_cache_write(const asa_cache_params* p, const void* K, const void* V, const int64_t k_strides[3],

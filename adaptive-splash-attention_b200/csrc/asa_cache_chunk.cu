@@ -227,7 +227,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
     if (warp == 0) {
         // ---- the tiles' records ---------------------------------------------------
         const int pieces = kTokens / s.P, blocks = s.P / kBlock;       // pages a tile, blocks a page (P <= 128)
-        while (next_segment(a, sm.pref, x, x1, g)) {
+        bool lost = false;                            // a wait gave up: no more is fetched
+        while (!lost && next_segment(a, sm.pref, x, x1, g)) {
             const View v = view_of(g);
             const int32_t* table = a.table + (int64_t)g.u * s.width;
             auto look_up = [&](int i) {               // this lane's page of the i-th tile: its id, -1 where none is to be read
@@ -242,7 +243,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             for (int i = 0; i < v.n; ++i, ++j) {
                 const int id = next, st = j & 1;
                 if (i + 1 < v.n) next = look_up(i + 1);
-                wait(sm.b.staged_free[st], (j >> 1) ^ 1u);
+                // read by all that convert it, and (should one of them have given up) landed
+                lost = !__all_sync(~0u, wait_full(&sm.b.staged_free[st], ((j >> 1) ^ 1u) & 1u, s.naps, a.err) &&
+                                            wait_full(&sm.b.staged_full[st], ((j >> 1) ^ 1u) & 1u, s.naps, a.err));
+                if (lost) break;
                 const uint32_t votes = __ballot_sync(~0u, id >= 0);
                 if (lane == 0) {
                     uint32_t present = 0;
@@ -260,7 +264,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
                 }
             }
         }
-        if (error_set(a.err))                         // a wait may have given up: no copy may outlive the CTA
+        if (lost || timed_out(a.err))                 // no copy may outlive the CTA
             for (uint32_t i = 0; i < 2 && i < j; ++i) mbar_drain(&sm.b.staged_full[(j - 1 - i) & 1], ((j - 1 - i) >> 1) & 1u);
     } else if (warp == 1) {
         // ---- the products -----------------------------------------------------------
@@ -307,7 +311,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_kernel(const __grid_constan
             __syncwarp();
             ++segs;
         }
-        if (lane == 0 && error_set(a.err)) {          // a wait may have given up: let the products finish
+        if (lane == 0 && timed_out(a.err)) {          // a wait gave up: let the products finish
             mma_commit(&sm.b.drain);
             mbar_drain(&sm.b.drain, 0);
         }

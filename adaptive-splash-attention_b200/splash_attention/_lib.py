@@ -26,7 +26,7 @@ SYMBOLS = ("asa_params_default", "asa_workspace_bytes", "asa_resolve_backend", "
            "asa_device_error_async", "asa_wait_probe", "asa_stable_workspace_bytes",
            "asa_stable_forward", "asa_stable_backward", "asa_cache_record_bytes",
            "asa_cache_workspace_bytes", "asa_cache_write", "asa_cache_read", "asa_cache_bounds",
-           "asa_cache_select", "asa_cache_attention")
+           "asa_cache_select", "asa_cache_attention", "asa_cache_wait_probe")
 NOALLOC_SCRATCH_BYTES = 1 << 20
 
 
@@ -110,6 +110,7 @@ def lib():
         L.asa_cache_bounds.argtypes = [cp, vp, vp, ctypes.c_int, vp, vp, vp]
         L.asa_cache_select.argtypes = [cp, vp, i64x3, vp, vp, vp, ctypes.c_int, vp, vp, sz, vp]
         L.asa_cache_attention.argtypes = [cp, vp, i64x3, vp, vp, vp, vp, ctypes.c_int, vp, vp, sz, vp]
+        L.asa_cache_wait_probe.argtypes = [ctypes.c_longlong, vp]
         L.asa_last_cuda_error.argtypes = []
         L.asa_last_cuda_error.restype = ctypes.c_char_p
         for name in SYMBOLS:

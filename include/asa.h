@@ -304,6 +304,11 @@ int asa_cache_attention(const asa_cache_params* p, const void* Q, const int64_t 
                         const int32_t* pages, int keep, void* O, void* ws, size_t ws_bytes,
                         asa_stream_t stream);
 
+/* Self-test of the cache kernels' bounded waits, as asa_wait_probe is of the
+ * others': a wait that nothing ends gives up after `spins` (spins of
+ * timeout_spins) and records ASA_ERR_DEVICE_TIMEOUT in the cache's error word. */
+int asa_cache_wait_probe(long long spins, asa_stream_t stream);
+
 /* The reference's host-side scrub done on the device: NaN -> 0, and if any
  * element is ±Inf the whole tensor is clamped to [-100, 100]
  * (:599-606, :684-697).  ws needs 16 bytes. */

@@ -73,3 +73,28 @@ def test_a_training_timeout_is_not_the_caches(cuda):
         o = sa().cache_attention(q, cache, dev(table), dev(lengths), alpha=alpha)
         assert [sa().device_error(), sa().device_error()] == [TIMEOUT, 0]
         check_attention(o, q, seqs, lengths, 64, alpha, 128 ** -0.5)
+
+
+def test_a_wait_that_gives_up_is_reported(cuda):
+    """The cache's kernels' bounded wait, on a barrier that nobody completes; training and the cache go on."""
+    import ctypes
+    from splash_attention import _lib as L
+    assert sa().device_error() == 0
+    want = step()
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    assert L.lib().asa_cache_wait_probe(0, stream) == INVALID
+    assert L.lib().asa_cache_wait_probe(1000, stream) == 0
+    for _ in range(3):
+        for a, b in zip(step(), want):
+            assert torch.equal(a, b)
+        torch.cuda.synchronize()
+    assert [sa().device_error(), sa().device_error()] == [TIMEOUT, 0]
+    misuse("read")                                            # a time-out is not lost to what came before it
+    assert L.lib().asa_cache_wait_probe(1, stream) == 0
+    assert [sa().device_error(), sa().device_error()] == [TIMEOUT, 0]
+    for T in (1, 70):
+        cache, table, seqs = filled(1, [300], 2, 64, 16, seed=3)
+        q = torch.randn(1, T, 4, 64, generator=torch.Generator().manual_seed(5)).bfloat16().cuda()
+        o = sa().cache_attention(q, cache, dev(table), dev([300]))
+        check_attention(o, q, seqs, [300], 16, 1.0, 64 ** -0.5)
+    assert sa().device_error() == 0
