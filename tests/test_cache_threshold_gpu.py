@@ -99,3 +99,27 @@ def test_clamped_scores_among_lower_ones(cuda, alpha):
         o = num(sa().cache_attention(q, cache, dev(table), dev([n]), sm_scale=1.0 / D, alpha=alpha, pages=pages))
         for row in o[0, 0]:
             check(row, v, (alpha - 1.0) * np.clip(z, -10.0, 10.0), alpha)
+
+
+@pytest.mark.parametrize("tokens", [0, 131072])
+@pytest.mark.parametrize("alpha", [1.5, 2.0, 2.125, 2.25, 2.5, 2.75, 3.0])
+def test_keys_at_the_edge_of_the_support(cuda, alpha, tokens):
+    """A few keys within a tenth of where support ends: above alpha 2 each enters it with infinite slope."""
+    B, n, P = 96, 6, 16
+    g = np.random.RandomState(int(8 * alpha))
+    end = 1.0 / (alpha - 1.0)
+    z = -np.round(end * (0.9 + 0.11 * g.rand(B, n)) * 2048.0) / 2048.0
+    z[:, 0] = 0.0
+    some = 1 + np.arange(B) % (n - 1)                         # keys that take part
+    z = np.where(np.arange(n) <= some[:, None], z, -3.0 * end)
+    z = z.astype(np.float16).astype(np.float64)
+    cache, table = fresh(B, [n] * B, 1, D, P, seed=1)
+    K = torch.as_tensor(z, dtype=torch.float32)[:, :, None, None].expand(B, n, 1, D).cuda()
+    V = (1.0 + torch.randn(B, n, 1, D, generator=torch.Generator().manual_seed(1))).cuda()
+    sa().cache_write(K, V, cache, dev(table), dev(np.zeros(B)))
+    v = F.decode(cache.pool.cpu().numpy(), D, P)[1][table[:, 0], 0, :n]
+    q = torch.ones(B, 1, 2, D, device="cuda").bfloat16()
+    o = num(sa().cache_attention(q, cache, dev(widened(table, tokens // P)), dev([n] * B), sm_scale=1.0 / D, alpha=alpha))
+    for b in range(B):
+        for row in o[b, 0]:
+            check(row, v[b], (alpha - 1.0) * z[b], alpha)
