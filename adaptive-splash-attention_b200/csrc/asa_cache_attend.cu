@@ -41,11 +41,12 @@
 // two, is not disturbed by more than its own size.  There the codes are brought to
 // n * 2^-9 first: the tensor cores align a product of a subnormal by the least normal
 // exponent, and cut what lies ten bits further up than need be (a value near zero
-// under a weight near one was off by 2^-16 of its offset).  Scores have room for that.  A row's largest P times
-// the scales starts near 2^4 and may grow to 2^14.5 before its reference is moved: a
-// running exponent fits P to the scales, so that small ones stay clear of fp16's
-// subnormals and large ones do not overflow.  Sums, maxima and
-// accumulators are fp32.
+// under a weight near one was off by 2^-16 of its offset).  Scores have room for that.  A
+// running exponent e of the largest scale fits P to the scales, so that small ones stay
+// clear of fp16's subnormals and large ones do not overflow: a row's largest P starts at
+// 2^4 (2^(4 - e) for e below 0, and less from e = 8 on) and may grow until P times the scales
+// reach 2^15.5 before its reference is moved.  So P keeps its 11 bits down to 2^-18 of the
+// largest weight, and 2^-13 at the largest scales.  Sums, maxima and accumulators are fp32.
 #include "asa_cache_attend.cuh"
 
 namespace asa {
@@ -56,6 +57,7 @@ constexpr int kTile = 2;              // blocks of a tile
 constexpr int kStages = 2;            // tiles a warp has in flight
 constexpr uint32_t kUp15 = 0x78007800u, kUp11 = 0x68006800u;   // fp16 pairs: 2^15, 2^11
 constexpr int kLeast = -8;            // weights are raised for small scales by 2^8 at most
+constexpr float kRoom = 3.0f;         // log2 of what a row's largest weight may grow by, at least, before its reference moves
 // Plan::item_cost.  Measured: 48 ragged sequences of up to 8192 tokens 57.7 us with 8, 50.8 with
 // 12, 48.8 with 16, 49.1 with 20, 52.1 with 28; 12 of up to 16384 42.8, 36.8, 35.6, 35.6, 36.3;
 // listed pages (items of one size) 41.8 with 8, 44.8 with 12, 46.2 with 4.
@@ -717,7 +719,8 @@ __global__ void __launch_bounds__(W * 32, NT == 1 ? 2 : 3) walk_kernel(const __g
                                     top = fmaxf(top, __shfl_xor_sync(~0u, top, 4));
                                     top = fmaxf(top, __shfl_xor_sync(~0u, top, 8));
                                     top = fmaxf(top, __shfl_xor_sync(~0u, top, 16));
-                                    const float to = top - kTop + (float)up;
+                                    // a large scale leaves less room above, not fewer bits below, down to kRoom
+                                    const float to = top - (up > 0 ? fminf(kTop, kMost - kRoom - (float)up) : kTop - (float)up);
                                     if (room[nt][e] > -INFINITY) by = fmaxf(by, to);
                                     else by = top > -INFINITY ? to : 0.0f;
                                     if (room[nt][e] > -INFINITY || top > -INFINITY) room[nt][e] = kMost - (float)max(up, 0);

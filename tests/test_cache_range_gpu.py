@@ -3,7 +3,8 @@ import numpy as np
 import pytest
 import torch
 
-from test_cache_gpu import check_attention, dev, filled, num, sa
+import cache_f64 as F
+from test_cache_gpu import check_attention, dev, filled, fresh, num, sa
 
 pytestmark = pytest.mark.gpu
 INVALID = 1
@@ -62,3 +63,28 @@ def test_indices_past_32_bits(cuda):
     lists = torch.tensor([0, 1 << 32], device="cuda").repeat(1, 1, H, 1)
     o = sa().cache_attention(q, cache, tab, dev([n]), pages=lists)
     check_attention(o, q, seqs, [n], P, 1.0, d ** -0.5, np.zeros((1, 1, H, 1), np.int32))
+
+
+@pytest.mark.parametrize("d,P", [(32, 16), (64, 32), (96, 64), (128, 128)])
+@pytest.mark.parametrize("rows", [1, 12, 64])
+@pytest.mark.parametrize("bits", [8.3, 11.3, 13.7])
+def test_small_weights_of_large_values(cuda, d, P, rows, bits):
+    """A key whose values are 0, and one of 2^-bits of its weight with values up to 60000: the second's alone are the
+    output.  Tolerance: the output's rounding (2^-8) and the weight's to 11 bits (2^-11 twice, for that and its
+    product with the scale's rest), and scores off by 2^-20 of themselves (2^-16)."""
+    n = rows + 1                                              # every row sees both keys; later ones are far below
+    K = torch.zeros(1, n, 1, d)
+    K[:, 0] = 1.0
+    K[:, 2:] = -8.0
+    V = torch.zeros(1, n, 1, d)
+    V[:, 1] = 60000.0 * (2.0 * torch.rand(d, generator=torch.Generator().manual_seed(1)) - 1.0)
+    V[0, 1, 0, ::32] = 60000.0
+    V[0, 1, 0, 1::32] = -60000.0
+    cache, table = fresh(1, [n], 1, d, P)
+    sa().cache_write(K.cuda(), V.cuda(), cache, dev(table), dev([0]))
+    v = F.decode(cache.pool.cpu().numpy(), d, P)[1][table[0, 0], 0, 1]
+    q = torch.ones(1, rows, 1, d, device="cuda").bfloat16()
+    o = num(sa().cache_attention(q, cache, dev(table), dev([n]), sm_scale=bits * float(np.log(2.0)) / d))
+    want = v / (1.0 + 2.0 ** bits)
+    tol = 2.0 ** -8 + 2.0 ** -10 + 2.0 ** -16
+    assert (np.abs(o[0, :, 0] - want) <= tol * np.abs(want) + 2.0 ** -20 * 60000.0 * 2.0 ** -bits).all()
