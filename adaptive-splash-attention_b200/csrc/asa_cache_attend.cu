@@ -17,15 +17,15 @@
 //
 // What it reads bounds it: 1.25 d bytes a token and key head, against 4 d operations
 // a query head.  Two sequences of 131072 tokens, 4 key heads of 8 query heads, d 128
-// (168 MB) take 52 us with the join, 3.2 TB/s: 33 us of that go by the tokens, 5.0 TB/s
-// or 0.78 of a copy's rate, the rest is starting, the warps' and the runs' joins.  A tile
+// (168 MB) take 53 us with the join, 3.2 TB/s: 36 us of that go by the tokens (65536 more
+// of each 18.0), 4.7 TB/s or 0.72 of a copy's rate, the rest is starting, the warps' and the runs' joins.  A tile
 // is some 1.6 us of a warp, most of it waiting on its own chain (codes, products,
 // maxima, weights, products); 16 warps an SM at 128 registers each cover that, and
 // keeping the next tile's products in registers as well was slower (it spilled).
 // Below a few thousand tokens the chain itself is what is left: 8 us for 100 tokens.
 // Entmax, 8 sequences of 32768, 8 key heads: scores 44 us (168 MB of keys in, 34 MB of
-// scores out), thresholds 14, values 18 of which most is finding the few tiles
-// that have weight.
+// scores out), thresholds 14, values 19 of which most is finding the few tiles
+// that have weight: 76 in all; at alpha 2 82, 3 86, 1.25 (much support) 239.
 //
 // Arithmetic.  A code 0..15 in an fp16 half is the subnormal n * 2^-24, and in
 // the next nibble n * 2^-20: masking a word gives tensor-core operands without
@@ -46,7 +46,7 @@
 // clear of fp16's subnormals and large ones do not overflow: a row's largest P starts at
 // 2^4 (2^(4 - e) for e below 0, and less from e = 8 on) and may grow until P times the scales
 // reach 2^15.5 before its reference is moved.  So P keeps its 11 bits down to 2^-18 of the
-// largest weight, and 2^-13 at the largest scales.  Sums, maxima and accumulators are fp32.
+// largest weight, and 2^-12 at the largest scales.  Sums, maxima and accumulators are fp32.
 #include "asa_cache_attend.cuh"
 
 namespace asa {
@@ -58,9 +58,9 @@ constexpr int kStages = 2;            // tiles a warp has in flight
 constexpr uint32_t kUp15 = 0x78007800u, kUp11 = 0x68006800u;   // fp16 pairs: 2^15, 2^11
 constexpr int kLeast = -8;            // weights are raised for small scales by 2^8 at most
 constexpr float kRoom = 3.0f;         // log2 of what a row's largest weight may grow by, at least, before its reference moves
-// Plan::item_cost.  Measured: 48 ragged sequences of up to 8192 tokens 57.7 us with 8, 50.8 with
-// 12, 48.8 with 16, 49.1 with 20, 52.1 with 28; 12 of up to 16384 42.8, 36.8, 35.6, 35.6, 36.3;
-// listed pages (items of one size) 41.8 with 8, 44.8 with 12, 46.2 with 4.
+// Plan::item_cost.  Measured: 48 ragged sequences of up to 8192 tokens 58.5 us with 8, 51.3 with
+// 12, 49.3 with 16, 49.8 with 20, 52.5 with 28; 12 of up to 16384 43.6, 37.1, 35.8, 35.9, 36.6;
+// listed pages (items of one size) 41.8 with 8, 44.8 with 12, 46.2 with 4 where they are cut.
 constexpr int kItemCost = 16, kListedCost = 8;
 constexpr int kSegments = 32;         // segments a CTA lines up at a time
 
@@ -1223,9 +1223,9 @@ constexpr int ctas_of(int nt) { return nt == 1 ? 2 : 3; }        // an SM holds
 // Row tiles (of 8) that a CTA takes at once.  Two share the reading and unpacking of the
 // codes, which pays where the tiles keep all warps busy: nine or more a warp, by
 // the rows that fill them.  Us with one and with two: 64 sequences of 1024 tokens, 8
-// key heads of 16 rows, head size 64, 53.1 and 37.6; 8 of 8192, 32 rows, 57.1 and 45.6; 32
-// of 4096, 16 rows, head size 128, 94.0 and 88.5.  With fewer the smaller grain wins:
-// 8 of 4096, 12 rows, 28.9 and 38.1; 1 of 4096, 13.7 and 19.2.
+// key heads of 16 rows, head size 64, 53.7 and 38.5; 8 of 8192, 32 rows, 60.6 and 46.3; 32
+// of 4096, 16 rows, head size 128, 98.6 and 94.8.  With fewer the smaller grain wins:
+// 8 of 4096, 12 rows, 30.2 and 39.7; 1 of 4096, 14.1 and 19.7.
 int row_tiles(const Shape& s, int keep) {
     const int64_t rows = keep ? s.G : (int64_t)s.T * s.G, blocks = (int64_t)(keep ? keep : s.width) * (s.P / kBlock);
     const int64_t tiles = (int64_t)(keep ? s.B * s.T : s.B) * s.H * ((blocks + kTile - 1) / kTile);
@@ -1249,9 +1249,9 @@ Plan make_plan(const Shape& s, int keep) {
     // are cut where that takes fewer rounds, lengths taken to be three quarters of
     // what the table holds.  Head size 128, 8 key heads of 4 query heads, us by CTA, by
     // cluster of the size taken, and by runs:
-    //    1 sequence   of   512 tokens  9.2,  9.2, 13.5;  4096  30.3, 11.4, 14.4;  16384  101.6, 20.8, 18.1
-    //    8 sequences  of  1024 tokens 12.8, 11.2, 16.5;  4096  31.8, 20.5, 25.1;  32768  202.0, 85.1, 82.5
-    //   64 sequences  of  1024 tokens 34.9, -, 41.4;     4096  89.7, -, 92.2;      8192  162.2, -, 154.9
+    //    1 sequence   of   512 tokens  9.4,  9.2, 12.3;  4096  32.4, 11.5, 14.0;  16384  111.2, 21.5, 16.9
+    //    8 sequences  of  1024 tokens 13.1, 11.3, 16.7;  4096  33.5, 21.2, 24.5;  32768  219.6, 90.2, 85.9
+    //   64 sequences  of  1024 tokens 36.1, -, 41.3;     4096  94.8, -, 95.6;      8192  172.1, -, 163.2
     const auto ceil_div = [](int64_t x, int64_t y) { return (x + y - 1) / y; };
     p.cluster = 1;
     while (p.cluster < 8 && items * 2 * p.cluster <= slots && p.cap > p.cluster * warps) p.cluster *= 2;
@@ -1260,8 +1260,8 @@ Plan make_plan(const Shape& s, int keep) {
     p.split = items < 8 * slots && whole > runs;      // (many items even out, and runs count them all)
     // The values of an entmax row are those of few tiles: taken to be a quarter at most,
     // items that fill the SMs at once are left whole more often, and need no join (with
-    // all three kernels, 8 sequences of 32768 tokens, 8 key heads, 74.2 us, 77.5 with the
-    // values cut as the scores; 32 of 4096 73.5, 76.4; but 1 of 32768, 64 CTAs, 77.2, 75.8).
+    // all three kernels, 8 sequences of 32768 tokens, 8 key heads, 75.5 us, 79.2 with the
+    // values cut as the scores; 32 of 4096 74.9, 78.1; but 1 of 32768, 64 CTAs, 77.2, 75.8).
     const bool fill = items * p.cluster <= slots && 2 * items * p.cluster > slots;
     p.values = p.split && s.alpha != 1.0f && fill && whole <= 4 * runs ? p.cluster : 0;
     if (p.split) p.cluster = 1;

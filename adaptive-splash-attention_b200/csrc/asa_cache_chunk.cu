@@ -14,17 +14,17 @@
 //
 // fp16 is chosen for all operands.  A key is (c + n s) + (z - c), c = -7.5 s: the first
 // part, of the size of its group's spread, rounds to fp16's 11 bits (bf16 would keep 8),
-// a 500th of a code's step at most; the second enters as a product of its own, z and c with
+// a 270th of a code's step at most; the second enters as a product of its own, z and c with
 // the group sums of q in two fp16 halves each, so that an offset far above the
 // scale takes no bits from the codes.  A value is z + n s, rounded once to 11 bits: that
 // error is weighted as the value is, and lies below the output's.  P keeps 11 bits
-// as well.  A row's reference moves only
-// when a weight outgrows it (kTop, kMost); O in tensor memory is then rescaled by the
+// as well, of weights down to 2^-14 of its row's reference.  A row's reference moves only
+// when a weight outgrows it (kMost); O in tensor memory is then rescaled by the
 // rows' own warps.
 //
 // Measured, 32 heads over 8 key heads, 8192 tokens, d 128: 512 query tokens (66.6 GFLOP)
-// 122 us, 545 TFLOP/s; of 4 sequences 461 us, 578 (0.35 of cuBLAS); d 64, 2048 tokens
-// (120 GFLOP) 361 us, 333.  A tile takes 1.7 us, of which the products are 0.75: the
+// 122 us, 546 TFLOP/s; of 4 sequences 485 us, 549 (0.33 of cuBLAS); d 64, 2048 tokens
+// (120 GFLOP) 366 us, 329.  A tile takes 1.8 us, of which the products are 0.8: the
 // exponentials and the conversion of codes, which do not depend on d and on the rows
 // respectively, take the SM's other issue slots.  Starting and ending an item is some 10 us.
 //
@@ -700,9 +700,9 @@ Plan chunk_plan(const Shape& s) {
     const int64_t items = (int64_t)p.U * p.tiles * s.H;
     // Items are left whole, or cut into equal runs, whose parts' way through memory
     // costs as much as about nine tiles and one to each twenty items.  Head size 128, 8 key
-    // heads of 4 query heads, us whole and cut: 128 tokens behind 384 17.9, 24.1, behind
-    // 3968 66.0, 34.4; 512 tokens behind 3584 67.0, 85.9, behind 32256 456, 421; 640
-    // tokens (160 items to 148 SMs) behind 7552 238.5, 160.8.
+    // heads of 4 query heads, us whole and cut: 128 tokens behind 384 18.4, 24.6, behind
+    // 3968 65.8, 35.8; 512 tokens behind 3584 67.6, 91.3, behind 32256 454, 428; 640
+    // tokens (160 items to 148 SMs) behind 7552 236.8, 168.4.
     const int64_t whole = (items + kSms - 1) / kSms * p.cap, runs = items * p.cap / kSms + 9 + items / 20;
     p.split = items < 8 * kSms && whole > runs;
     p.least = kChunkCost + 2;
@@ -744,9 +744,9 @@ cudaError_t chunk_as(const Args& a, cudaStream_t st) {
 }  // namespace
 
 // Rows enough for a 128-row tile a key head to pay.  Us here and on mma.sync (asa_cache_attend.cu),
-// 8 key heads: 8 sequences of 4096 tokens, d 128, 16 rows 51.0, 38.7, 32 rows 52.9, 53.5, 64 rows
-// 55.7, 88.1, 128 rows 63.4, 155.4; d 64, 32 rows 40.2, 31.0, 64 rows 41.8, 50.1; one
-// sequence of 4096, 64 rows 26.5, 25.0, 128 rows 28.7, 37.3.
+// 8 key heads: 8 sequences of 4096 tokens, d 128, 16 rows 48.9, 30.6, 32 rows 50.2, 54.2, 64 rows
+// 52.3, 91.4, 128 rows 59.1, 160.5; d 64, 32 rows 37.2, 30.3, 64 rows 37.6, 49.6; one
+// sequence of 4096, whose few items clusters share, 64 rows 28.2, 19.6, 128 rows 30.4, 29.3.
 bool chunk_takes(const Shape& s, int keep) {
     return keep == 0 && s.alpha == 1.0f && (s.d == 64 || s.d == 128) && (int64_t)s.T * s.G >= 64;
 }

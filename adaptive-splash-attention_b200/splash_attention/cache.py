@@ -12,8 +12,9 @@ carry no gradients.  The reference has no counterpart.
 
 Index tensors (block tables, lengths, starts, counts, page lists) are int32 on
 the cache's device; other integer types are converted.  Positions past the
-block table and page ids outside the pool are neither read nor written, and
-record an error that ``device_error()`` reads.
+block table and page ids outside the pool (whole numbers that int32 does not hold
+among them) are neither read nor written, and record an error that
+``device_error()`` reads; the training operators do not see it.
 """
 from typing import NamedTuple
 
@@ -79,7 +80,8 @@ def cache_read(cache, block_table, start, T, count=None, *, dtype=torch.bfloat16
 
 def cache_bounds(cache, pages):
     """The bounds of the pool's pages ``pages`` [n] as values: (upper, lower)
-    float32 [n, kv_heads, head_dim], no channel's keys above or below them."""
+    float32 [n, kv_heads, head_dim], no channel's keys, as they were given, above or
+    below them (what is read back has been rounded, and may lie outside)."""
     return _cache_bounds(cache.bounds, pages)
 
 
@@ -88,8 +90,9 @@ def select_pages(q, cache, block_table, lengths, keep):
     [B, T, kv_heads, keep], ascending places in the block table row, -1 behind
     the last.  q: [B, T, heads, head_dim] bfloat16; query t of sequence b stands
     at position lengths[b] - T + t.  Its own page is always among them; the others
-    score highest by an upper bound of q.k from their bounds, the largest over the
-    heads that share the key head, ties to the earlier page."""
+    score highest by an upper bound of q.k from their bounds, q rounded to 8 bits (so a
+    page may score a little below its best key), the largest over the heads that
+    share the key head, ties to the earlier page."""
     return _cache_select(q, cache.pool, cache.bounds, block_table, lengths, keep)
 
 
@@ -104,7 +107,9 @@ def cache_attention(q, cache, block_table, lengths, *, sm_scale=None, alpha=1.0,
     ``splash_attention(tau_mode="exact", ref_tile_load=False)``, scores clamped to ±10
     as in training.  ``pages`` (from ``select_pages``: no page twice) restricts each
     query to the listed pages.  A query that sees no key gives zeros, one holding a
-    NaN or an infinity NaN."""
+    NaN or an infinity NaN.  Weights are held in 11 bits; softmax over 64 and more query
+    rows a key head (T * heads / kv_heads, head_dim 64 or 128, no ``pages``) also holds
+    keys, less their group's middle, and values in 11 bits."""
     if sm_scale is None:
         sm_scale = q.shape[-1] ** -0.5
     return _cache_attention(q, cache.pool, cache.bounds, block_table, lengths, pages, sm_scale, alpha)

@@ -223,7 +223,8 @@ int asa_stable_backward(const asa_params* p, const void* Q, const void* K, const
  *            rounded down), and the int32 exponent e of their unit 2^e, the
  *            least with max |key| <= 127 * 2^e (-126 for a page of zeros).  They
  *            start over when a page's first slot is written, and do not depend
- *            on how many calls wrote the page.  NaN counts as 0.
+ *            on how many calls wrote the page.  NaN counts as 0.  They are of
+ *            the keys as given; what is read back has been rounded to codes.
  *   block_table  int32 [B, table_width], the page of each page_size tokens
  *   start, count, lengths  int32 [B]
  *
